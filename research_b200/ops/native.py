@@ -136,6 +136,15 @@ def _declare(lib: ctypes.CDLL) -> None:
     sig("b200_decode_attn_paged", c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int,
         c_int, c_int, c_int, c_ll, c_ll, c_ll, c_int, c_float, c_int, c_ll, c_void_p, c_void_p)
     sig("b200_decode_attn_paged_splits", c_int, c_int, c_int, c_int)
+    sig("b200_q4_kv_write", c_void_p, c_void_p, c_ll, c_ll, c_ll, c_ll, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+        c_int, c_int, c_int, c_int, c_int, c_int, c_void_p)
+    sig("b200_q4_kv_read", c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int,
+        c_int, c_int, c_int, c_void_p)
+    sig("b200_q4_quantize_rows", c_void_p, c_ll, c_void_p, c_void_p, c_ll, c_int, c_void_p)
+    sig("b200_q4_dequantize_rows", c_void_p, c_void_p, c_void_p, c_ll, c_int, c_void_p)
+    sig("b200_q4_decode_attn", c_void_p, c_ll, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int,
+        c_int, c_int, c_int, c_int, c_int, c_float, c_void_p)
+    sig("b200_q4_linear", c_void_p, c_ll, c_void_p, c_void_p, c_void_p, c_ll, c_int, c_int, c_int, c_void_p)
     sig("b200_kv_append", c_void_p, c_void_p, c_ll, c_ll, c_void_p, c_void_p, c_void_p, c_ll, c_ll, c_ll, c_ll, c_int,
         c_int, c_int, c_int, c_void_p)
     sig("b200_attn_fwd", c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int,

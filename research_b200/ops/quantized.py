@@ -1,0 +1,424 @@
+"""Rows held in 4 bits: the K/V cache of a decode, attention over it, and linears with 4-bit weights.
+
+A row is cut into groups of 64 channels.  ``z`` is the least value of a group and ``s = bf16((most - least) / 15)``; a
+channel is the code ``n`` (0 to 15) nearest to ``(x - z) / s``, of two equally near ones the even one, and stands for
+``s n + z``.  A group without spread (or with one whose ``s`` is below the least normal bf16) has ``s = 0`` and reads back
+as ``z``; a group with a NaN or an infinity, or with a spread beyond fp32, reads back as NaN throughout.  Inputs count as
+bf16: wider ones are rounded to it first.
+
+:class:`Q4Rows` holds rows of ``K`` channels at the width ``W`` = 64 for ``K <= 64``, else ``K`` rounded up to a multiple of
+128 (padding has ``s = z = 0``): ``codes`` uint8 ``[..., W / 2]`` and ``affine`` bf16 ``[..., W / 64, 2]`` = ``(s, z)``, 36
+bytes for 64 channels.  Eight channels make a 32-bit word, channel ``i`` of the eight at nibble ``i // 2 + 4 * (i % 2)``;
+words of a block of 128 alternate between its two groups (word ``2 g + h``: channels ``64 h + 8 g ..``).
+
+Nothing here has a gradient: a call that would record one is refused.  On a CUDA device bf16 tensors go to the kernels of
+``csrc/quant4.cu``, ``csrc/decode_q4.cu`` and ``csrc/linear_q4.cu``; on the CPU the restatements below run, in any dtype.
+"""
+
+from __future__ import annotations
+
+import math
+from contextlib import nullcontext
+from typing import NamedTuple
+
+import torch
+import torch.nn.functional as F
+
+from research_b200.errors import KernelError
+from research_b200.ops import native
+
+GROUP = 64
+#: Rows up to which a product reads the 4-bit weights themselves; above, they are expanded once for the GEMM.
+LINEAR_ROWS = 64
+
+
+class Q4Rows(NamedTuple):
+    """Rows in 4 bits: ``codes`` uint8 ``[..., W / 2]``, ``affine`` bf16 ``[..., W / 64, 2]`` (scale, least value)."""
+
+    codes: torch.Tensor
+    affine: torch.Tensor
+
+
+def row_width(channels: int) -> int:
+    """Channels that a row of ``channels`` is stored as."""
+
+    return GROUP if channels <= GROUP else -(-channels // (2 * GROUP)) * 2 * GROUP
+
+
+def empty_rows(*shape: int, channels: int, device=None) -> Q4Rows:
+    """``Q4Rows`` of zeros: ``shape`` rows of ``channels`` channels (a cache: ``[B, pages, Hkv, page_rows]`` rows of D)."""
+
+    width = row_width(channels)
+    return Q4Rows(torch.zeros(*shape, width // 2, dtype=torch.uint8, device=device),
+                  torch.zeros(*shape, width // GROUP, 2, dtype=torch.bfloat16, device=device))
+
+
+# --------------------------------------------------------------------------------------------------
+# plain restatements
+# --------------------------------------------------------------------------------------------------
+_NIBBLE = tuple(i // 2 + 4 * (i % 2) for i in range(8))
+
+
+def quantize_rows_reference(x: torch.Tensor) -> Q4Rows:
+    channels, width = x.shape[-1], row_width(x.shape[-1])
+    groups = F.pad(x.to(torch.bfloat16), (0, width - channels)).unflatten(-1, (-1, GROUP)).double()
+    real = (torch.arange(width, device=x.device) < channels).view(-1, GROUP)
+    some = real[:, :1]
+    z = torch.where(some, groups.masked_fill(~real, math.inf).amin(-1, keepdim=True), 0.0)
+    spread = torch.where(some, groups.masked_fill(~real, -math.inf).amax(-1, keepdim=True), 0.0) - z
+    s = torch.where(spread <= torch.finfo(torch.float32).max, spread / 15.0, math.nan).to(torch.bfloat16).double()
+    s = torch.where(s < torch.finfo(torch.bfloat16).tiny, 0.0, s)
+    coded = real & (s > 0)
+    step = torch.where(s > 0, s, 1.0)
+    d = groups - z
+    k = torch.floor(d / step)
+    k = torch.where((k + 1.5) * step <= d, k + 1, torch.where((k - 0.5) * step > d, k - 1, k))
+    above = d - (k + 0.5) * step                        # exact next to 0; what d itself lost decides where it is 0
+    back = d - groups
+    lost = (groups - (d - back)) - (z + back)
+    up = (above > 0) | ((above == 0) & ((lost > 0) | ((lost == 0) & (k % 2 == 1))))
+    n = torch.where(coded, (k + up).clamp(0, 15), 0.0).to(torch.uint8)
+    pair = 2 if width > GROUP else 1
+    words = n.unflatten(-2, (-1, pair)).unflatten(-1, (8, 8)).transpose(-3, -2)
+    nibbles = words[..., [_NIBBLE.index(k) for k in range(8)]]
+    return Q4Rows((nibbles[..., 0::2] | (nibbles[..., 1::2] << 4)).flatten(-4),
+                  torch.cat([s, z], dim=-1).to(torch.bfloat16))
+
+
+def dequantize_rows_reference(rows: Q4Rows, channels: int, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    width = rows.codes.shape[-1] * 2
+    b = rows.codes.unflatten(-1, (-1, 8, 2 if width > GROUP else 1, 4))
+    nibbles = torch.stack([b & 15, b >> 4], dim=-1).flatten(-2)
+    n = nibbles[..., list(_NIBBLE)].transpose(-3, -2).flatten(-2).flatten(-3, -2)              # [..., groups, 64]
+    a = rows.affine.float()
+    return (n.float() * a[..., :1] + a[..., 1:]).flatten(-2)[..., :channels].to(dtype)
+
+
+def _pool_index(pool: Q4Rows, T: int, start: torch.Tensor | None):
+    """Page and row in it of positions ``start[b] + t``, and which of them the cache has."""
+
+    B, pages, _, page_rows, _ = pool.codes.shape
+    at = torch.arange(T, device=pool.codes.device).expand(B, T)
+    if start is not None:
+        at = at + start.to(at.device).long()[:, None]
+    inside = (at >= 0) & (at < pages * page_rows)
+    return at, inside
+
+
+def kv_write_paged_q4_reference(k, v, k_pool: Q4Rows, v_pool: Q4Rows, start=None) -> None:
+    at, inside = _pool_index(k_pool, k.shape[1], start)
+    b = torch.arange(k.shape[0], device=at.device)[:, None].expand_as(at)[inside]
+    at, page_rows = at[inside], k_pool.codes.shape[3]
+    for x, pool in ((k, k_pool), (v, v_pool)):
+        held = quantize_rows_reference(x)
+        pool.codes[b, at // page_rows, :, at % page_rows] = held.codes[inside]
+        pool.affine[b, at // page_rows, :, at % page_rows] = held.affine[inside]
+
+
+def kv_read_paged_q4_reference(k_pool: Q4Rows, v_pool: Q4Rows, rows: int, start=None, *, channels: int,
+                               dtype: torch.dtype = torch.bfloat16):
+    at, inside = _pool_index(k_pool, rows, start)
+    b = torch.arange(at.shape[0], device=at.device)[:, None].expand_as(at)
+    at, page_rows = at.clamp(0, k_pool.codes.shape[1] * k_pool.codes.shape[3] - 1), k_pool.codes.shape[3]
+    out = []
+    for pool in (k_pool, v_pool):
+        held = Q4Rows(*(t[b, at // page_rows, :, at % page_rows] for t in pool))
+        out.append(dequantize_rows_reference(held, channels, dtype).masked_fill(~inside[:, :, None, None], 0.0))
+    return tuple(out)
+
+
+def decode_attention_paged_q4_reference(q: torch.Tensor, k_pool: Q4Rows, v_pool: Q4Rows, lengths: torch.Tensor,
+                                        lo: torch.Tensor | None = None, scale: float | None = None) -> torch.Tensor:
+    B, Hq, D = q.shape
+    k, v = (dequantize_rows_reference(pool, D).permute(0, 2, 1, 3, 4).flatten(2, 3) for pool in (k_pool, v_pool))
+    Hkv = k.shape[1]
+    s = torch.einsum("bhgd,bhrd->bhgr", q.float().view(B, Hkv, Hq // Hkv, D), k) * (D ** -0.5 if scale is None else scale)
+    at = torch.arange(k.shape[2], device=q.device)
+    seen = at < lengths.long()[:, None]
+    if lo is not None:
+        seen = seen & (at >= lo.long()[:, None])
+    s = s.masked_fill(~seen[:, None, None], -math.inf)
+    none = ~seen.any(-1)
+    p = torch.softmax(s.masked_fill(none[:, None, None, None], 0.0), dim=-1)
+    # what a masked row holds counts for nothing, whatever it is; a row of probability 0 counts
+    o = torch.einsum("bhgr,bhrd->bhgd", p, v.masked_fill(~seen[:, None, :, None], 0.0))
+    return o.masked_fill(none[:, None, None, None], 0.0).reshape(B, Hq * D).to(q.dtype)
+
+
+def linear_q4_reference(x: torch.Tensor, w: Q4Rows) -> torch.Tensor:
+    return F.linear(x.float(), dequantize_rows_reference(w, x.shape[-1])).to(x.dtype)
+
+
+# --------------------------------------------------------------------------------------------------
+# argument checks
+# --------------------------------------------------------------------------------------------------
+def _records(*tensors: torch.Tensor) -> bool:
+    return torch.is_grad_enabled() and any(t.requires_grad for t in tensors)
+
+
+def _no_gradient(what: str, *tensors: torch.Tensor) -> None:
+    if _records(*tensors):
+        raise KernelError(f"{what} has no gradient: call it under torch.no_grad() or on detached tensors")
+
+
+def _same_device(what: str, first: torch.Tensor, *others: torch.Tensor | None) -> None:
+    for t in others:
+        if t is not None and t.device != first.device:
+            raise KernelError(f"{what}: all tensors have to be on {first.device}, got one on {t.device}")
+
+
+def _on(device: torch.device):
+    """Launches go to the current stream of the tensors' own device."""
+
+    return nullcontext() if device.index == torch._C._cuda_getDevice() else torch.cuda.device(device)
+
+
+def _check_rows(what: str, rows: Q4Rows, channels: int) -> None:
+    width = row_width(channels)
+    codes, affine = rows
+    if codes.dtype != torch.uint8 or affine.dtype != torch.bfloat16:
+        raise KernelError(f"{what}: 4-bit rows are uint8 codes and bf16 pairs, got {codes.dtype} and {affine.dtype}")
+    if codes.shape[-1] * 2 != width or affine.shape != (*codes.shape[:-1], width // GROUP, 2):
+        raise KernelError(f"{what}: rows of {channels} channels are codes [..., {width // 2}] with pairs [..., "
+                          f"{width // GROUP}, 2], got {tuple(codes.shape)} and {tuple(affine.shape)}")
+    if not codes.is_contiguous() or not affine.is_contiguous():
+        raise KernelError(f"{what}: codes and pairs have to be contiguous")
+    _same_device(what, codes, affine)
+
+
+def _check_pools(what: str, k_pool: Q4Rows, v_pool: Q4Rows, B: int, Hkv: int | None, D: int) -> tuple[int, int, int]:
+    for pool in (k_pool, v_pool):
+        if pool.codes.dim() != 5:
+            raise KernelError(f"{what}: a cache has codes [B, pages, Hkv, page_rows, D / 2], got {tuple(pool.codes.shape)}")
+        _check_rows(what, pool, D)
+    if k_pool.codes.shape != v_pool.codes.shape:
+        raise KernelError(f"{what}: the K and the V cache must have one shape, got {tuple(k_pool.codes.shape)} and "
+                          f"{tuple(v_pool.codes.shape)}")
+    _same_device(what, k_pool.codes, v_pool.codes)
+    if k_pool.codes.shape[0] != B or (Hkv is not None and k_pool.codes.shape[2] != Hkv):
+        raise KernelError(f"{what}: a cache {tuple(k_pool.codes.shape)} does not hold {B} sequences"
+                          + ("" if Hkv is None else f" of {Hkv} heads"))
+    _, pages, heads, page_rows, _ = k_pool.codes.shape
+    if pages * page_rows > 2 ** 31 - 1:
+        raise KernelError(f"{what}: a sequence has at most 2^31 - 1 rows, got {pages} pages of {page_rows}")
+    return pages, heads, page_rows
+
+
+def _per_sequence(what: str, name: str, t: torch.Tensor | None, B: int, like: torch.Tensor) -> torch.Tensor | None:
+    if t is None:
+        return None
+    if t.shape != (B,) or t.dtype not in (torch.int32, torch.int64):
+        raise KernelError(f"{what}: {name} is an int32 or int64 tensor [{B}], got {tuple(t.shape)} {t.dtype}")
+    _same_device(what, like, t)
+    return t.clamp(-2 ** 31, 2 ** 31 - 1).to(torch.int32) if t.dtype == torch.int64 else t.contiguous()
+
+
+def _head_dim(what: str, D: int) -> None:
+    if D not in (64, 128):
+        raise KernelError(f"{what} supports head_dim 64 and 128 on a CUDA device, got {D}")
+
+
+# --------------------------------------------------------------------------------------------------
+# whole rows
+# --------------------------------------------------------------------------------------------------
+@torch.no_grad()
+def quantize_rows_q4(x: torch.Tensor) -> Q4Rows:
+    """4-bit form of the rows of ``x [..., K]`` (for weights, once; fp32 values are rounded to bf16 first)."""
+
+    if x.dim() < 1 or x.shape[-1] < 1 or not x.is_floating_point():
+        raise KernelError(f"quantize_rows_q4 needs rows of floating point numbers, got {tuple(x.shape)} {x.dtype}")
+    if not x.is_cuda:
+        return quantize_rows_reference(x)
+    x2 = x.to(torch.bfloat16).reshape(-1, x.shape[-1])
+    if x2.stride(1) != 1:
+        x2 = x2.contiguous()
+    width = row_width(x.shape[-1])
+    codes = torch.empty(*x.shape[:-1], width // 2, dtype=torch.uint8, device=x.device)
+    affine = torch.empty(*x.shape[:-1], width // GROUP, 2, dtype=torch.bfloat16, device=x.device)
+    if x2.shape[0]:
+        with _on(x.device):
+            native._check(native.load().b200_q4_quantize_rows(
+                x2.data_ptr(), x2.stride(0), codes.data_ptr(), affine.data_ptr(), x2.shape[0], x2.shape[1],
+                native._stream()), "b200_q4_quantize_rows")
+    return Q4Rows(codes, affine)
+
+
+def dequantize_rows_q4(rows: Q4Rows, channels: int, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """Values ``[..., channels]`` of 4-bit rows, rounded once to ``dtype`` (bf16 on a CUDA device)."""
+
+    _check_rows("dequantize_rows_q4", rows, channels)
+    if not rows.codes.is_cuda:
+        return dequantize_rows_reference(rows, channels, dtype)
+    if dtype != torch.bfloat16:
+        raise KernelError(f"dequantize_rows_q4 writes bf16 on a CUDA device, got {dtype}")
+    return _expand(rows)[..., :channels]
+
+
+def _expand(rows: Q4Rows) -> torch.Tensor:
+    width = rows.codes.shape[-1] * 2
+    out = torch.empty(*rows.codes.shape[:-1], width, dtype=torch.bfloat16, device=rows.codes.device)
+    if out.numel():
+        with _on(out.device):
+            native._check(native.load().b200_q4_dequantize_rows(
+                rows.codes.data_ptr(), rows.affine.data_ptr(), out.data_ptr(), out.numel() // width, width,
+                native._stream()), "b200_q4_dequantize_rows")
+    return out
+
+
+# --------------------------------------------------------------------------------------------------
+# cache
+# --------------------------------------------------------------------------------------------------
+def _heads_apart(t: torch.Tensor) -> bool:
+    return (t.stride(3) == 1 and t.stride(2) == t.shape[3] and t.stride(1) % 8 == 0 and t.stride(0) % 8 == 0
+            and t.data_ptr() % 16 == 0)
+
+
+def kv_write_paged_q4(k: torch.Tensor, v: torch.Tensor, k_pool: Q4Rows, v_pool: Q4Rows,
+                      start: torch.Tensor | None = None) -> None:
+    """Quantise ``k`` / ``v`` ``[B, T, Hkv, D]`` into rows ``start[b] .. start[b] + T - 1`` of head-major paged caches of 4-bit
+    rows ``[B, pages, Hkv, page_rows, D]`` (``start`` int32 or int64 ``[B]``; None: rows ``0 .. T - 1``, which then have to
+    fit).  One token per sequence is ``T = 1`` with ``start`` the positions.  Rows that the cache does not have are left
+    out; all others keep what they held."""
+
+    what = "kv_write_paged_q4"
+    if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or not k.is_floating_point():
+        raise KernelError(f"{what}: k and v are [B, T, Hkv, D] of one shape and type, got {tuple(k.shape)} {k.dtype} and "
+                          f"{tuple(v.shape)} {v.dtype}")
+    B, T, Hkv, D = k.shape
+    pages, _, page_rows = _check_pools(what, k_pool, v_pool, B, Hkv, D)
+    _same_device(what, k, v, k_pool.codes)
+    start = _per_sequence(what, "start", start, B, k)
+    if start is None and T > pages * page_rows:
+        raise KernelError(f"{what}: {T} rows do not fit a cache of {pages} pages of {page_rows}")
+    _no_gradient(what, k, v)
+    if k.numel() == 0:
+        return
+    if not k.is_cuda:
+        return kv_write_paged_q4_reference(k, v, k_pool, v_pool, start)
+    _head_dim(what, D)
+    if k.dtype != torch.bfloat16:
+        raise KernelError(f"{what} quantises bf16 rows on a CUDA device, got {k.dtype}")
+    k, v = (t if _heads_apart(t) else t.contiguous() for t in (k, v))
+    with _on(k.device):
+        native._check(native.load().b200_q4_kv_write(
+            k.data_ptr(), v.data_ptr(), k.stride(1), k.stride(0), v.stride(1), v.stride(0), k_pool.codes.data_ptr(),
+            k_pool.affine.data_ptr(), v_pool.codes.data_ptr(), v_pool.affine.data_ptr(), native._ptr(start), B, T, Hkv,
+            D, pages, page_rows, native._stream()), "b200_q4_kv_write")
+
+
+def kv_read_paged_q4(k_pool: Q4Rows, v_pool: Q4Rows, rows: int, start: torch.Tensor | None = None, *,
+                     head_dim: int | None = None, dtype: torch.dtype = torch.bfloat16):
+    """Rows ``start[b] .. start[b] + rows - 1`` (None: from 0) of both caches as dense ``(k, v)`` ``[B, rows, Hkv, D]`` bf16.
+    Rows that the cache does not have read as zeros.  ``head_dim`` is D where it is not the stored width, ``dtype`` another
+    result type (both on the CPU only)."""
+
+    what = "kv_read_paged_q4"
+    D = k_pool.codes.shape[-1] * 2 if head_dim is None else head_dim
+    B = k_pool.codes.shape[0]
+    pages, Hkv, page_rows = _check_pools(what, k_pool, v_pool, B, None, D)
+    start = _per_sequence(what, "start", start, B, k_pool.codes)
+    if rows < 0:
+        raise KernelError(f"{what}: rows must not be negative, got {rows}")
+    if not k_pool.codes.is_cuda:
+        return kv_read_paged_q4_reference(k_pool, v_pool, rows, start, channels=D, dtype=dtype)
+    _head_dim(what, D)
+    if dtype != torch.bfloat16:
+        raise KernelError(f"{what} writes bf16 on a CUDA device, got {dtype}")
+    out = torch.empty(2, B, rows, Hkv, D, dtype=torch.bfloat16, device=k_pool.codes.device)
+    if out.numel() and pages * page_rows:
+        with _on(out.device):
+            native._check(native.load().b200_q4_kv_read(
+                out[0].data_ptr(), out[1].data_ptr(), k_pool.codes.data_ptr(), k_pool.affine.data_ptr(),
+                v_pool.codes.data_ptr(), v_pool.affine.data_ptr(), native._ptr(start), B, rows, Hkv, D, pages,
+                page_rows, native._stream()), "b200_q4_kv_read")
+    else:
+        out.zero_()
+    return out[0], out[1]
+
+
+def decode_attention_paged_q4(q: torch.Tensor, k_pool: Q4Rows, v_pool: Q4Rows, lengths: torch.Tensor,
+                              lo: torch.Tensor | None = None, scale: float | None = None) -> torch.Tensor:
+    """Attention of one query token per sequence, ``q [B, Hq, D]``, over rows ``lo[b] <= r < lengths[b]`` of caches of 4-bit
+    rows ``[B, pages, Hkv, page_rows, D]`` (``lengths``, ``lo`` int32 or int64 ``[B]``; rows beyond the cache do not count, a
+    sequence without a row gets zeros).  Up to 8 query heads share a K/V head.  Returns ``[B, Hq * D]`` in q's type."""
+
+    what = "decode_attention_paged_q4"
+    if q.dim() != 3 or not q.is_floating_point():
+        raise KernelError(f"{what}: q is [B, Hq, D], got {tuple(q.shape)} {q.dtype}")
+    B, Hq, D = q.shape
+    pages, Hkv, page_rows = _check_pools(what, k_pool, v_pool, B, None, D)
+    if Hkv == 0 or Hq % Hkv:
+        raise KernelError(f"{what}: {Hq} query heads do not share {Hkv} K/V heads evenly")
+    _same_device(what, q, k_pool.codes)
+    lengths, lo = _per_sequence(what, "lengths", lengths, B, q), _per_sequence(what, "lo", lo, B, q)
+    if lengths is None:
+        raise KernelError(f"{what} needs the lengths of the sequences")
+    _no_gradient(what, q)
+    if not q.is_cuda:
+        return decode_attention_paged_q4_reference(q, k_pool, v_pool, lengths, lo, scale)
+    _head_dim(what, D)
+    if q.dtype != torch.bfloat16 or Hq // Hkv > 8:
+        raise KernelError(f"{what} supports bf16 queries and up to 8 query heads to a K/V head on a CUDA device, got "
+                          f"{q.dtype}, Hq={Hq}, Hkv={Hkv}")
+    if q.stride(2) != 1 or q.stride(1) != D or q.stride(0) % 8 or q.data_ptr() % 16:
+        q = q.contiguous()
+    out = torch.empty(B, Hq * D, dtype=torch.bfloat16, device=q.device)
+    if out.numel() == 0:
+        return out
+    if pages * page_rows == 0:
+        return out.zero_()
+    with _on(q.device):
+        native._check(native.load().b200_q4_decode_attn(
+            q.data_ptr(), q.stride(0), k_pool.codes.data_ptr(), k_pool.affine.data_ptr(), v_pool.codes.data_ptr(),
+            v_pool.affine.data_ptr(), lengths.data_ptr(), native._ptr(lo), out.data_ptr(), B, Hq, Hkv, D, pages,
+            page_rows, float(D ** -0.5 if scale is None else scale), native._stream()), "b200_q4_decode_attn")
+    return out
+
+
+# --------------------------------------------------------------------------------------------------
+# linear
+# --------------------------------------------------------------------------------------------------
+def linear_q4(x: torch.Tensor, w: Q4Rows) -> torch.Tensor:
+    """``y = x W^T`` for ``x [..., K]`` and weights ``w`` of ``N`` 4-bit rows of K channels; ``y [..., N]`` in x's type.  Up to
+    64 rows of x the weights are read as they are (sums of exact products in fp32); for more they are expanded to bf16
+    once, which rounds each to 2^-8 of itself at most, and go through the GEMM."""
+
+    what = "linear_q4"
+    if x.dim() < 1 or not x.is_floating_point() or x.shape[-1] < 1:
+        raise KernelError(f"{what}: x is [..., K], got {tuple(x.shape)} {x.dtype}")
+    K = x.shape[-1]
+    if w.codes.dim() != 2:
+        raise KernelError(f"{what}: weights are [N, K] as 4-bit rows, got codes {tuple(w.codes.shape)}")
+    _check_rows(what, w, K)
+    _same_device(what, x, w.codes)
+    _no_gradient(what, x)
+    if not x.is_cuda:
+        return linear_q4_reference(x, w)
+    if x.dtype != torch.bfloat16:
+        raise KernelError(f"{what} takes bf16 rows on a CUDA device, got {x.dtype}")
+    N = w.codes.shape[0]
+    x2 = x.reshape(-1, K)
+    rows = x2.shape[0]
+    if rows == 0 or N == 0:
+        return torch.empty(*x.shape[:-1], N, dtype=x.dtype, device=x.device)
+    with _on(x.device):
+        if rows > LINEAR_ROWS:
+            return _expanded_linear(x2, w).view(*x.shape[:-1], N)
+        if x2.stride(1) != 1:
+            x2 = x2.contiguous()
+        out = torch.empty(rows, N, dtype=torch.bfloat16, device=x.device)
+        native._check(native.load().b200_q4_linear(x2.data_ptr(), x2.stride(0), w.codes.data_ptr(), w.affine.data_ptr(),
+                                                   out.data_ptr(), N, rows, N, K, native._stream()), "b200_q4_linear")
+    return out.view(*x.shape[:-1], N)
+
+
+def _expanded_linear(x: torch.Tensor, w: Q4Rows) -> torch.Tensor:
+    (rows, K), N = x.shape, w.codes.shape[0]
+    full = _expand(w)
+    if x.stride(1) != 1 or x.stride(0) % 8 or x.stride(0) < K or x.data_ptr() % 16:
+        x = F.pad(x, (0, full.shape[1] - K))            # the GEMM's rows start on 16 bytes
+    full = full[:, :x.shape[1]]
+    ld = -(-N // 8) * 8
+    out = torch.empty(rows, ld, dtype=torch.bfloat16, device=x.device)
+    native.gemm(x, full, out=out[:, :N])
+    return out if ld == N else out[:, :N].contiguous()
