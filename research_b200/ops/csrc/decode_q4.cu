@@ -12,6 +12,7 @@
 //   o       = sum_r (p_r s_r) (128 + n_r) - 136 sum_r (p_r s_r) + sum_r p_r (z_r + 8 s_r)      (centred: n - 8)
 // p s enters the second product as two bf16 parts (up to four heads: in columns 4 .. 7 of the same product, else in a
 // second one), which holds it to 2^-14; a single bf16 would cost as much as the rounding of the result does.
+#include <math.h>
 #include <math_constants.h>
 
 #include "quant4.cuh"
@@ -28,9 +29,10 @@ struct AttnParams {
   const uint8_t *k_codes, *k_affine, *v_codes, *v_affine;
   const int *lengths, *lo;
   __nv_bfloat16* out;                 // [B, Hq, D]
-  float *part_o, *part_ml;            // [B, Hq, splits, D], [B, Hq, splits, 2]: (m in log2 units, l)
-  int B, Hq, Hkv, pages, page_rows, splits;
-  float scale_log2;
+  float *part_o, *part_ml;            // [slots, G, D], [slots, G, 2]: (m in log2 units, l)
+  int B, Hq, Hkv, pages, page_rows, warps;
+  float scale_log2;                   // above zero: a negative scale changes the queries' sign
+  uint32_t q_sign;                    // of two bf16
 };
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
@@ -56,118 +58,234 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t v) {
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
   return r;
 }
-// codes p of both halves of w as bf16 128 + n
+// codes P of both halves of w as bf16 128 + n: one shift and one three-input operation (a & b) | c, whose constants are kept
+// in registers, since an instruction has room for one
 template <int P>
-__device__ __forceinline__ uint32_t coded(uint32_t w) { return ((w >> (4 * P)) & 0x000f000fu) | 0x43004300u; }
+__device__ __forceinline__ uint32_t coded(uint32_t w, uint32_t mask, uint32_t magic) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(P ? w >> (4 * P) : w), "r"(mask), "r"(magic));
+  return r;
+}
 
 constexpr uint32_t kOnes = 0x3f803f80u;
 
-// A warp works by itself on tiles of TR rows that it brings into a ring of its own in shared memory (cp.async, so pages may
-// end anywhere); the warps of a block take turns, and their states are joined at the end.
+// Rows of sequence b that count: [first, end), in tiles of TR rows from tile_lo to tile_hi (none: tile_lo = tile_hi).
+template <int TR>
+struct Span {
+  int first, end, tile_lo, tile_hi;
+  __device__ __forceinline__ Span(const AttnParams& p, int b) {
+    first = p.lo ? max(p.lo[b], 0) : 0;
+    end = min(p.lengths[b], p.pages * p.page_rows);
+    tile_lo = end > first ? first / TR : 0;
+    tile_hi = end > first ? (end + TR - 1) / TR : 0;
+  }
+  __device__ __forceinline__ int tiles() const { return tile_hi - tile_lo; }
+};
+
+// The tiles of all (sequence, K/V head) pairs in their order are dealt to the warps of the grid in equal runs, so that ragged
+// lengths leave no SM behind.  Warp i has tiles [i * share, (i + 1) * share); what it finds for pair bh goes to slot i + bh,
+// which no other run and pair have (in that order either the warp or the pair goes up from one piece to the next).
+struct Deal {
+  long long total, share;
+  __device__ __forceinline__ Deal(long long tiles, int warps) : total(tiles) {
+    // the 64-bit quotient only where there are that many tiles
+    share = tiles + warps <= 0x7fffffff ? (static_cast<int>(tiles) + warps - 1) / warps : (tiles + warps - 1) / warps;
+  }
+  __device__ __forceinline__ int run_of(long long tile) const {
+    return total <= 0x7fffffff ? static_cast<int>(tile) / static_cast<int>(share) : static_cast<int>(tile / share);
+  }
+};
+
+// Where a warp is: tile `tile` of pair (b, h).
+template <int TR>
+struct Cursor {
+  int b, h, tile, first, end, tile_lo, tile_hi;
+  __device__ __forceinline__ void load(const AttnParams& p) {
+    const Span<TR> s(p, b);
+    first = s.first, end = s.end, tile_lo = s.tile_lo, tile_hi = s.tile_hi;
+  }
+  __device__ __forceinline__ void next(const AttnParams& p) {
+    if (++tile < tile_hi) return;
+    if (++h == p.Hkv) {
+      h = 0;
+      do {
+        if (++b >= p.B) return;
+        load(p);
+      } while (tile_lo == tile_hi);
+    }
+    tile = tile_lo;
+  }
+};
+
+// A warp works by itself: it brings tiles of TR rows into a ring of its own in shared memory (cp.async, so pages may end
+// anywhere) and keeps the state of a pair's heads in registers until its run leaves the pair.
 //
 // Fragments.  Lane (g, t) = (lane / 4, lane % 4).  In the products over the channels row m of the 16 is cache row pi(m) of the
 // tile, pi(2 j) = j, pi(2 j + 1) = 7 - j (+ 8 for m >= 8): the lane's rows in the second product, whose index runs over the
 // cache rows 2 t, 2 t + 1, 2 t + 8, 2 t + 9, are then t, 7 - t, 8 + t, 15 - t, and neither product's reads from shared
 // memory meet in a bank (rows of 128 with their 16-byte chunks swapped in pairs every second pair of rows).
-template <int D, bool WIDE, int WARPS, int TR, int STAGES>
-__global__ void __launch_bounds__(WARPS * 32) decode_q4_kernel(const __grid_constant__ AttnParams p) {
+template <int D, bool WIDE, int WARPS, int TR, int STAGES, int BLOCKS>
+__global__ void __launch_bounds__(WARPS * 32, BLOCKS) decode_q4_kernel(const __grid_constant__ AttnParams p) {
   constexpr int GROUPS = D / 64, KW = D / 32, STEPS = TR / 16;
   constexpr int CODE_BYTES = D / 2, PAIR_BYTES = D / 16;
   constexpr int OFF_V = TR * CODE_BYTES, OFF_KA = 2 * OFF_V, OFF_VA = OFF_KA + TR * PAIR_BYTES;
   constexpr int SLOT = OFF_VA + TR * PAIR_BYTES;
-  static_assert(SLOT * STAGES >= (8 * D + 16) * 4, "the states of a warp go over its ring");
   extern __shared__ __align__(16) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int split = blockIdx.x % p.splits, bh = blockIdx.x / p.splits;
-  const int b = bh / p.Hkv, h = bh - b * p.Hkv, G = p.Hq / p.Hkv;
+  const int G = p.Hq / p.Hkv;
   uint8_t* ring = smem + warp * (SLOT * STAGES);
   const uint32_t ring_s = b200::smem_u32(ring);
 
-  b200::pdl_launch_dependents();
+  // the dependent (the kernel below) may read the lengths before its own wait, so it is let in after this one
   b200::pdl_wait();
-  const int capacity = p.pages * p.page_rows;
-  const int first = p.lo ? max(p.lo[b], 0) : 0;
-  const int end = min(p.lengths[b], capacity);
-  const int tile_lo = first / TR, tile_hi = end > first ? (end + TR - 1) / TR : tile_lo;
-  const int per = (tile_hi - tile_lo + p.splits - 1) / p.splits;
-  const int t_begin = tile_lo + split * per, t_end = min(t_begin + per, tile_hi);
-  const bool whole = p.page_rows % TR == 0;    // a tile never leaves its page
-
-  auto fill = [&](int tile, int slot) {
-    if (tile < t_end) {
-      const uint32_t dst = ring_s + slot * SLOT;
-      const int r0 = tile * TR;
-      const int pg0 = r0 / p.page_rows, in0 = r0 - pg0 * p.page_rows;
-      auto pool_row = [&](int j) {    // of row r0 + j
-        int pg = pg0, in = in0 + j;
-        if (!whole) {
-          pg = (r0 + j) / p.page_rows;
-          in = r0 + j - pg * p.page_rows;
-        }
-        return ((static_cast<long long>(b) * p.pages + pg) * p.Hkv + h) * p.page_rows + in;
-      };
-      constexpr int CHUNKS = CODE_BYTES / 16, ROWS = 32 / CHUNKS;
-      const int c = lane % CHUNKS;
+  b200::pdl_launch_dependents();
+  // neighbouring runs go to different blocks, so that few tiles spread over the SMs
+  const int run = warp * gridDim.x + blockIdx.x;
+  const Span<TR> near(p, min(lane, p.B - 1));
+  long long tiles = lane < p.B ? near.tiles() : 0;
+  for (int b = lane + 32; b < p.B; b += 32) tiles += Span<TR>(p, b).tiles();
 #pragma unroll
-      for (int j0 = 0; j0 < TR; j0 += ROWS) {
-        const int j = j0 + lane / CHUNKS;
-        if (r0 + j >= first && r0 + j < end) {
-          const long long src = pool_row(j) * CODE_BYTES + c * 16;
-          const uint32_t to = dst + j * CODE_BYTES + ((D == 128 ? c ^ (j & 2) : c) * 16);
-          cp_async16(to, p.k_codes + src);
-          cp_async16(to + OFF_V, p.v_codes + src);
+  for (int off = 16; off > 0; off >>= 1) tiles += __shfl_xor_sync(0xffffffffu, tiles, off);
+  const Deal deal(tiles * p.Hkv, p.warps);
+  const long long begin = run * deal.share;
+  if (run >= p.warps || begin >= deal.total) return;
+  const int count = static_cast<int>(min(deal.share, deal.total - begin));
+  Cursor<TR> at;
+  {
+    long long before = 0;     // tiles of one head of the sequences before the 32 looked at
+    for (int b0 = 0;; b0 += 32) {
+      const Span<TR> span = b0 ? Span<TR>(p, min(b0 + lane, p.B - 1)) : near;
+      const int n = b0 + lane < p.B ? span.tiles() : 0;
+      long long sum = n;
+#pragma unroll
+      for (int off = 1; off < 32; off <<= 1) {
+        const long long up = __shfl_up_sync(0xffffffffu, sum, off);
+        if (lane >= off) sum += up;
+      }
+      const unsigned past = __ballot_sync(0xffffffffu, (before + sum) * p.Hkv > begin);
+      if (past) {             // always in the last 32 at the latest: begin is below the total
+        const int which = __ffs(past) - 1;
+        const long long rest = begin - (before + __shfl_sync(0xffffffffu, sum - n, which)) * p.Hkv;
+        at.b = b0 + which;
+        at.first = __shfl_sync(0xffffffffu, span.first, which);
+        at.end = __shfl_sync(0xffffffffu, span.end, which);
+        at.tile_lo = __shfl_sync(0xffffffffu, span.tile_lo, which);
+        at.tile_hi = __shfl_sync(0xffffffffu, span.tile_hi, which);
+        const int per_head = at.tile_hi - at.tile_lo;
+        at.h = static_cast<int>(rest / per_head);
+        at.tile = at.tile_lo + static_cast<int>(rest - static_cast<long long>(at.h) * per_head);
+        break;
+      }
+      before += __shfl_sync(0xffffffffu, sum, 31);
+    }
+  }
+  const bool whole = p.page_rows % TR == 0;    // a tile never leaves its page: its rows are contiguous, and all there
+
+  auto fill = [&](const Cursor<TR>& c, int slot) {
+    const uint32_t dst = ring_s + slot * SLOT;
+    const int r0 = c.tile * TR;
+    constexpr int CHUNKS = CODE_BYTES / 16, ROWS = 32 / CHUNKS;
+    const int chunk = lane % CHUNKS, row = lane / CHUNKS;      // of the first copy; the next ones are ROWS rows further
+    const uint32_t to = dst + row * CODE_BYTES + ((D == 128 ? chunk ^ (row & 2) : chunk) * 16);
+    if (whole) {
+      const int pg = r0 / p.page_rows;
+      const long long r = ((static_cast<long long>(c.b) * p.pages + pg) * p.Hkv + c.h) * p.page_rows + (r0 - pg * p.page_rows);
+      const uint8_t *k = p.k_codes + r * CODE_BYTES + lane * 16, *v = p.v_codes + r * CODE_BYTES + lane * 16;
+#pragma unroll
+      for (int j = 0; j < TR / ROWS; ++j) {
+        cp_async16(to + j * 512, k + j * 512);
+        cp_async16(to + OFF_V + j * 512, v + j * 512);
+      }
+      const uint8_t *ka = p.k_affine + (r + lane) * PAIR_BYTES, *va = p.v_affine + (r + lane) * PAIR_BYTES;
+#pragma unroll
+      for (int j = 0; j < TR; j += 32) {
+        cp_async_small<PAIR_BYTES>(dst + OFF_KA + (j + lane) * PAIR_BYTES, ka + j * PAIR_BYTES);
+        cp_async_small<PAIR_BYTES>(dst + OFF_VA + (j + lane) * PAIR_BYTES, va + j * PAIR_BYTES);
+      }
+    } else {
+      auto pool_row = [&](int r) {
+        const int pg = r / p.page_rows;
+        return ((static_cast<long long>(c.b) * p.pages + pg) * p.Hkv + c.h) * p.page_rows + (r - pg * p.page_rows);
+      };
+#pragma unroll 2
+      for (int j = 0; j < TR / ROWS; ++j) {
+        const int r = r0 + row + j * ROWS;
+        if (r >= c.first && r < c.end) {
+          const long long src = pool_row(r) * CODE_BYTES + chunk * 16;
+          cp_async16(to + j * 512, p.k_codes + src);
+          cp_async16(to + OFF_V + j * 512, p.v_codes + src);
         }
       }
 #pragma unroll
-      for (int j0 = 0; j0 < TR; j0 += 32) {
-        const int j = j0 + lane;
-        if (j < TR && r0 + j >= first && r0 + j < end) {
-          const long long src = pool_row(j) * PAIR_BYTES;
+      for (int j = lane; j < TR; j += 32) {
+        const int r = r0 + j;
+        if (r >= c.first && r < c.end) {
+          const long long src = pool_row(r) * PAIR_BYTES;
           cp_async_small<PAIR_BYTES>(dst + OFF_KA + j * PAIR_BYTES, p.k_affine + src);
           cp_async_small<PAIR_BYTES>(dst + OFF_VA + j * PAIR_BYTES, p.v_affine + src);
         }
       }
     }
-    cp_async_commit();
   };
+  Cursor<TR> ahead = at;
 #pragma unroll
-  for (int i = 0; i < STAGES - 1; ++i) fill(t_begin + warp + i * WARPS, i);
-
-  // queries: column g of the first product is head g (WIDE) or g % 4, whose second copy gives the low parts of p s
-  uint32_t qf[KW][4];
-  float qsum[GROUPS][2] = {};
-  {
-    const int hq = WIDE ? g : (g & 3);
-#pragma unroll
-    for (int j = 0; j < KW; ++j) {
-      const int c = D == 128 ? 64 * (j & 1) + 16 * t + 8 * (j >> 1) : 16 * t + 8 * j;
-      uint4 v = make_uint4(0, 0, 0, 0);
-      if (hq < G) v = *reinterpret_cast<const uint4*>(p.q + b * p.q_batch + static_cast<long long>(h * G + hq) * D + c);
-      qf[j][0] = v.x, qf[j][1] = v.y, qf[j][2] = v.z, qf[j][3] = v.w;
+  for (int i = 0; i < STAGES - 1; ++i) {
+    if (i < count) {
+      fill(ahead, i);
+      ahead.next(p);
     }
-#pragma unroll
-    for (int gr = 0; gr < GROUPS; ++gr) {
-      float c[4] = {};
-#pragma unroll
-      for (int j = 0; j < KW; ++j)
-        if (GROUPS == 1 || (j & 1) == gr) {
-          mma(c, kOnes, kOnes, kOnes, kOnes, qf[j][0], qf[j][1]);
-          mma(c, kOnes, kOnes, kOnes, kOnes, qf[j][2], qf[j][3]);
-        }
-      qsum[gr][0] = c[0], qsum[gr][1] = c[1];
-    }
+    cp_async_commit();
   }
 
+  uint32_t mask = 0x000f000fu, magic = 0x43004300u;
+  asm volatile("" : "+r"(mask), "+r"(magic));
   const int pi = (g & 1) ? 7 - (g >> 1) : g >> 1;
   const float low = (!WIDE && t >= 2) ? 1.f : 0.f;
-  float o[GROUPS * 4][4] = {}, zacc[GROUPS][2] = {}, m[2] = {-CUDART_INF_F, -CUDART_INF_F}, l[2] = {};
-  int i = 0;
-  for (int tile = t_begin + warp; tile < t_end; tile += WARPS, ++i) {
+  uint32_t qf[KW][4];
+  float qsum[GROUPS][2];
+  float o[GROUPS * 4][4], zacc[GROUPS][2], m[2], l[2];
+  bool fresh = true;
+  for (int i = 0; i < count; ++i) {
+    if (fresh) {
+      // queries: column g of the first product is head g (WIDE) or g % 4, whose second copy gives the low parts of p s
+      fresh = false;
+      const int hq = WIDE ? g : (g & 3);
+#pragma unroll
+      for (int j = 0; j < KW; ++j) {
+        const int c = D == 128 ? 64 * (j & 1) + 16 * t + 8 * (j >> 1) : 16 * t + 8 * j;
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (hq < G)
+          v = *reinterpret_cast<const uint4*>(p.q + at.b * p.q_batch + static_cast<long long>(at.h * G + hq) * D + c);
+        qf[j][0] = v.x ^ p.q_sign, qf[j][1] = v.y ^ p.q_sign, qf[j][2] = v.z ^ p.q_sign, qf[j][3] = v.w ^ p.q_sign;
+      }
+#pragma unroll
+      for (int gr = 0; gr < GROUPS; ++gr) {
+        float c[4] = {};
+#pragma unroll
+        for (int j = 0; j < KW; ++j)
+          if (GROUPS == 1 || (j & 1) == gr) {
+            mma(c, kOnes, kOnes, kOnes, kOnes, qf[j][0], qf[j][1]);
+            mma(c, kOnes, kOnes, kOnes, kOnes, qf[j][2], qf[j][3]);
+          }
+        qsum[gr][0] = c[0], qsum[gr][1] = c[1];
+        zacc[gr][0] = zacc[gr][1] = 0.f;
+      }
+#pragma unroll
+      for (int v = 0; v < GROUPS * 4; ++v)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[v][e] = 0.f;
+      m[0] = m[1] = -CUDART_INF_F;
+      l[0] = l[1] = 0.f;
+    }
     cp_async_wait<STAGES - 2>();
     __syncwarp();
-    fill(tile + (STAGES - 1) * WARPS, (i + STAGES - 1) % STAGES);
+    if (i + STAGES - 1 < count) {
+      fill(ahead, (i + STAGES - 1) % STAGES);
+      ahead.next(p);
+    }
+    cp_async_commit();
     const uint8_t* slot = ring + (i % STAGES) * SLOT;
-    const int r0 = tile * TR;
+    const int r0 = at.tile * TR, first = at.first, end = at.end;
     const bool edge = r0 < first || r0 + TR > end;
 
     float sc[STEPS][4];
@@ -194,22 +312,22 @@ __global__ void __launch_bounds__(WARPS * 32) decode_q4_kernel(const __grid_cons
 #pragma unroll
       for (int gr = 0; gr < GROUPS; ++gr)
 #pragma unroll
-        for (int c = 0; c < 4; ++c) acc[gr][c] = -128.f * qsum[gr][c & 1];
+        for (int c = 0; c < 4; ++c) acc[gr][c] = 0.f;
 #pragma unroll
       for (int j = 0; j < KW; ++j) {
         float(&a)[4] = acc[GROUPS == 1 ? 0 : (j & 1)];
-        mma(a, coded<0>(ka[j]), coded<0>(kb[j]), coded<1>(ka[j]), coded<1>(kb[j]), qf[j][0], qf[j][1]);
-        mma(a, coded<2>(ka[j]), coded<2>(kb[j]), coded<3>(ka[j]), coded<3>(kb[j]), qf[j][2], qf[j][3]);
+        mma(a, coded<0>(ka[j], mask, magic), coded<0>(kb[j], mask, magic), coded<1>(ka[j], mask, magic), coded<1>(kb[j], mask, magic), qf[j][0], qf[j][1]);
+        mma(a, coded<2>(ka[j], mask, magic), coded<2>(kb[j], mask, magic), coded<3>(ka[j], mask, magic), coded<3>(kb[j], mask, magic), qf[j][2], qf[j][3]);
       }
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        float s = 0.f;
+      for (int c = 0; c < 4; ++c) sc[mt][c] = 0.f;
 #pragma unroll
-        for (int gr = 0; gr < GROUPS; ++gr) {
-          const uint32_t a = c < 2 ? aa[gr] : ab[gr];
-          s = fmaf(scale_of(a), acc[gr][c], fmaf(least_of(a), qsum[gr][c & 1], s));
-        }
-        sc[mt][c] = s * p.scale_log2;
+      for (int gr = 0; gr < GROUPS; ++gr) {
+        const float sa = scale_of(aa[gr]), sb = scale_of(ab[gr]);
+        const float za = fmaf(-128.f, sa, least_of(aa[gr])), zb = fmaf(-128.f, sb, least_of(ab[gr]));
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          sc[mt][c] = fmaf(c < 2 ? sa : sb, acc[gr][c], fmaf(c < 2 ? za : zb, qsum[gr][c & 1], sc[mt][c]));
       }
       if (edge) {
         const bool seen_a = r0 + ja >= first && r0 + ja < end, seen_b = r0 + jb >= first && r0 + jb < end;
@@ -227,14 +345,14 @@ __global__ void __launch_bounds__(WARPS * 32) decode_q4_kernel(const __grid_cons
       for (int mt = 0; mt < STEPS; ++mt) mx = fmaxf(mx, fmaxf(sc[mt][e], sc[mt][e + 2]));
 #pragma unroll
       for (int off = 4; off < 32; off <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
-      const float use = mx == -CUDART_INF_F ? 0.f : mx;
-      alpha[e] = b200::ex2_approx(m[e] - use);
+      const float use = mx == -CUDART_INF_F ? 0.f : mx * p.scale_log2;
+      alpha[e] = b200::ex2_approx(fmaf(m[e], p.scale_log2, -use));
       m[e] = mx;
       float sum = 0.f;
 #pragma unroll
       for (int mt = 0; mt < STEPS; ++mt) {
-        sc[mt][e] = b200::ex2_approx(sc[mt][e] - use);
-        sc[mt][e + 2] = b200::ex2_approx(sc[mt][e + 2] - use);
+        sc[mt][e] = b200::ex2_approx(fmaf(sc[mt][e], p.scale_log2, -use));
+        sc[mt][e + 2] = b200::ex2_approx(fmaf(sc[mt][e + 2], p.scale_log2, -use));
         sum += sc[mt][e] + sc[mt][e + 2];
       }
       l[e] = fmaf(l[e], alpha[e], sum);
@@ -325,139 +443,185 @@ __global__ void __launch_bounds__(WARPS * 32) decode_q4_kernel(const __grid_cons
           mma(c, x0, x1, x2, x3, bh_[gr][mt][0], bh_[gr][mt][1]);
           if constexpr (WIDE) mma(c, x0, x1, x2, x3, bl_[gr][mt][0], bl_[gr][mt][1]);
         };
-        step(acc[gr * 4 + 0], coded<0>(a0), coded<0>(a1), coded<0>(a2), coded<0>(a3));
-        step(acc[gr * 4 + 1], coded<1>(a0), coded<1>(a1), coded<1>(a2), coded<1>(a3));
-        step(acc[gr * 4 + 2], coded<2>(a0), coded<2>(a1), coded<2>(a2), coded<2>(a3));
-        step(acc[gr * 4 + 3], coded<3>(a0), coded<3>(a1), coded<3>(a2), coded<3>(a3));
+        step(acc[gr * 4 + 0], coded<0>(a0, mask, magic), coded<0>(a1, mask, magic), coded<0>(a2, mask, magic), coded<0>(a3, mask, magic));
+        step(acc[gr * 4 + 1], coded<1>(a0, mask, magic), coded<1>(a1, mask, magic), coded<1>(a2, mask, magic), coded<1>(a3, mask, magic));
+        step(acc[gr * 4 + 2], coded<2>(a0, mask, magic), coded<2>(a1, mask, magic), coded<2>(a2, mask, magic), coded<2>(a3, mask, magic));
+        step(acc[gr * 4 + 3], coded<3>(a0, mask, magic), coded<3>(a1, mask, magic), coded<3>(a2, mask, magic), coded<3>(a3, mask, magic));
       }
     }
 #pragma unroll
     for (int v = 0; v < GROUPS * 4; ++v)
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[v][e] = fmaf(o[v][e], alpha[e & 1], acc[v][e]);
+
+    const int b = at.b, h = at.h;
+    fresh = i + 1 == count || at.tile + 1 == at.tile_hi;
+    at.next(p);
+    if (!fresh) continue;
+    // the run leaves the pair: its state goes to the pair's slot
+    const long long place = static_cast<long long>(run) + static_cast<long long>(b) * p.Hkv + h;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+#pragma unroll
+      for (int off = 4; off < 32; off <<= 1) {
+        l[e] += __shfl_xor_sync(0xffffffffu, l[e], off);
+#pragma unroll
+        for (int gr = 0; gr < GROUPS; ++gr) zacc[gr][e] += __shfl_xor_sync(0xffffffffu, zacc[gr][e], off);
+      }
+      const int hq = WIDE ? 2 * t + e : (2 * t + e) & 3;
+      if (g == 0 && low == 0.f && hq < G)
+        *reinterpret_cast<float2*>(p.part_ml + (place * G + hq) * 2) = make_float2(m[e] * p.scale_log2, l[e]);
+#pragma unroll
+      for (int gr = 0; gr < GROUPS; ++gr)
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+          float x = o[gr * 4 + v][e], y = o[gr * 4 + v][e + 2];
+          if constexpr (!WIDE) {      // the low parts are two lanes further
+            x += __shfl_xor_sync(0xffffffffu, x, 2);
+            y += __shfl_xor_sync(0xffffffffu, y, 2);
+          }
+          if (low == 0.f && hq < G)
+            *reinterpret_cast<float2*>(p.part_o + (place * G + hq) * D + 64 * gr + 8 * g + 2 * v) =
+                make_float2(x + zacc[gr][e], y + zacc[gr][e]);
+        }
+    }
   }
   cp_async_wait<0>();
-  __syncwarp();
+}
 
-  // the warp's state over its ring: o [8][D], m [8], l [8]
-  float* st = reinterpret_cast<float*>(ring);
+// Joins the pieces of a head: out = sum_i w_i o_i / sum_i w_i l_i, w_i = 2^(m_i - max m); a piece that met no number has
+// m = -inf and l = NaN, which counts.  The threads of a channel share the pieces.
+constexpr int kMergeThreads = 256;
+template <int D, int TR>
+__global__ void __launch_bounds__(kMergeThreads) decode_q4_merge_kernel(const __grid_constant__ AttnParams p) {
+  constexpr int PARTS = kMergeThreads / D, WARPS = kMergeThreads / 32;
+  __shared__ long long s_sum[2][WARPS];
+  __shared__ float s_max[WARPS], s_w[kMergeThreads], s_l[WARPS], s_o[PARTS][D];
+  const int b = blockIdx.x / p.Hq, hq = blockIdx.x - b * p.Hq, G = p.Hq / p.Hkv, h = hq / G;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  b200::pdl_launch_dependents();
+  long long sum[2] = {0, 0};    // tiles of one head: of all sequences, of those before b
+  for (int i = threadIdx.x; i < p.B; i += kMergeThreads) {
+    const int n = Span<TR>(p, i).tiles();
+    sum[0] += n;
+    if (i < b) sum[1] += n;
+  }
+  const int tiles = Span<TR>(p, b).tiles();
+  b200::pdl_wait();
 #pragma unroll
-  for (int e = 0; e < 2; ++e) {
+  for (int k = 0; k < 2; ++k) {
 #pragma unroll
-    for (int off = 4; off < 32; off <<= 1) {
-      l[e] += __shfl_xor_sync(0xffffffffu, l[e], off);
-#pragma unroll
-      for (int gr = 0; gr < GROUPS; ++gr) zacc[gr][e] += __shfl_xor_sync(0xffffffffu, zacc[gr][e], off);
-    }
-    if (g == 0) {
-      st[8 * D + 2 * t + e] = m[e];
-      st[8 * D + 8 + 2 * t + e] = l[e];
-    }
-#pragma unroll
-    for (int gr = 0; gr < GROUPS; ++gr) {
-      const float z = low == 0.f ? zacc[gr][e] : 0.f;
-#pragma unroll
-      for (int v = 0; v < 4; ++v)
-        *reinterpret_cast<float2*>(st + (2 * t + e) * D + 64 * gr + 8 * g + 2 * v) =
-            make_float2(o[gr * 4 + v][e] + z, o[gr * 4 + v][e + 2] + z);
-    }
+    for (int off = 16; off > 0; off >>= 1) sum[k] += __shfl_xor_sync(0xffffffffu, sum[k], off);
+    if (lane == 0) s_sum[k][warp] = sum[k];
   }
   __syncthreads();
-  for (int idx = threadIdx.x; idx < G * D; idx += WARPS * 32) {
-    const int hq = idx / D, d = idx - hq * D;
-    float mm = -CUDART_INF_F;
 #pragma unroll
-    for (int w = 0; w < WARPS; ++w) mm = fmaxf(mm, reinterpret_cast<const float*>(smem + w * (SLOT * STAGES))[8 * D + hq]);
-    float sum = 0.f, ls = 0.f;
+  for (int k = 0; k < 2; ++k) {
+    sum[k] = 0;
 #pragma unroll
-    for (int w = 0; w < WARPS; ++w) {
-      const float* s = reinterpret_cast<const float*>(smem + w * (SLOT * STAGES));
-      const float mw = s[8 * D + hq], lw = s[8 * D + 8 + hq];
-      // a warp that saw no row has l = 0; one that saw no number has m = -inf and l = NaN, which counts
-      const float wgt = mw == -CUDART_INF_F ? (lw == 0.f ? 0.f : 1.f) : b200::ex2_approx(mw - mm);
-      float v = s[hq * D + d];
-      if constexpr (!WIDE) v += s[(hq + 4) * D + d];
-      sum = fmaf(v, wgt, sum);
-      ls = fmaf(lw, wgt, ls);
+    for (int w = 0; w < WARPS; ++w) sum[k] += s_sum[k][w];
+  }
+  const int d = threadIdx.x % D, part = threadIdx.x / D;
+  __nv_bfloat16* out = p.out + (static_cast<long long>(b) * p.Hq + hq) * D + d;
+  if (tiles == 0) {
+    if (part == 0) *out = __float2bfloat16(0.f);
+    return;
+  }
+  const Deal deal(sum[0] * p.Hkv, p.warps);
+  const long long from = sum[1] * p.Hkv + static_cast<long long>(h) * tiles;
+  const int first = deal.run_of(from), pieces = deal.run_of(from + tiles - 1) - first + 1;
+  const long long place = first + static_cast<long long>(b) * p.Hkv + h;
+  const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + place * G + (hq - h * G);
+  const float* o = p.part_o + (place * G + (hq - h * G)) * D + d;
+  float mm = -CUDART_INF_F;
+  for (int i = threadIdx.x; i < pieces; i += kMergeThreads) mm = fmaxf(mm, ml[static_cast<long long>(i) * G].x);
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, off));
+  if (lane == 0) s_max[warp] = mm;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < WARPS; ++w) mm = fmaxf(mm, s_max[w]);
+  float acc = 0.f, l = 0.f;
+  for (int i0 = 0; i0 < pieces; i0 += kMergeThreads) {
+    const int n = min(pieces - i0, kMergeThreads);
+    if (threadIdx.x < n) {
+      const float2 v = ml[static_cast<long long>(i0 + threadIdx.x) * G];
+      const float w = v.x == -CUDART_INF_F ? (v.y == 0.f ? 0.f : 1.f) : b200::ex2_approx(v.x - mm);
+      s_w[threadIdx.x] = w;
+      l = fmaf(v.y, w, l);
     }
-    const long long head = static_cast<long long>(b) * p.Hq + h * G + hq;
-    if (p.splits == 1) {
-      p.out[head * D + d] = __float2bfloat16(end > first ? sum / ls : 0.f);
-    } else {
-      p.part_o[(head * p.splits + split) * D + d] = sum;
-      if (d == 0) *reinterpret_cast<float2*>(p.part_ml + (head * p.splits + split) * 2) = make_float2(mm, ls);
-    }
+    __syncthreads();
+#pragma unroll 8
+    for (int i = part; i < n; i += PARTS) acc = fmaf(o[static_cast<long long>(i0 + i) * G * D], s_w[i], acc);
+    __syncthreads();
+  }
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
+  if (lane == 0) s_l[warp] = l;
+  s_o[part][d] = acc;
+  __syncthreads();
+  if (part == 0) {
+    l = 0.f;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) l += s_l[w];
+#pragma unroll
+    for (int k = 1; k < PARTS; ++k) acc += s_o[k][d];
+    *out = __float2bfloat16(acc / l);
   }
 }
 
-// Joins the splits of a head, as above.
-template <int D>
-__global__ void __launch_bounds__(D) decode_q4_merge_kernel(const __grid_constant__ AttnParams p) {
-  const long long head = blockIdx.x;
-  const int d = threadIdx.x;
-  b200::pdl_launch_dependents();
-  b200::pdl_wait();
-  const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + head * p.splits;
-  const float* part = p.part_o + head * p.splits * D + d;
-  float mm = -CUDART_INF_F, sum = 0.f, ls = 0.f;
-  bool any = false;
-  for (int s = 0; s < p.splits; ++s) mm = fmaxf(mm, ml[s].x);
-  for (int s = 0; s < p.splits; ++s) {
-    const float2 v = ml[s];
-    const bool none = v.x == -CUDART_INF_F && v.y == 0.f;
-    const float wgt = v.x == -CUDART_INF_F ? (none ? 0.f : 1.f) : b200::ex2_approx(v.x - mm);
-    any = any || !none;
-    sum = fmaf(part[static_cast<long long>(s) * D], wgt, sum);
-    ls = fmaf(v.y, wgt, ls);
-  }
-  p.out[head * D + d] = __float2bfloat16(any ? sum / ls : 0.f);
-}
-
-constexpr int kWarps = 4, kRows = 64, kStages = 3;
+#ifndef VROWS
+#define VROWS 64
+#define VSTAGES 3
+#define VBLOCKS 2
+#endif
+constexpr int kWarps = 4, kRows = VROWS, kStages = VSTAGES, kBlocks = VBLOCKS;
 
 template <int D, bool WIDE>
 int launch(const AttnParams& p, cudaStream_t s) {
   constexpr int bytes = kWarps * kStages * kRows * (D + D / 8);
-  auto* kern = decode_q4_kernel<D, WIDE, kWarps, kRows, kStages>;
+  auto* kern = decode_q4_kernel<D, WIDE, kWarps, kRows, kStages, kBlocks>;
   static bool configured[b200host::kMaxDevices] = {};
   if (int rc = b200host::ensure_dynamic_smem(kern, bytes, configured)) return rc;
   const bool pdl = b200host::pdl_enabled() != 0;
-  if (cudaError_t e = b200host::launch_kernel(kern, dim3(p.B * p.Hkv * p.splits), dim3(kWarps * 32), bytes, s, pdl, p))
-    return static_cast<int>(e);
-  if (p.splits == 1) return 0;
-  return static_cast<int>(b200host::launch_kernel(decode_q4_merge_kernel<D>, dim3(p.B * p.Hq), dim3(D), 0, s, pdl, p));
+  // fewer runs than the device has blocks: one warp of a block each, on as many SMs
+  const int most = kBlocks * b200host::sm_count(), grid = p.warps < most ? p.warps : most;
+  if (cudaError_t e = b200host::launch_kernel(kern, dim3(grid), dim3(kWarps * 32), bytes, s, pdl, p)) return static_cast<int>(e);
+  return static_cast<int>(b200host::launch_kernel(decode_q4_merge_kernel<D, kRows>, dim3(p.B * p.Hq), dim3(kMergeThreads), 0,
+                                                  s, pdl, p));
 }
 
 }  // namespace
 
-// Parts that a sequence's rows are cut into: as many as give each SM two blocks, of at least a tile a warp.
-extern "C" int b200_q4_decode_attn_splits(int B, int Hkv, long long rows) {
-  const long long base = (long long)B * Hkv, tiles = (rows + kRows - 1) / kRows;
-  long long splits = base > 0 ? 2 * b200host::sm_count() / base : 1;
-  if (splits > (tiles + kWarps - 1) / kWarps) splits = (tiles + kWarps - 1) / kWarps;
-  if (splits > 64) splits = 64;
-  return splits < 1 ? 1 : (int)splits;
+// Runs that the rows are dealt to for a cache of `rows` rows a sequence: one per warp of a wave of blocks, or one
+// per tile where that is fewer.
+extern "C" int b200_q4_decode_attn_runs(int B, int Hkv, long long rows) {
+  const long long tiles = (rows + kRows - 1) / kRows * B * Hkv, most = (long long)kBlocks * b200host::sm_count() * kWarps;
+  return (int)(tiles < 1 ? 1 : (tiles < most ? tiles : most));
 }
 
 // q [B, Hq, D] bf16 (q_batch elements between sequences), caches [B, pages, Hkv, page_rows, ..] contiguous, lengths and lo
-// int32 [B] (lo may be null), out [B, Hq, D] bf16.  D 64 or 128, up to 8 query heads to a K/V head.  With more than one
-// split: part_o [B, Hq, splits, D] and part_ml [B, Hq, splits, 2] fp32 of the call's own.
+// int32 [B] (lo may be null), out [B, Hq, D] bf16.  D 64 or 128, up to 8 query heads to a K/V head.  `runs` from
+// b200_q4_decode_attn_runs (pages * page_rows rows); part_o and part_ml are the call's own: (runs + B * Hkv) * (Hq / Hkv) times
+// D and 2 floats.
 extern "C" int b200_q4_decode_attn(const void* q, long long q_batch, const void* k_codes, const void* k_affine,
                                    const void* v_codes, const void* v_affine, const void* lengths, const void* lo,
                                    void* out, void* part_o, void* part_ml, int B, int Hq, int Hkv, int D, int pages,
-                                   int page_rows, int splits, float scale, void* stream) {
+                                   int page_rows, int runs, float scale, void* stream) {
   if (B <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || Hq / Hkv > 8 || pages <= 0 || page_rows <= 0 || (D != 64 && D != 128) ||
-      splits < 1 || (long long)pages * page_rows > 0x7fffff00ll || (long long)B * Hq * splits > 0x7fffffffll ||
-      (splits > 1 && (!part_o || !part_ml)))
+      runs < 1 || (long long)pages * page_rows > 0x7fffff00ll || (long long)B * Hq > 0x7fffffffll || !part_o || !part_ml)
     return b200host::RC_BAD_SHAPE;
+  if (runs > kBlocks * b200host::sm_count() * kWarps) return b200host::RC_BAD_SHAPE;
   if ((q_batch & 7) || ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k_codes) |
                          reinterpret_cast<uintptr_t>(k_affine) | reinterpret_cast<uintptr_t>(v_codes) |
                          reinterpret_cast<uintptr_t>(v_affine) | reinterpret_cast<uintptr_t>(out)) & 15))
     return b200host::RC_BAD_ALIGNMENT;
   AttnParams p{(const __nv_bfloat16*)q, q_batch, (const uint8_t*)k_codes, (const uint8_t*)k_affine,
                (const uint8_t*)v_codes, (const uint8_t*)v_affine, (const int*)lengths, (const int*)lo,
-               (__nv_bfloat16*)out, (float*)part_o, (float*)part_ml, B, Hq, Hkv, pages, page_rows, splits,
-               scale * kLog2e};
+               (__nv_bfloat16*)out, (float*)part_o, (float*)part_ml, B, Hq, Hkv, pages, page_rows, runs, fabsf(scale) * kLog2e,
+               scale < 0.f ? 0x80008000u : 0u};
+  // a scale of zero weighs all rows alike, as one does that no score is large enough for; infinite scores stay none
+  if (p.scale_log2 < 1e-36f) p.scale_log2 = 1e-36f;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   const bool wide = Hq / Hkv > 4;
   if (D == 128) return wide ? launch<128, true>(p, s) : launch<128, false>(p, s);

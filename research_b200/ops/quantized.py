@@ -369,15 +369,15 @@ def decode_attention_paged_q4(q: torch.Tensor, k_pool: Q4Rows, v_pool: Q4Rows, l
         return out.zero_()
     lib = native.load()
     with _on(q.device):
-        splits = lib.b200_q4_decode_attn_splits(B, Hkv, pages * page_rows)
-        parts = torch.empty(B * Hq * splits * (D + 2), dtype=torch.float32, device=q.device) if splits > 1 else None
+        runs = lib.b200_q4_decode_attn_runs(B, Hkv, pages * page_rows)
+        slots = (runs + B * Hkv) * (Hq // Hkv)
+        parts = torch.empty(slots * (D + 2), dtype=torch.float32, device=q.device)
         native._check(lib.b200_q4_decode_attn(
             q.data_ptr(), q.stride(0), k_pool.codes.data_ptr(), k_pool.affine.data_ptr(), v_pool.codes.data_ptr(),
-            v_pool.affine.data_ptr(), lengths.data_ptr(), native._ptr(lo), out.data_ptr(), native._ptr(parts),
-            None if parts is None else parts.data_ptr() + 4 * B * Hq * splits * D, B, Hq, Hkv, D, pages, page_rows,
-            splits, float(D ** -0.5 if scale is None else scale), native._stream()), "b200_q4_decode_attn")
-    if splits > 1:
-        native.LAUNCHES += 1                            # _check counts one launch; joining the splits is the second
+            v_pool.affine.data_ptr(), lengths.data_ptr(), native._ptr(lo), out.data_ptr(), parts.data_ptr(),
+            parts.data_ptr() + 4 * slots * D, B, Hq, Hkv, D, pages, page_rows, runs,
+            float(D ** -0.5 if scale is None else scale), native._stream()), "b200_q4_decode_attn")
+    native.LAUNCHES += 1                                # _check counts one launch; joining the runs is the second
     return out
 
 
