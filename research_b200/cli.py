@@ -129,6 +129,8 @@ def build_parser() -> argparse.ArgumentParser:
     p.add_argument("--max-new-tokens", required=True, type=int)
     p.add_argument("--temperature", type=float, default=1.0)
     p.add_argument("--top-k", type=int, default=None)
+    p.add_argument("--cache-bits", type=int, default=16, choices=[4, 16])
+    p.add_argument("--weight-bits", type=int, default=16, choices=[4, 16])
     p.add_argument("--json", action="store_true")
     return parser
 
@@ -317,7 +319,8 @@ def _dispatch(args: argparse.Namespace) -> int:
         from research_b200.runtime.sampling import sample_checkpoint
 
         row = sample_checkpoint(args.run_dir, args.checkpoint, prompt_ids=args.prompt_ids,
-                                max_new_tokens=args.max_new_tokens, temperature=args.temperature, top_k=args.top_k)
+                                max_new_tokens=args.max_new_tokens, temperature=args.temperature, top_k=args.top_k,
+                                cache_bits=args.cache_bits, weight_bits=args.weight_bits)
         if _is_rank0():
             if args.json:
                 _print_json(row)

@@ -17,6 +17,7 @@ import torch
 
 from research_b200.errors import ContractError
 from research_b200.ops import functional as Fn
+from research_b200.ops import quantized
 
 
 class PagedKVCache:
@@ -31,11 +32,13 @@ class PagedKVCache:
         self.max_len = self.pages_per_seq * page_size
         total_pages = batch * self.pages_per_seq
         shape = (layers, total_pages, kv_heads, page_size, head_dim)
-        self.k = torch.zeros(shape, dtype=dtype, device=device)
-        self.v = torch.zeros(shape, dtype=dtype, device=device)
+        self.k, self.v = (self._pool(shape, dtype, device) for _ in range(2))
         self.page_table = torch.arange(total_pages, device=device, dtype=torch.int32).view(batch, self.pages_per_seq)
         self.lengths = torch.zeros(batch, dtype=torch.int32, device=device)
         self.batch = batch
+
+    def _pool(self, shape, dtype, device):
+        return torch.zeros(shape, dtype=dtype, device=device)
 
     @contextmanager
     def prompt(self):
@@ -131,6 +134,84 @@ class PagedKVCache:
         self.lengths = torch.maximum(self.lengths, (positions.max(dim=1).values + 1).to(torch.int32))
 
 
+class QuantizedKVCache(PagedKVCache):
+    """The same pages with rows in 4 bits (:mod:`research_b200.ops.quantized`: groups of 64 channels with a bf16 scale and
+    least value), 36 bytes for 64 channels instead of 128.
+
+    Rows are quantised as they are written and a decode step attends over them as they are held.  A prompt into an empty
+    cache attends over its own rows, which it still has in full; a later piece of several tokens reads the rows before it
+    back.  ``k`` and ``v`` are :class:`research_b200.ops.quantized.Q4Rows` ``[layers, pages, kv_heads, page_size, ..]``."""
+
+    def _pool(self, shape, dtype, device):
+        return quantized.empty_rows(*shape[:-1], channels=shape[-1], device=device)
+
+    def _pages(self, pool, layer: int):
+        return quantized.Q4Rows(*(t[layer].view(self.batch, self.pages_per_seq, *t.shape[2:]) for t in pool))
+
+    def update_and_attend(self, layer: int, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                          positions: torch.Tensor, window: int | None) -> torch.Tensor:
+        """Write k, v at ``positions`` ([B,T]) and attend q over everything written so far (causal)."""
+
+        B, T, Hq, D = q.shape
+        kp, vp = self._pages(self.k, layer), self._pages(self.v, layer)
+        native_ok = q.is_cuda and q.dtype == torch.bfloat16 and D in (64, 128) and Hq <= 8 * k.shape[2]
+        # on a CUDA device the restatements take what the kernels do not: other types, head sizes and head counts
+        write = quantized.kv_write_paged_q4 if native_ok or not q.is_cuda else quantized.kv_write_paged_q4_reference
+        attend = (quantized.decode_attention_paged_q4 if native_ok or not q.is_cuda
+                  else quantized.decode_attention_paged_q4_reference)
+        if T == 1:
+            step = getattr(self, "_step_positions", None)       # made by the first layer, reused by the others
+            if layer == 0 or step is None or step[0] is not positions:
+                pos = positions[:, 0].to(torch.int32).contiguous()
+                step = self._step_positions = (positions, pos, pos + 1, {None: None})
+            _, pos, lengths, bounds = step
+            if window not in bounds:
+                bounds[window] = (pos - (window - 1)).clamp_min(0)
+            write(k, v, kp, vp, pos)
+            return attend(q[:, 0], kp, vp, lengths, bounds[window])[:, None]
+        first = positions[:, :1]
+        in_a_row = self._from_zero or bool(
+            (positions == first + torch.arange(T, device=q.device, dtype=positions.dtype)).all())
+        if not in_a_row:
+            for t in range(T):                                  # a position given twice keeps its last row
+                write(k[:, t:t + 1], v[:, t:t + 1], kp, vp, positions[:, t])
+        elif self._from_zero or not bool(first.any()):
+            write(k, v, kp, vp)
+            return self._attend_rows(q, k, v, 0, window, positions, native_ok)
+        else:
+            write(k, v, kp, vp, positions[:, 0])
+        start = int(first.min())
+        end = int(positions.max()) + 1
+        keys, vals = quantized.kv_read_paged_q4(kp, vp, end) if native_ok else quantized.kv_read_paged_q4_reference(
+            kp, vp, end, channels=D, dtype=q.dtype)
+        if in_a_row and start + T == end:                       # every sequence at the same place
+            return self._attend_rows(q, keys, vals, start, window, positions, native_ok)
+        return self._attend_rows(q, keys, vals, None, window, positions, False)
+
+    def _attend_rows(self, q, keys, vals, start, window, positions, native_ok) -> torch.Tensor:
+        """Causal attention of tokens at ``positions`` over dense rows from position 0 on."""
+
+        B, T, Hq, D = q.shape
+        if not native_ok:
+            at = torch.arange(keys.shape[1], device=q.device)
+            allowed = at <= positions.long()[:, :, None]
+            if window is not None:
+                allowed = allowed & (at > positions.long()[:, :, None] - window)
+            return _masked_attention(q, keys, vals, allowed)
+        from research_b200.ops import native
+
+        front = start % 128                                     # the kernel's queries begin at a multiple of 128
+        if front:
+            q = torch.cat([q.new_zeros(B, front, Hq, D), q], dim=1)
+        q, keys, vals = (t if _packed_view(t) else t.contiguous() for t in (q, keys, vals))
+        lo = None
+        if window is not None:
+            at = torch.arange(start - front, start + T, device=q.device, dtype=torch.int32)
+            lo = (at - (window - 1)).clamp_min(0).expand(B, front + T).contiguous()
+        o, _ = native.attn_fwd(q, keys, vals, causal=True, lo=lo, q_offset=start - front)
+        return o[:, front:].reshape(B, T, Hq * D)
+
+
 def _packed_view(t: torch.Tensor) -> bool:
     """Whether the flash and cache kernels can read ``[B, T, heads, D]`` in place: dense heads, 16-byte rows."""
 
@@ -150,12 +231,17 @@ def _masked_attention(q, k, v, allowed):
     return torch.einsum("bhqk,bhkd->bhqd", p, vf).permute(0, 2, 1, 3).to(q.dtype).reshape(B, T, Hq * D)
 
 
-def init_kv_cache(model, batch: int, max_len: int, *, page_size: int = 128) -> PagedKVCache:
+def init_kv_cache(model, batch: int, max_len: int, *, page_size: int = 128, cache_bits: int = 16) -> PagedKVCache:
+    """An empty cache for ``model``: rows in the parameters' type (``cache_bits=16``) or in 4 bits (``cache_bits=4``)."""
+
+    if cache_bits not in (4, 16):
+        raise ContractError(f"generation.cache_bits must be 4 or 16, got {cache_bits!r}")
     spec = model.spec
     p = next(model.parameters())
     attn = model.layers[0].attn
-    return PagedKVCache(layers=spec.num_layers, batch=batch, max_len=max_len, kv_heads=attn.hkv,
-                        head_dim=spec.head_dim, page_size=page_size, dtype=p.dtype, device=p.device)
+    kind = QuantizedKVCache if cache_bits == 4 else PagedKVCache
+    return kind(layers=spec.num_layers, batch=batch, max_len=max_len, kv_heads=attn.hkv, head_dim=spec.head_dim,
+                page_size=page_size, dtype=p.dtype, device=p.device)
 
 
 def sample_next_token(logits: torch.Tensor, *, temperature: float, top_k: int | None, top_p: float | None,
@@ -226,6 +312,52 @@ def _graph_ok(model, device: torch.device) -> bool:
 KVCache = PagedKVCache
 
 
+class QuantizedWeights:
+    """4-bit copies of a model's linear weights, in use from :func:`quantize_weights` until :meth:`remove` (or the end of a
+    ``with`` block).  They are copies: parameters that change meanwhile are not seen."""
+
+    def __init__(self, params: list[torch.nn.Parameter]):
+        self._params = params
+
+    def remove(self) -> None:
+        for p in self._params:
+            if hasattr(p, "q4"):
+                del p.q4
+        self._params = []
+
+    def __enter__(self) -> "QuantizedWeights":
+        return self
+
+    def __exit__(self, *exc) -> None:
+        self.remove()
+
+
+_BLOCK_LINEARS = ("wqkv", "wo", "wgate", "w_gate_up", "w_down")
+
+
+@torch.no_grad()
+def quantize_weights(model) -> QuantizedWeights:
+    """Give every attention and dense feed-forward linear of ``model`` 4-bit rows (:mod:`research_b200.ops.quantized`) that
+    the calls without gradients multiply with; the embedding, the lm_head, norms, routers and routed experts stay as they
+    are, and a call that records gradients takes the parameter itself."""
+
+    if getattr(getattr(model, "ex", None), "tp_size", 1) > 1:
+        raise ContractError("generation.weight_bits=4 needs whole weights: the model is split over tensor-parallel ranks")
+    params = []
+    dtype = getattr(model, "compute_dtype", torch.float32)
+    for index, layer in enumerate(model.layers):
+        if model.layer_prepare is not None:
+            model.layer_prepare(index)
+        for module in layer.modules():
+            for name in _BLOCK_LINEARS:
+                p = module._parameters.get(name)
+                if p is None or p.dim() != 2:                   # routed experts are stacks of matrices
+                    continue
+                p.q4 = quantized.quantize_rows_q4(Fn.compute_weight(p, torch.empty(0, dtype=dtype, device=p.device)))
+                params.append(p)
+    return QuantizedWeights(params)
+
+
 @torch.no_grad()
 def prefill(model, prompt_ids: torch.Tensor, cache: PagedKVCache) -> torch.Tensor:
     """Run the prompt ``[B, P]`` through the model, fill ``cache`` and return the logits of the last position
@@ -264,8 +396,11 @@ class GenerationResult:
 @torch.no_grad()
 def generate_tokens(model, prompt_ids: torch.Tensor, *, max_new_tokens: int, temperature: float = 1.0,
                     top_k: int | None = None, top_p: float | None = None, seed: int = 0,
-                    page_size: int = 128) -> GenerationResult:
-    """prompt_ids: [B, P] (all prompts the same length).  Prefill once, then one decode step per new token."""
+                    page_size: int = 128, cache_bits: int = 16, weight_bits: int = 16) -> GenerationResult:
+    """prompt_ids: [B, P] (all prompts the same length).  Prefill once, then one decode step per new token.
+
+    ``cache_bits=4`` holds the K/V cache in 4 bits, ``weight_bits=4`` runs the blocks' linears on 4-bit copies of their
+    weights for the call (:func:`quantize_weights`)."""
 
     if max_new_tokens <= 0:
         raise ContractError(f"generation.max_new_tokens must be positive, got {max_new_tokens}")
@@ -273,11 +408,17 @@ def generate_tokens(model, prompt_ids: torch.Tensor, *, max_new_tokens: int, tem
     total = P + max_new_tokens
     if total > model.spec.max_seq_len:
         raise ContractError(f"prompt + max_new_tokens = {total} exceeds model.max_seq_len = {model.spec.max_seq_len}")
+    if weight_bits not in (4, 16):
+        raise ContractError(f"generation.weight_bits must be 4 or 16, got {weight_bits!r}")
+    if weight_bits == 4:
+        with quantize_weights(model):
+            return generate_tokens(model, prompt_ids, max_new_tokens=max_new_tokens, temperature=temperature, top_k=top_k,
+                                   top_p=top_p, seed=seed, page_size=page_size, cache_bits=cache_bits)
     device = next(model.parameters()).device
     prompt_ids = prompt_ids.to(device)
     was_training = model.training
     model.eval()
-    cache = init_kv_cache(model, B, total, page_size=page_size)
+    cache = init_kv_cache(model, B, total, page_size=page_size, cache_bits=cache_bits)
     gen = torch.Generator(device=device).manual_seed(int(seed))
     positions = torch.arange(P, device=device, dtype=torch.int32).expand(B, P).contiguous()
     with cache.prompt():

@@ -20,7 +20,7 @@ import torch
 import torch.nn.functional as F
 from torch.autograd import forward_ad
 
-from research_b200.ops import native
+from research_b200.ops import native, quantized
 
 # RESEARCH_B200_LIBRARY=1 runs the whole stack on stock PyTorch operators (cuBLAS matmuls, the library's
 # scaled_dot_product_attention, plain tensor ops in the optimizer, NCCL collectives): the comparison arm of the
@@ -128,8 +128,12 @@ class _LinearFn(torch.autograd.Function):
 
 
 def linear(x: torch.Tensor, p: torch.Tensor) -> torch.Tensor:
-    """``y = x @ W^T`` with ``W`` stored ``[out, in]``."""
+    """``y = x @ W^T`` with ``W`` stored ``[out, in]``; where ``W`` has 4-bit rows (its ``q4``) and nothing records
+    gradients, with those."""
 
+    rows = getattr(p, "q4", None)
+    if rows is not None and not torch.is_grad_enabled():
+        return (quantized.linear_q4 if use_native(x) or not x.is_cuda else quantized.linear_q4_reference)(x, rows)
     if use_native(x):
         if not torch.is_grad_enabled() and x.numel() // x.shape[-1] <= 64:
             # decode-sized input: stream the weight with the whole device (split-K), no autograd bookkeeping

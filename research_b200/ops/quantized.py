@@ -17,6 +17,7 @@ Nothing here has a gradient: a call that would record one is refused.  On a CUDA
 
 from __future__ import annotations
 
+import functools
 import math
 from contextlib import nullcontext
 from typing import NamedTuple
@@ -162,20 +163,28 @@ def _no_gradient(what: str, *tensors: torch.Tensor) -> None:
 
 
 def _same_device(what: str, first: torch.Tensor, *others: torch.Tensor | None) -> None:
+    at = first.get_device()                             # -1: the CPU
     for t in others:
-        if t is not None and t.device != first.device:
+        if t is not None and t.get_device() != at:
             raise KernelError(f"{what}: all tensors have to be on {first.device}, got one on {t.device}")
 
 
-def _on(device: torch.device):
+_SAME = nullcontext()
+
+
+def _on(t: torch.Tensor):
     """Launches go to the current stream of the tensors' own device."""
 
-    return nullcontext() if device.index == torch._C._cuda_getDevice() else torch.cuda.device(device)
+    return _SAME if t.get_device() == torch._C._cuda_getDevice() else torch.cuda.device(t.device)
 
 
 def _check_rows(what: str, rows: Q4Rows, channels: int) -> None:
     width = row_width(channels)
     codes, affine = rows
+    if (codes.dtype is torch.uint8 and affine.dtype is torch.bfloat16 and codes.shape[-1] * 2 == width
+            and affine.shape == codes.shape[:-1] + (width // GROUP, 2) and codes.is_contiguous()
+            and affine.is_contiguous() and codes.get_device() == affine.get_device()):
+        return
     if codes.dtype != torch.uint8 or affine.dtype != torch.bfloat16:
         raise KernelError(f"{what}: 4-bit rows are uint8 codes and bf16 pairs, got {codes.dtype} and {affine.dtype}")
     if codes.shape[-1] * 2 != width or affine.shape != (*codes.shape[:-1], width // GROUP, 2):
@@ -191,14 +200,15 @@ def _check_pools(what: str, k_pool: Q4Rows, v_pool: Q4Rows, B: int, Hkv: int | N
         if pool.codes.dim() != 5:
             raise KernelError(f"{what}: a cache has codes [B, pages, Hkv, page_rows, D / 2], got {tuple(pool.codes.shape)}")
         _check_rows(what, pool, D)
-    if k_pool.codes.shape != v_pool.codes.shape:
-        raise KernelError(f"{what}: the K and the V cache must have one shape, got {tuple(k_pool.codes.shape)} and "
+    shape = k_pool.codes.shape
+    if shape != v_pool.codes.shape:
+        raise KernelError(f"{what}: the K and the V cache must have one shape, got {tuple(shape)} and "
                           f"{tuple(v_pool.codes.shape)}")
     _same_device(what, k_pool.codes, v_pool.codes)
-    if k_pool.codes.shape[0] != B or (Hkv is not None and k_pool.codes.shape[2] != Hkv):
-        raise KernelError(f"{what}: a cache {tuple(k_pool.codes.shape)} does not hold {B} sequences"
+    seqs, pages, heads, page_rows, _ = shape
+    if seqs != B or (Hkv is not None and heads != Hkv):
+        raise KernelError(f"{what}: a cache {tuple(shape)} does not hold {B} sequences"
                           + ("" if Hkv is None else f" of {Hkv} heads"))
-    _, pages, heads, page_rows, _ = k_pool.codes.shape
     if pages * page_rows > 2 ** 31 - 1:
         raise KernelError(f"{what}: a sequence has at most 2^31 - 1 rows, got {pages} pages of {page_rows}")
     return pages, heads, page_rows
@@ -207,9 +217,10 @@ def _check_pools(what: str, k_pool: Q4Rows, v_pool: Q4Rows, B: int, Hkv: int | N
 def _per_sequence(what: str, name: str, t: torch.Tensor | None, B: int, like: torch.Tensor) -> torch.Tensor | None:
     if t is None:
         return None
-    if t.shape != (B,) or t.dtype not in (torch.int32, torch.int64):
+    if t.dim() != 1 or t.shape[0] != B or t.dtype not in (torch.int32, torch.int64):
         raise KernelError(f"{what}: {name} is an int32 or int64 tensor [{B}], got {tuple(t.shape)} {t.dtype}")
-    _same_device(what, like, t)
+    if t.get_device() != like.get_device():
+        _same_device(what, like, t)
     return t.clamp(-2 ** 31, 2 ** 31 - 1).to(torch.int32) if t.dtype == torch.int64 else t.contiguous()
 
 
@@ -236,8 +247,8 @@ def quantize_rows_q4(x: torch.Tensor) -> Q4Rows:
     codes = torch.empty(*x.shape[:-1], width // 2, dtype=torch.uint8, device=x.device)
     affine = torch.empty(*x.shape[:-1], width // GROUP, 2, dtype=torch.bfloat16, device=x.device)
     if x2.shape[0]:
-        with _on(x.device):
-            native._check(native.load().b200_q4_quantize_rows(
+        with _on(x):
+            native._check((native._lib or native.load()).b200_q4_quantize_rows(
                 x2.data_ptr(), x2.stride(0), codes.data_ptr(), affine.data_ptr(), x2.shape[0], x2.shape[1],
                 native._stream()), "b200_q4_quantize_rows")
     return Q4Rows(codes, affine)
@@ -258,8 +269,8 @@ def _expand(rows: Q4Rows) -> torch.Tensor:
     width = rows.codes.shape[-1] * 2
     out = torch.empty(*rows.codes.shape[:-1], width, dtype=torch.bfloat16, device=rows.codes.device)
     if out.numel():
-        with _on(out.device):
-            native._check(native.load().b200_q4_dequantize_rows(
+        with _on(out):
+            native._check((native._lib or native.load()).b200_q4_dequantize_rows(
                 rows.codes.data_ptr(), rows.affine.data_ptr(), out.data_ptr(), out.numel() // width, width,
                 native._stream()), "b200_q4_dequantize_rows")
     return out
@@ -269,8 +280,8 @@ def _expand(rows: Q4Rows) -> torch.Tensor:
 # cache
 # --------------------------------------------------------------------------------------------------
 def _heads_apart(t: torch.Tensor) -> bool:
-    return (t.stride(3) == 1 and t.stride(2) == t.shape[3] and t.stride(1) % 8 == 0 and t.stride(0) % 8 == 0
-            and t.data_ptr() % 16 == 0)
+    batch, row, head, one = t.stride()
+    return one == 1 and head == t.shape[3] and row % 8 == 0 and batch % 8 == 0 and t.data_ptr() % 16 == 0
 
 
 def kv_write_paged_q4(k: torch.Tensor, v: torch.Tensor, k_pool: Q4Rows, v_pool: Q4Rows,
@@ -298,9 +309,10 @@ def kv_write_paged_q4(k: torch.Tensor, v: torch.Tensor, k_pool: Q4Rows, v_pool: 
     _head_dim(what, D)
     if k.dtype != torch.bfloat16:
         raise KernelError(f"{what} quantises bf16 rows on a CUDA device, got {k.dtype}")
-    k, v = (t if _heads_apart(t) else t.contiguous() for t in (k, v))
-    with _on(k.device):
-        native._check(native.load().b200_q4_kv_write(
+    k = k if _heads_apart(k) else k.contiguous()
+    v = v if _heads_apart(v) else v.contiguous()
+    with _on(k):
+        native._check((native._lib or native.load()).b200_q4_kv_write(
             k.data_ptr(), v.data_ptr(), k.stride(1), k.stride(0), v.stride(1), v.stride(0), k_pool.codes.data_ptr(),
             k_pool.affine.data_ptr(), v_pool.codes.data_ptr(), v_pool.affine.data_ptr(), native._ptr(start), B, T, Hkv,
             D, pages, page_rows, native._stream()), "b200_q4_kv_write")
@@ -326,8 +338,8 @@ def kv_read_paged_q4(k_pool: Q4Rows, v_pool: Q4Rows, rows: int, start: torch.Ten
         raise KernelError(f"{what} writes bf16 on a CUDA device, got {dtype}")
     out = torch.empty(2, B, rows, Hkv, D, dtype=torch.bfloat16, device=k_pool.codes.device)
     if out.numel() and pages * page_rows:
-        with _on(out.device):
-            native._check(native.load().b200_q4_kv_read(
+        with _on(out):
+            native._check((native._lib or native.load()).b200_q4_kv_read(
                 out[0].data_ptr(), out[1].data_ptr(), k_pool.codes.data_ptr(), k_pool.affine.data_ptr(),
                 v_pool.codes.data_ptr(), v_pool.affine.data_ptr(), native._ptr(start), B, rows, Hkv, D, pages,
                 page_rows, native._stream()), "b200_q4_kv_read")
@@ -367,8 +379,8 @@ def decode_attention_paged_q4(q: torch.Tensor, k_pool: Q4Rows, v_pool: Q4Rows, l
         return out
     if pages * page_rows == 0:
         return out.zero_()
-    lib = native.load()
-    with _on(q.device):
+    lib = native._lib or native.load()
+    with _on(q):
         runs = lib.b200_q4_decode_attn_runs(B, Hkv, pages * page_rows)
         slots = (runs + B * Hkv) * (Hq // Hkv)
         parts = torch.empty(slots * (D + 2), dtype=torch.float32, device=q.device)
@@ -407,15 +419,21 @@ def linear_q4(x: torch.Tensor, w: Q4Rows) -> torch.Tensor:
     rows = x2.shape[0]
     if rows == 0 or N == 0:
         return torch.empty(*x.shape[:-1], N, dtype=x.dtype, device=x.device)
-    with _on(x.device):
+    with _on(x):
         if rows > LINEAR_ROWS:
             return _expanded_linear(x2, w).view(*x.shape[:-1], N)
         if x2.stride(1) != 1:
             x2 = x2.contiguous()
         out = torch.empty(rows, N, dtype=torch.bfloat16, device=x.device)
-        native._check(native.load().b200_q4_linear(x2.data_ptr(), x2.stride(0), w.codes.data_ptr(), w.affine.data_ptr(),
-                                                   out.data_ptr(), N, rows, N, K, native._stream()), "b200_q4_linear")
+        native._check((native._lib or native.load()).b200_q4_linear(x2.data_ptr(), x2.stride(0), w.codes.data_ptr(), w.affine.data_ptr(),
+                                                   out.data_ptr(), N, rows, N, K, *linear_shape(rows, N, K),
+                                                   native._stream()), "b200_q4_linear")
     return out.view(*x.shape[:-1], N)
+
+
+@functools.lru_cache(maxsize=4096)
+def linear_shape(rows: int, n: int, k: int) -> tuple[int, int]:
+    return 2, 1
 
 
 def _expanded_linear(x: torch.Tensor, w: Q4Rows) -> torch.Tensor:

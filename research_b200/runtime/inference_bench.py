@@ -17,12 +17,13 @@ import time
 import torch
 
 from research_b200.config import load_config
+from research_b200.errors import ContractError
 from research_b200.infer import generation
 
 
 def run_inference_bench(spec, *, batch: int, prompt: int, new_tokens: int, temperature: float, top_k: int | None,
                         warmup: int = 1, repeats: int = 3, seed: int = 0, device: str | None = None,
-                        use_graph: bool = True) -> dict:
+                        use_graph: bool = True, cache_bits: int = 16, weight_bits: int = 16) -> dict:
     import dataclasses
     import os
 
@@ -39,6 +40,10 @@ def run_inference_bench(spec, *, batch: int, prompt: int, new_tokens: int, tempe
     g = torch.Generator(device="cpu").manual_seed(seed)
     prompts = torch.randint(0, spec.model.vocab_size, (batch, prompt), generator=g, dtype=torch.int32).to(dev)
     cuda = dev.type == "cuda"
+    if weight_bits not in (4, 16):
+        raise ContractError(f"generation.weight_bits must be 4 or 16, got {weight_bits!r}")
+    if weight_bits == 4:
+        generation.quantize_weights(model)
 
     def sync():
         if cuda:
@@ -46,7 +51,7 @@ def run_inference_bench(spec, *, batch: int, prompt: int, new_tokens: int, tempe
 
     def one_run():
         with torch.no_grad():
-            cache = generation.init_kv_cache(model, batch, prompt + new_tokens)
+            cache = generation.init_kv_cache(model, batch, prompt + new_tokens, cache_bits=cache_bits)
             gen = torch.Generator(device=dev).manual_seed(seed)
             pos = torch.arange(prompt, device=dev, dtype=torch.int32).expand(batch, prompt).contiguous()
             sync()
@@ -97,6 +102,7 @@ def run_inference_bench(spec, *, batch: int, prompt: int, new_tokens: int, tempe
         "ttft_ms": 1e3 * t_first,
         "batch": batch, "prompt_tokens": prompt, "new_tokens": new_tokens, "temperature": temperature, "top_k": top_k,
         "cuda_graph": bool(use_graph and cuda), "model": spec.model.name, "device": str(dev), "dtype": str(next(model.parameters()).dtype),
+        "cache_bits": cache_bits, "weight_bits": weight_bits,
         "data": "synthetic (random-init weights, uniform random prompt ids)",
     }
 
@@ -111,12 +117,15 @@ def main(argv: list[str] | None = None) -> int:
     ap.add_argument("--top-k", type=int, default=1)
     ap.add_argument("--repeats", type=int, default=3)
     ap.add_argument("--device", default=None)
+    ap.add_argument("--cache-bits", type=int, default=16, choices=[4, 16], help="bits of a K/V cache element")
+    ap.add_argument("--weight-bits", type=int, default=16, choices=[4, 16], help="bits of the blocks' linear weights")
     ap.add_argument("--no-graph", action="store_true", help="launch every decode kernel separately")
     args = ap.parse_args(argv)
     spec = load_config(args.config)
     prompt = args.prompt if args.prompt is not None else min(512, spec.model.max_seq_len // 2)
     out = run_inference_bench(spec, batch=args.batch, prompt=prompt, new_tokens=args.new, temperature=args.temperature,
-                              top_k=args.top_k, repeats=args.repeats, device=args.device, use_graph=not args.no_graph)
+                              top_k=args.top_k, repeats=args.repeats, device=args.device, use_graph=not args.no_graph,
+                              cache_bits=args.cache_bits, weight_bits=args.weight_bits)
     print(json.dumps(out))
     return 0
 

@@ -45,7 +45,8 @@ def parse_prompt_ids(value, vocab_size: int | None = None) -> list[int]:
 
 
 def sample_checkpoint(run_dir: str | Path, selector: str, *, prompt_ids, max_new_tokens: int,
-                      temperature: float = 1.0, top_k: int | None = None) -> dict[str, Any]:
+                      temperature: float = 1.0, top_k: int | None = None, cache_bits: int = 16,
+                      weight_bits: int = 16) -> dict[str, Any]:
     run_dir = Path(run_dir)
     prompt = parse_prompt_ids(prompt_ids)                    # a malformed prompt fails before anything is restored
     ck = restore_inference_checkpoint(run_dir, selector)
@@ -56,7 +57,7 @@ def sample_checkpoint(run_dir: str | Path, selector: str, *, prompt_ids, max_new
     page_size = spec.generation.page_size if spec.generation is not None else 128
     result = generate_tokens(ck.model, torch.tensor([prompt], dtype=torch.int64), max_new_tokens=max_new_tokens,
                              temperature=temperature, top_k=top_k, seed=ck.trainer.rng.sample & 0x7FFFFFFF,
-                             page_size=page_size)
+                             page_size=page_size, cache_bits=cache_bits, weight_bits=weight_bits)
     m = spec.model
     row = {
         "schema_version": 1, "status": "completed", "created_at": utc_now(), "run_id": spec.run_id,
@@ -68,6 +69,8 @@ def sample_checkpoint(run_dir: str | Path, selector: str, *, prompt_ids, max_new
         "logprobs": result.logprobs[0], "max_new_tokens": max_new_tokens, "temperature": temperature, "top_k": top_k,
         "sampler": "greedy" if top_k == 1 else "categorical",
     }
+    if (cache_bits, weight_bits) != (16, 16):                # a plain sample's row keeps its fields
+        row["sampling"].update(cache_bits=cache_bits, weight_bits=weight_bits)
     if ck.trainer.is_writer:
         path = LocalArtifactWriter(run_dir).append_checkpoint_sample(ck.record.step, row)
         row["artifact_path"] = path.relative_to(run_dir).as_posix()
