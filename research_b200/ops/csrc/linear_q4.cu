@@ -1,286 +1,496 @@
-// y = x W^T for a few rows of x and weights held in 4 bits (quant4.cuh): x [rows, K] bf16, W [N, K], y [rows, N] bf16 with
-// fp32 sums.  The time is that of streaming the codes once (0.56 bytes a weight), as long as expanding them keeps up.
+// y = x W^T for up to 64 rows of x and weights held in 4 bits (quant4.cuh): x [rows, K] bf16, W [N, K], y [rows, N] bf16 with
+// fp32 sums.  The time is that of streaming the codes once (0.56 bytes a weight), as long as expanding them keeps up: at the
+// copy bandwidth an SM gets 46 codes a clock, which is what the arrangement below is for.
 //
-// Weights are the 16-row operand of m16n8k16, the rows of x its columns, eight to a tile.  A code becomes the bf16 128 + n by
-// half a shift and one and-or per two codes, exact; a group's sum is scaled in fp32, and what the offset and the least values
-// add is taken off at the end by a small product over the groups:
-//   y = sum_g s_g (sum_k x_k (128 + n_k)) + sum_g (z_g - 128 s_g) X_g,   X_g = sum_k x_k,
-// with X_g, itself a product with ones, as three bf16 parts (24 bits) against s and z, which are bf16.
+// The weights are the 128-row operand of tcgen05.mma, from tensor memory, the rows of x its columns (16 or 32 at a time), both in
+// e4m3.  The bytes 0 .. 15 are, as e4m3, the numbers n 2^-9 (subnormals and the first binade are one straight line), so that a
+// word of eight codes becomes eight operands by two masks and a shift, a third of what bf16 operands take, in half the tensor
+// memory.  A row of x is brought to [128, 256) by a power of two and split into two e4m3 numbers, high + low, which go into
+// one accumulator: the eight bits of a bf16 are two times four, so that is exact down to 2^-10 of the row's largest value, and
+// below that off by 2^-19 of it at most.  The product of each group is taken by itself.  The sum X_g of x over a group gets
+// into every lane as a product too, of fours with 32 e4m3 numbers that add up to a quarter of it (16 times its sixteenth, then
+// what is left: to 2^-16 of the row's largest value); scales and least values are applied to both in fp32:
+//   y = x_max (sum_g s_g (sum_k x'_k n_k) + z_g X'_g),   x' = x / x_max
+// (weights rounded to bf16 instead would cost as much precision again as the result's own rounding; sums and scales of x from
+// shared memory, the same word for all lanes, take one pass a word: 16 passes a column and 128 x 128 block, 85 us for 28672 x
+// 4096 with 64 rows).  K is cut over the blocks of a cluster, which add up their partial sums in rank order: the same bits
+// every time.
 //
-// A block of eight warps has 16 WM weight rows and a slice of K; WM warps share the rows, 8 / WM the slice's blocks of 128
-// channels, and the blocks of a cluster share K.  Codes go straight to the registers of the lane that expands them, four
-// blocks ahead; x goes through shared memory, two stages, rows 16 bytes apart from a multiple of 128, so that no two lanes
-// of a read meet in a bank.  Partial sums are added in the order of warps and ranks, the same bits every time.
+// A first kernel splits x once for all blocks, while the second one, launched as its dependent, brings its first codes into
+// L2.  The second one's warps:
+//   warp 0     TMA: 256 channels of codes (128 x 128 bytes) and of the split x through a ring of stages
+//   warp 1     MMA issuer: for each group the products with the high and the low parts
+//   warps 2-5  a weight row per thread: expand the next half stage's codes, then scale and add up the current one's products
+// An SM has up to four such blocks, which wait at different places: roles of their own for expanding and for adding up, in one
+// block of 20 warps, took 33 us for 28672 x 4096 with 16 rows, most of it in handing over.
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+#include <math_constants.h>
+
 #include "quant4.cuh"
 #include "host_util.cuh"
 
 namespace {
 
 using namespace q4;
+using namespace b200;
 
-constexpr int kWarps = 8, kThreads = kWarps * 32, kAhead = 4;
+constexpr int kThreads = 192;
+constexpr int kStage = 256;                    // channels of a stage
+constexpr int kCodeBytes = 128 * kStage / 2;
+constexpr int kMaxStages = 8;
+constexpr int kFours = 32, kProducts = 48;     // tensor memory: half a stage's codes (128 bytes a row), 32 fours, products
+constexpr int ERR_Q4_A = 41, ERR_Q4_D = 42;    // status codes: operands or products that never came
 
 struct LinearParams {
-  const __nv_bfloat16* x;
-  long long ldx, ldo;
-  const uint8_t *codes, *affine;
+  const uint8_t* affine;
+  const float* xs;                    // [rows]: what a row of x was divided by
   __nv_bfloat16* out;
-  int rows, N, K, width, cluster;
-  int aligned;                        // rows of x start on 16 bytes
+  long long ldo;
+  int rows, N, width, cluster, stages, token_tiles;
+  int* status;
 };
 
-__device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                    uint32_t b1) {
-  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+// D[tmem] (+)= A[tmem] * B[smem], both e4m3, fp32 accumulate; 32 channels
+__device__ __forceinline__ void tc_mma_ts_e4m3(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
+                                               uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], [%1], %2, %3, p;\n\t}"
+      ::"r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
 }
-// Codes P of both halves of w as bf16 128 + n: one shift and one three-input operation (a & b) | c, whose constants are kept
-// in registers, since an instruction has room for one.
-template <int P>
-__device__ __forceinline__ uint32_t coded(uint32_t w, uint32_t mask, uint32_t magic) {
-  uint32_t r;
-  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(P ? w >> (4 * P) : w), "r"(mask), "r"(magic));
-  return r;
+// instruction descriptor: e4m3 operands (format 0), both K-major, fp32 result
+__host__ __device__ constexpr uint32_t make_idesc_e4m3(int m, int n) {
+  return (1u << 4) | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24);
 }
-constexpr uint32_t kOnes = 0x3f803f80u;
+
+// A wait that looks a few times without the suspend hint of mbar_wait first: 46 clocks instead of 84 where the phase is
+// complete, and no waking up where it is soon.
+__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, const AbortCtx& ab, int code) {
+#pragma unroll 1
+  for (int i = 0; i < 2; ++i) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    if (ok) return true;
+  }
+  return mbar_wait(bar, parity, ab, code);
+}
+__device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, const AbortCtx& ab, int code) {
+  return __all_sync(0xffffffffu, wait(bar, parity, ab, code));
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+      ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+        "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+template <int COLS>
+__device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t* r) {
+  if constexpr (COLS == 16) {
+    tmem_ld_32x32b_x16(taddr, *reinterpret_cast<uint32_t(*)[16]>(r));
+  } else {
+    tmem_ld_32x32b_x32(taddr, *reinterpret_cast<uint32_t(*)[32]>(r));
+  }
+}
 
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-__device__ __forceinline__ float ld_cluster(uint32_t saddr, uint32_t rank) {
+__device__ __forceinline__ float4 ld_cluster4(uint32_t saddr, uint32_t rank) {
   uint32_t peer;
-  float v;
+  float4 v;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(peer) : "r"(saddr), "r"(rank));
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(peer) : "memory");
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(peer)
+               : "memory");
   return v;
 }
 
-template <int NT, int WM>
-struct Shape {
-  static constexpr int WK = kWarps / WM;
-  static constexpr int BPW = WK >= 4 ? 1 : 2;                 // blocks a warp has in a stage
-  static constexpr int STAGE_BLOCKS = WK * BPW, STAGE_CHANNELS = STAGE_BLOCKS * 128;
-  static constexpr int TOKENS = NT * 8, PITCH = STAGE_CHANNELS * 2 + 16;
-  static constexpr int STAGE_BYTES = TOKENS * PITCH;
-  static constexpr int SUM_BYTES = kWarps * 16 * TOKENS * 4;  // partial results, over the stages
-  static constexpr int RING_BYTES = 2 * STAGE_BYTES > SUM_BYTES ? 2 * STAGE_BYTES : SUM_BYTES;
-  // groups of the slice: a 16-multiple of them, X_g in fp32
-  static int xs_bytes(int slice_blocks) { return ((2 * slice_blocks + 15) / 16 * 16) * TOKENS * 4; }
-};
+template <int NT>
+constexpr int stage_bytes() { return kCodeBytes + (2 * 2 + 1) * NT * 128; }   // codes; [half][high, low] of x; its sums
 
-template <int NT, int WM>
-__global__ void __launch_bounds__(kThreads, NT <= 4 ? 2 : 1) linear_q4_kernel(const __grid_constant__ LinearParams p) {
-  using S = Shape<NT, WM>;
-  constexpr int WK = S::WK, BPW = S::BPW, TOKENS = S::TOKENS;
-  extern __shared__ __align__(16) uint8_t smem[];
-  float* xs = reinterpret_cast<float*>(smem + S::RING_BYTES);   // [groups][TOKENS]
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int wm = warp % WM, wk = warp / WM;
-  const int rank = blockIdx.x % p.cluster, tile = blockIdx.x / p.cluster;
-  const int blocks = p.width / 128;
-  const int slice = (blocks + p.cluster - 1) / p.cluster;       // blocks of 128 channels of a rank
-  const int kb0 = rank * slice, n_blocks = max(min(slice, blocks - kb0), 0);
-  const int mine = (n_blocks - wk + WK - 1) / WK;               // of this warp: kb0 + wk + i WK (may be none)
-  const int stages = (n_blocks + S::STAGE_BLOCKS - 1) / S::STAGE_BLOCKS;
-
-  const int n0 = (tile * WM + wm) * 16 + g;
-  const long long ra = min(n0, p.N - 1), rb = min(n0 + 8, p.N - 1);
-  const uint8_t* ca = p.codes + ra * (p.width / 2) + (kb0 + wk) * 64 + t * 16;
-  const uint8_t* cb = p.codes + rb * (p.width / 2) + (kb0 + wk) * 64 + t * 16;
-  const uint8_t* sa = p.affine + ra * (p.width / 16) + (kb0 + wk) * 8;
-  const uint8_t* sb = p.affine + rb * (p.width / 16) + (kb0 + wk) * 8;
-  b200::pdl_launch_dependents();
+// x [rows, K] -> per NT rows xq [high, low][NT][width] e4m3, behind all of them the groups' sums [rows][width / 64][32], and
+// xs [rows] fp32, rows rounded up to NT; a block per row.  Channels go into the order in which a word's codes fall into its low and its high nibbles: 0 4 1 5 2 6 3 7.
+__global__ void __launch_bounds__(512) linear_q4_split_kernel(const __nv_bfloat16* __restrict__ x, long long ldx, int rows,
+                                                              int K, int width, int NT, int aligned,
+                                                              uint8_t* __restrict__ xq,
+                                                              float* __restrict__ xs) {
+  __shared__ uint32_t s_most[16];
+  const int r = blockIdx.x;
+  const bool there = r < rows;
+  pdl_launch_dependents();
+  pdl_wait();
+  auto load = [&](int c, float (&f)[16]) {
+    if (there && aligned && c + 16 <= K) {
+      const uint4* at = reinterpret_cast<const uint4*>(x + r * ldx + c);
+      float lo[8], hi[8];
+      unpack_bf16(at[0], lo);
+      unpack_bf16(at[1], hi);
 #pragma unroll
-  for (int i = 0; i < kAhead; ++i)      // what runs before may be what writes the weights: only into L2 ahead of the wait
-    if (i < mine && t == 0) {
-      asm volatile("prefetch.global.L2 [%0];" ::"l"(ca + i * WK * 64));
-      asm volatile("prefetch.global.L2 [%0];" ::"l"(cb + i * WK * 64));
-    }
-  // columns behind the last row of x stay zero
-  for (int i = threadIdx.x; i < 2 * (TOKENS - p.rows) * (S::PITCH / 16); i += kThreads) {
-    const int c = i % (S::PITCH / 16), r = i / (S::PITCH / 16);
-    *reinterpret_cast<uint4*>(smem + (r & 1) * S::STAGE_BYTES + (p.rows + (r >> 1)) * S::PITCH + c * 16) = make_uint4(0, 0, 0, 0);
-  }
-  b200::pdl_wait();
-
-  uint4 wa[kAhead], wb[kAhead];
-  uint2 fa[kAhead], fb[kAhead];
-  auto load = [&](int i, int slot) {
-    if (i < mine) {
-      wa[slot] = __ldg(reinterpret_cast<const uint4*>(ca + static_cast<long long>(i) * (WK * 64)));
-      wb[slot] = __ldg(reinterpret_cast<const uint4*>(cb + static_cast<long long>(i) * (WK * 64)));
-      fa[slot] = __ldg(reinterpret_cast<const uint2*>(sa + static_cast<long long>(i) * (WK * 8)));
-      fb[slot] = __ldg(reinterpret_cast<const uint2*>(sb + static_cast<long long>(i) * (WK * 8)));
+      for (int k = 0; k < 8; ++k) f[k] = lo[k], f[8 + k] = hi[k];
+    } else {
+#pragma unroll
+      for (int k = 0; k < 16; ++k) f[k] = there && c + k < K ? __bfloat162float(x[r * ldx + c + k]) : 0.f;
     }
   };
+  uint32_t most = 0;
+  for (int c = threadIdx.x * 16; c < width; c += 512 * 16) {
+    float f[16];
+    load(c, f);
 #pragma unroll
-  for (int i = 0; i < kAhead; ++i) load(i, i);
-
-  auto stage_in = [&](int s) {
-    if (s < stages) {
-      uint8_t* dst = smem + (s & 1) * S::STAGE_BYTES;
-      const int c0 = kb0 * 128 + s * S::STAGE_CHANNELS;
-      constexpr int CHUNKS = S::STAGE_CHANNELS / 8;
-      for (int i = threadIdx.x; i < p.rows * CHUNKS; i += kThreads) {
-        const int r = i / CHUNKS, cc = i - r * CHUNKS, c = c0 + cc * 8;
-        uint8_t* to = dst + r * S::PITCH + cc * 16;
-        const __nv_bfloat16* from = p.x + r * p.ldx + c;
-        if (p.aligned) {
-          const int bytes = max(min((p.K - c) * 2, 16), 0);
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(b200::smem_u32(to)), "l"(bytes ? from : p.x), "r"(bytes)
-                       : "memory");
-        } else {
-          const uint16_t* u = reinterpret_cast<const uint16_t*>(from);
-          uint32_t v[4] = {};
-#pragma unroll
-          for (int k = 0; k < 8; ++k)
-            if (c + k < p.K) v[k >> 1] |= static_cast<uint32_t>(u[k]) << (16 * (k & 1));
-          *reinterpret_cast<uint4*>(to) = make_uint4(v[0], v[1], v[2], v[3]);
-        }
-      }
-    }
-    asm volatile("cp.async.commit_group;" ::: "memory");
-  };
-  stage_in(0);
-
-  uint32_t mask = 0x000f000fu, magic = 0x43004300u;
-  asm volatile("" : "+r"(mask), "+r"(magic));
-  float y[NT][4] = {};
-  for (int i0 = 0; i0 < stages * BPW; i0 += kAhead) {
-#pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-      const int i = i0 + u;
-      if (i < stages * BPW) {             // the same for every thread of the block
-        const int s = i / BPW;
-        if (i % BPW == 0) {
-          asm volatile("cp.async.wait_group 0;" ::: "memory");
-          __syncthreads();                // stage s is there, and nobody reads stage s - 1 any more
-          stage_in(s + 1);
-        }
-        if (i < mine) {
-          const uint8_t* xb = smem + (s & 1) * S::STAGE_BYTES + g * S::PITCH + ((i % BPW) * WK + wk) * 256 + t * 32;
-          const uint32_t ka[4] = {wa[u].x, wa[u].y, wa[u].z, wa[u].w}, kb[4] = {wb[u].x, wb[u].y, wb[u].z, wb[u].w};
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            float acc[NT][4], ones[NT][4];
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-              for (int c = 0; c < 4; ++c) acc[n][c] = ones[n][c] = 0.f;
-#pragma unroll
-            for (int j = h; j < 4; j += 2) {
-              const uint32_t a0 = coded<0>(ka[j], mask, magic), a1 = coded<0>(kb[j], mask, magic);
-              const uint32_t a2 = coded<1>(ka[j], mask, magic), a3 = coded<1>(kb[j], mask, magic);
-              const uint32_t e0 = coded<2>(ka[j], mask, magic), e1 = coded<2>(kb[j], mask, magic);
-              const uint32_t e2 = coded<3>(ka[j], mask, magic), e3 = coded<3>(kb[j], mask, magic);
-#pragma unroll
-              for (int n = 0; n < NT; ++n) {
-                const uint4 b = *reinterpret_cast<const uint4*>(xb + n * 8 * S::PITCH + h * 128 + (j >> 1) * 16);
-                mma(acc[n], a0, a1, a2, a3, b.x, b.y);
-                mma(acc[n], e0, e1, e2, e3, b.z, b.w);
-                if ((h * NT + n) % WM == wm) {        // the warps of the rows share the sums of x
-                  mma(ones[n], kOnes, kOnes, kOnes, kOnes, b.x, b.y);
-                  mma(ones[n], kOnes, kOnes, kOnes, kOnes, b.z, b.w);
-                }
-              }
-            }
-            const float s0 = scale_of(h ? fa[u].y : fa[u].x), s1 = scale_of(h ? fb[u].y : fb[u].x);
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-              y[n][0] = fmaf(s0, acc[n][0], y[n][0]);
-              y[n][1] = fmaf(s0, acc[n][1], y[n][1]);
-              y[n][2] = fmaf(s1, acc[n][2], y[n][2]);
-              y[n][3] = fmaf(s1, acc[n][3], y[n][3]);
-              if ((h * NT + n) % WM == wm && g == 0)
-                *reinterpret_cast<float2*>(xs + ((i * WK + wk) * 2 + h) * TOKENS + n * 8 + 2 * t) =
-                    make_float2(ones[n][0], ones[n][1]);
-            }
-          }
-        }
-        load(i + kAhead, u);
-      }
-    }
+    for (int k = 0; k < 16; ++k) most = max(most, __float_as_uint(f[k]) & 0x7f800000u);
   }
-  asm volatile("cp.async.wait_group 0;" ::: "memory");
-  // groups up to a multiple of 16 count nothing
-  for (int i = 2 * n_blocks * TOKENS + threadIdx.x; i < (2 * n_blocks + 15) / 16 * 16 * TOKENS; i += kThreads) xs[i] = 0.f;
+  most = __reduce_max_sync(0xffffffffu, most);
+  if ((threadIdx.x & 31) == 0) s_most[threadIdx.x >> 5] = most;
   __syncthreads();
-
-  // sum_g z_g X_g - 128 s_g X_g: 16 groups a step, dealt to the warps that share the slice
-  for (int k0 = wk * 16; k0 < 2 * n_blocks; k0 += WK * 16) {
-    uint32_t as[4], az[4];        // (row g, groups 2t, 2t + 1), (row g + 8, same), (row g, + 8), (row g + 8, + 8)
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const int group = k0 + 2 * t + (q >> 1) * 8;
-      uint2 v = make_uint2(0, 0);
-      if (group < 2 * n_blocks)
-        v = __ldg(reinterpret_cast<const uint2*>(p.affine + ((q & 1) ? rb : ra) * (p.width / 16) + (kb0 * 2 + group) * 4));
-      as[q] = __byte_perm(v.x, v.y, 0x5410);
-      az[q] = __byte_perm(v.x, v.y, 0x7632);
+  for (int w = 0; w < 16; ++w) most = max(most, s_most[w]);
+  // times 2^(7 - e): the largest is in [128, 256).  A row with an infinity or a NaN counts as NaN.
+  const int e = max(static_cast<int>(most >> 23), 8);
+  const float up = e == 255 ? CUDART_NAN_F : __uint_as_float(static_cast<uint32_t>(261 - e) << 23);
+  if (threadIdx.x == 0) xs[r] = e == 255 ? CUDART_NAN_F : __uint_as_float(static_cast<uint32_t>(e - 7) << 23);
+  for (int c0 = 0; c0 < width; c0 += 512 * 16) {
+    const int c = c0 + threadIdx.x * 16;       // four threads have a group; beyond the row they have zeros
+    float f[16], sum = 0.f;
+    load(c, f);
+    uint32_t hi[4], lo[4];
+#pragma unroll
+    for (int k = 0; k < 16; ++k) {
+      f[k] *= up;
+      sum += f[k];
     }
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      uint32_t bz[3][2], bs[3][2];
+    for (int h = 0; h < 2; ++h) {
+      constexpr int order[8] = {0, 4, 1, 5, 2, 6, 3, 7};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float a0 = f[8 * h + order[2 * k]], a1 = f[8 * h + order[2 * k + 1]];
+        const __nv_fp8x2_storage_t u = __nv_cvt_float2_to_fp8x2(make_float2(a0, a1), __NV_SATFINITE, __NV_E4M3);
+        const __half2 back(__nv_cvt_fp8x2_to_halfraw2(u, __NV_E4M3));
+        const __nv_fp8x2_storage_t l =
+            __nv_cvt_float2_to_fp8x2(make_float2(a0 - __low2float(back), a1 - __high2float(back)), __NV_SATFINITE, __NV_E4M3);
+        if (k & 1) {
+          hi[2 * h + (k >> 1)] |= static_cast<uint32_t>(u) << 16;
+          lo[2 * h + (k >> 1)] |= static_cast<uint32_t>(l) << 16;
+        } else {
+          hi[2 * h + (k >> 1)] = u;
+          lo[2 * h + (k >> 1)] = l;
+        }
+      }
+    }
+    sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+    sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+    if (c >= width) continue;                  // no shuffles below
+    uint8_t* to = xq + (static_cast<long long>(r / NT) * 2 * NT + r % NT) * width + c;
+    *reinterpret_cast<uint4*>(to) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+    *reinterpret_cast<uint4*>(to + static_cast<long long>(NT) * width) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+    if ((threadIdx.x & 3) == 0) {
+      float rest = sum * 0.25f;
+      uint32_t part[5];
+#pragma unroll
+      for (int k = 0; k < 5; ++k) {
+        const float of = k ? rest : rest * 0.0625f;
+        const __nv_fp8_storage_t v = __nv_cvt_float_to_fp8(of, __NV_SATFINITE, __NV_E4M3);
+        const float back = __half2float(__half(__nv_cvt_fp8_to_halfraw(v, __NV_E4M3)));
+        rest -= k ? back : 16.f * back;
+        part[k] = v;
+      }
+      const uint32_t all = part[0] * 0x01010101u;
+      uint8_t* at = xq + 2ll * gridDim.x * width + (static_cast<long long>(r) * width + c) / 2;
+      *reinterpret_cast<uint4*>(at) = make_uint4(all, all, all, all);
+      *reinterpret_cast<uint4*>(at + 16) = make_uint4(part[1] | part[2] << 8 | part[3] << 16 | part[4] << 24, 0, 0, 0);
+    }
+  }
+}
+
+// blocks an SM: by tensor memory (128 columns with 16 rows of x, else 256) and shared memory
+template <int NT>
+constexpr int blocks_per_sm() { return NT == 16 ? 4 : 2; }
+
+template <int NT>
+__global__ void __launch_bounds__(kThreads, blocks_per_sm<NT>())
+linear_q4_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX,
+                 const __grid_constant__ CUtensorMap tmS, const __grid_constant__ LinearParams p) {
+  constexpr int STAGE = stage_bytes<NT>();
+  constexpr int UNIT = NT == 16 ? 2 : 1;       // groups whose products are there at a time: NT columns, and NT of the ones'
+  constexpr int TMEM_COLUMNS = kProducts + UNIT * 2 * NT <= 128 ? 128 : 256;
+  static_assert(kProducts + UNIT * 2 * NT <= 256 && TMEM_COLUMNS * blocks_per_sm<NT>() <= 512, "tensor memory");
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  __shared__ uint64_t full[kMaxStages], empty[kMaxStages], go[1], done[1];
+  __shared__ uint32_t tmem_slot[1];
+  __shared__ int abort_word;
+  pdl_launch_dependents();
+  volatile int* abort_flag = &abort_word;
+  const AbortCtx ab{abort_flag, p.status};
+  const int warp = warp_uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
+  const int rank = blockIdx.x % p.cluster;
+  const int tokens0 = blockIdx.x / p.cluster % p.token_tiles, tile = blockIdx.x / p.cluster / p.token_tiles;
+  const int blocks = (p.width + kStage - 1) / kStage, per = (blocks + p.cluster - 1) / p.cluster;
+  const int kb0 = rank * per, n_kb = max(min(per, blocks - kb0), 0);
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < p.stages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 4 + 1);             // the warps that read the codes, the MMA
+    }
+    mbar_init(go, 4);
+    mbar_init(done, 1);
+    *abort_flag = 0;
+    mbar_fence_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, TMEM_COLUMNS);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  float* red = reinterpret_cast<float*>(smem);   // [token][128], over the ring once everything has been read
+
+  if (warp == 0) {
+    if (elect_one()) {
+      tma_prefetch_desc(&tmW);
+      tma_prefetch_desc(&tmX);
+      // what runs before may be what writes the weights: they are read after the wait, and only brought into L2 ahead of it
+      for (int i = 0; i < min(n_kb, 4); ++i) tma_prefetch_l2_2d(&tmW, (kb0 + i) * (kStage / 2), tile * 128);
+      pdl_wait();
+      bool ok = true;
+      for (int i = 0, s = 0, ph = 1; i < n_kb; ++i) {
+        if (!wait(&empty[s], ph, ab, ERR_WAIT_EMPTY)) { ok = false; break; }
+        uint8_t* to = smem + s * STAGE;
+        mbar_expect_tx(&full[s], STAGE);
+        tma_load_2d(to, &tmW, &full[s], (kb0 + i) * (kStage / 2), tile * 128);
+        tma_load_2d(to + kCodeBytes, &tmX, &full[s], (kb0 + i) * kStage, tokens0 * 2 * NT);
+        tma_load_2d(to + kCodeBytes + 2 * NT * 128, &tmX, &full[s], (kb0 + i) * kStage + 128, tokens0 * 2 * NT);
+        tma_load_2d(to + kCodeBytes + 4 * NT * 128, &tmS, &full[s], (kb0 + i) * (kStage / 2), tokens0 * NT);
+        if (++s == p.stages) {
+          s = 0;
+          ph ^= 1;
+        }
+      }
+      if (!ok) {
+        // give copies already in flight time to land before the CTA's shared memory goes away
+        const uint64_t t0 = globaltimer_ns();
+        while (globaltimer_ns() - t0 < 200000ull) __nanosleep(1000);
+      }
+    }
+  } else if (warp == 1) {
+    if (elect_one()) {
+      constexpr uint32_t idesc = make_idesc_e4m3(128, NT);
+      bool ok = true;
+      for (int i = 0, s = 0, ph = 0; i < n_kb && ok; ++i) {
+        ok = wait(&full[s], ph, ab, ERR_WAIT_FULL);
+        const uint64_t xdesc = make_smem_desc_sw128(smem_u32(smem + s * STAGE + kCodeBytes), 16, 1024);
+#pragma unroll
+        for (int u = 0; u < 4 / UNIT; ++u) {   // the codes are expanded and the last products have been read
+          ok = ok && wait(go, (i * (4 / UNIT) + u) & 1, ab, ERR_Q4_A);
+          if (!ok) break;
+          tc_fence_after();
+#pragma unroll
+          for (int h = 0; h < UNIT; ++h) {
+            const int g = u * UNIT + h;        // of the stage's four groups
+            tc_mma_ts_e4m3(tmem + kProducts + (h * 2 + 1) * NT, tmem + kFours, xdesc + (uint64_t)((4 * NT * 128 + g * 32) >> 4),
+                           idesc, 0u);
+#pragma unroll
+            for (int k = 0; k < 4; ++k)        // high parts, low parts: two steps of 32 channels each
+              tc_mma_ts_e4m3(tmem + kProducts + h * 2 * NT, tmem + (g & 1) * 16 + (k & 1) * 8,
+                             xdesc + (uint64_t)((((g >> 1) * 2 + (k >> 1)) * NT * 128 + (g & 1) * 64 + (k & 1) * 32) >> 4),
+                             idesc, k != 0 ? 1u : 0u);
+          }
+          tc_commit(done);
+        }
+        if (ok) tc_commit(&empty[s]);
+        if (++s == p.stages) {
+          s = 0;
+          ph ^= 1;
+        }
+      }
+    }
+  } else {
+    const int quad = warp & 3, row = quad * 32 + lane;
+    const uint32_t lane_sel = static_cast<uint32_t>(quad * 32) << 16;
+    const uint2* pairs = reinterpret_cast<const uint2*>(
+        p.affine + static_cast<long long>(min(tile * 128 + row, p.N - 1)) * (p.width / 16)) + 2 * kb0;
+    const int n_pairs = min(2 * n_kb, p.width / 128 - 2 * kb0);   // of 128 channels; the last stage may have one
+    uint32_t r[32];
+    // codes of half a stage: rows of 128 bytes, their 16-byte chunks exchanged by row % 8
+    auto expand = [&](int s, int half) {
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const uint4 w = *reinterpret_cast<const uint4*>(smem + s * STAGE + sw128_offset(row, half * 4 + c));
+        const uint32_t v[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {          // word 4 c + k: channels 64 (k & 1) + 8 (2 c + k / 2) ..
+          const int at = 16 * (k & 1) + 2 * (2 * c + (k >> 1));
+          r[at] = v[k] & 0x0f0f0f0fu;
+          r[at + 1] = (v[k] >> 4) & 0x0f0f0f0fu;
+        }
+      }
+    };
+    auto hand_over = [&] {                     // what this warp wrote and read of tensor memory is done with
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(go);
+    };
+    uint64_t y[NT / 2];                        // two rows of x each
+#pragma unroll
+    for (int c = 0; c < NT / 2; ++c) y[c] = f2_pack(0.f, 0.f);
+    {
+      uint32_t fours[16];
+#pragma unroll
+      for (int c = 0; c < 16; ++c) fours[c] = 0x48484848u;
+      tmem_st16(tmem + kFours + lane_sel, fours);
+    }
+    pdl_wait();
+    uint2 f[2] = {0 < n_pairs ? __ldg(pairs) : make_uint2(0, 0), 1 < n_pairs ? __ldg(pairs + 1) : make_uint2(0, 0)};
+    bool ok = true;
+    if (n_kb > 0) {
+      ok = wait_warp(&full[0], 0, ab, ERR_WAIT_FULL);
+      if (ok) {
+        expand(0, 0);
+        tmem_st_32x32b_x32(tmem + lane_sel, r);
+        tmem_st_wait();
+        hand_over();
+      }
+    }
+    for (int i = 0, s = 0, ph = 0; i < n_kb && ok; ++i) {
+      const int s1 = s + 1 == p.stages ? 0 : s + 1, ph1 = s + 1 == p.stages ? ph ^ 1 : ph;
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
-        const float* at = xs + (k0 + 2 * t + half * 8) * TOKENS + n * 8 + g;
-        float u = at[0], v = at[TOKENS];
+        const int j = 2 * i + half;
+        const bool more = half == 0 || i + 1 < n_kb;
+        const uint2 pair = f[half];
+        f[half] = j + 2 < n_pairs ? __ldg(pairs + j + 2) : make_uint2(0, 0);
+        if (more) {                            // while the products of this half are made
+          if (half == 1) ok = ok && wait_warp(&full[s1], ph1, ab, ERR_WAIT_FULL);
+          if (!ok) break;
+          expand(half == 0 ? s : s1, half ^ 1);
+        }
+        if (half == 0) {
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&empty[s]);
+        }
+        constexpr int COLS = 16;
 #pragma unroll
-        for (int part = 0; part < 3; ++part) {
-          const float hu = __uint_as_float(__float_as_uint(u) & 0xffff0000u), hv = __uint_as_float(__float_as_uint(v) & 0xffff0000u);
-          bz[part][half] = __byte_perm(__float_as_uint(hu), __float_as_uint(hv), 0x7632);
-          bs[part][half] = b200::pack_bf16x2(-128.f * hu, -128.f * hv);
-          u -= hu;
-          v -= hv;
+        for (int u = 0; u < 2 / UNIT; ++u) {
+          ok = ok && wait_warp(done, (j * (2 / UNIT) + u) & 1, ab, ERR_Q4_D);
+          if (!ok) break;
+          tc_fence_after();
+#pragma unroll
+          for (int h = 0; h < UNIT; ++h) {
+            const uint32_t of = u * UNIT + h ? pair.y : pair.x;
+            const float w = 512.f * scale_of(of), z = least_of(of);
+            const uint64_t w2 = f2_pack(w, w), z2 = f2_pack(z, z);
+#pragma unroll
+            for (int c = 0; c < NT; c += COLS) {
+              uint32_t v[COLS], o[COLS];
+              tmem_ld<COLS>(tmem + kProducts + h * 2 * NT + c + lane_sel, v);
+              tmem_ld<COLS>(tmem + kProducts + (h * 2 + 1) * NT + c + lane_sel, o);
+              tmem_ld_wait();
+#pragma unroll
+              for (int k = 0; k < COLS; k += 2)
+                y[(c + k) / 2] = f2_fma(z2, f2_pack(__uint_as_float(o[k]), __uint_as_float(o[k + 1])),
+                                        f2_fma(w2, f2_pack(__uint_as_float(v[k]), __uint_as_float(v[k + 1])), y[(c + k) / 2]));
+            }
+          }
+          if (u + 1 < 2 / UNIT) hand_over();   // the half's second group
+        }
+        if (!ok) break;
+        if (more) {
+          tmem_st_32x32b_x32(tmem + lane_sel, r);
+          tmem_st_wait();
+          hand_over();
         }
       }
+      s = s1;
+      ph = ph1;
+    }
+    // every product has been made, so every copy has landed and every operand has been used: the ring is free
 #pragma unroll
-      for (int part = 0; part < 3; ++part) {
-        mma(y[n], as[0], as[1], as[2], as[3], bs[part][0], bs[part][1]);
-        mma(y[n], az[0], az[1], az[2], az[3], bz[part][0], bz[part][1]);
-      }
+    for (int c = 0; c < NT; c += 2) {
+      float u, v;
+      f2_unpack(y[c / 2], u, v);
+      red[c * 128 + row] = u;
+      red[(c + 1) * 128 + row] = v;
     }
   }
-
-  // partial sums [wk][token][16 WM rows] over the stages of x
-  constexpr int ROWS = 16 * WM;
-  float* part = reinterpret_cast<float*>(smem);
-#pragma unroll
-  for (int n = 0; n < NT; ++n)
-#pragma unroll
-    for (int c = 0; c < 4; ++c)
-      part[(wk * TOKENS + n * 8 + 2 * t + (c & 1)) * ROWS + wm * 16 + g + (c >> 1) * 8] = y[n][c];
+  __syncwarp();
+  tc_fence_before();
   if (p.cluster > 1)
     cluster_sync();
   else
     __syncthreads();
-  const int share = ROWS / p.cluster;             // weight rows that this rank finishes
-  for (int it = threadIdx.x; it < p.rows * share; it += kThreads) {
-    const int token = it / share, r = rank * share + (it - token * share), n = tile * ROWS + r;
-    float v = 0.f;
-    for (int c = 0; c < p.cluster; ++c)
-#pragma unroll
-      for (int k = 0; k < WK; ++k) {
-        const float* at = part + (k * TOKENS + token) * ROWS + r;
-        v += p.cluster == 1 ? *at : ld_cluster(b200::smem_u32(at), c);
-      }
-    if (n < p.N) p.out[token * p.ldo + n] = __float2bfloat16(v);
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, TMEM_COLUMNS);
   }
-  if (p.cluster > 1) cluster_sync();              // peers may still read this block's sums
+
+  // weight rows [rank, rank + 1) * 128 / cluster, summed over the cluster in rank order
+  pdl_wait();   // what the output replaces may still be read by the predecessor
+  const int width = 128 / p.cluster, vecs = width >> 2;
+  const int rows = min(p.rows - tokens0 * NT, NT);
+  for (int it = threadIdx.x; it < rows * vecs; it += kThreads) {
+    const int token = it / vecs, nl = rank * width + (it - token * vecs) * 4, n = tile * 128 + nl;
+    if (n >= p.N) continue;
+    const float* at = red + token * 128 + nl;
+    float4 v = *reinterpret_cast<const float4*>(at);
+    if (p.cluster > 1) {
+      v = ld_cluster4(smem_u32(at), 0);
+      for (int r = 1; r < p.cluster; ++r) {
+        const float4 w = ld_cluster4(smem_u32(at), r);
+        v.x += w.x;
+        v.y += w.y;
+        v.z += w.z;
+        v.w += w.w;
+      }
+    }
+    const float scale = p.xs[tokens0 * NT + token];
+    v.x *= scale;
+    v.y *= scale;
+    v.z *= scale;
+    v.w *= scale;
+    __nv_bfloat16* dst = p.out + (tokens0 * NT + token) * p.ldo + n;
+    if (((p.N | p.ldo) & 3) == 0) {
+      *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16x2(v.x, v.y), pack_bf16x2(v.z, v.w));
+    } else {
+      const float e[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (n + i < p.N) dst[i] = __float2bfloat16(e[i]);
+    }
+  }
+  if (p.cluster > 1) {
+    __syncwarp();
+    cluster_sync();   // peers may still read this block's sums
+  }
 }
 
 // Rows of up to 64 channels (one group, words in channel order): one warp per weight row and eight rows of x, a lane per word.
-__global__ void __launch_bounds__(128) linear_q4_narrow_kernel(const __grid_constant__ LinearParams p) {
+__global__ void __launch_bounds__(128) linear_q4_narrow_kernel(const __nv_bfloat16* x, long long ldx, const uint32_t* codes,
+                                                               const uint32_t* affine, __nv_bfloat16* out, long long ldo,
+                                                               int rows, int N, int K) {
   const int n = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31, m0 = blockIdx.y * 8;
-  b200::pdl_launch_dependents();
-  b200::pdl_wait();
-  if (n >= p.N) return;
-  const int m1 = min(p.rows - m0, 8), c = (lane & 7) * 8;
-  const uint32_t a = reinterpret_cast<const uint32_t*>(p.affine)[n];
+  pdl_launch_dependents();
+  pdl_wait();
+  if (n >= N) return;
+  const int m1 = min(rows - m0, 8), c = (lane & 7) * 8;
+  const uint32_t a = affine[n];
   float acc[8] = {}, v[8];
-  unpack(lane < 8 ? reinterpret_cast<const uint32_t*>(p.codes)[static_cast<long long>(n) * 8 + lane] : 0u, v);
+  unpack(lane < 8 ? codes[static_cast<long long>(n) * 8 + lane] : 0u, v);
 #pragma unroll
   for (int i = 0; i < 8; ++i) v[i] = fmaf(v[i], scale_of(a), least_of(a));
 #pragma unroll
@@ -288,72 +498,79 @@ __global__ void __launch_bounds__(128) linear_q4_narrow_kernel(const __grid_cons
     if (m >= m1) break;
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-      if (lane < 8 && c + i < p.K) acc[m] = fmaf(__bfloat162float(p.x[(m0 + m) * p.ldx + c + i]), v[i], acc[m]);
+      if (lane < 8 && c + i < K) acc[m] = fmaf(__bfloat162float(x[(m0 + m) * ldx + c + i]), v[i], acc[m]);
   }
 #pragma unroll
   for (int m = 0; m < 8; ++m) {
 #pragma unroll
     for (int off = 4; off > 0; off >>= 1) acc[m] += __shfl_xor_sync(0xffffffffu, acc[m], off);
-    if (lane == 0 && m < m1) p.out[(m0 + m) * p.ldo + n] = __float2bfloat16(acc[m]);
+    if (lane == 0 && m < m1) out[(m0 + m) * ldo + n] = __float2bfloat16(acc[m]);
   }
 }
 
-template <int NT, int WM>
-int launch(LinearParams p, int cluster, cudaStream_t stream) {
-  using S = Shape<NT, WM>;
-  auto* kern = linear_q4_kernel<NT, WM>;
-  p.cluster = cluster;
-  const int blocks = p.width / 128, slice = (blocks + cluster - 1) / cluster;
-  const int bytes = S::RING_BYTES + S::xs_bytes(slice);
-  if (bytes > 226 * 1024) return b200host::RC_TOO_LARGE;
+template <int NT>
+int launch(const CUtensorMap& tmW, const CUtensorMap& tmX, const CUtensorMap& tmS, LinearParams p, cudaStream_t stream) {
+  auto* kern = linear_q4_kernel<NT>;
+  const int blocks = (p.width + kStage - 1) / kStage, slice = (blocks + p.cluster - 1) / p.cluster;
+  p.stages = (222 * 1024 / blocks_per_sm<NT>() - 2048) / stage_bytes<NT>();
+  if (p.stages > kMaxStages) p.stages = kMaxStages;
+  if (p.stages > slice) p.stages = slice;
+  if (p.stages < 2) p.stages = 2;
+  const int ring = p.stages * stage_bytes<NT>(), sums = NT * 128 * 4;   // the partial sums reuse the ring
+  const int smem_bytes = (ring > sums ? ring : sums) + 1024;
   static bool configured[b200host::kMaxDevices] = {};
-  if (int rc = b200host::ensure_dynamic_smem(kern, 226 * 1024, configured)) return rc;
+  if (int rc = b200host::ensure_dynamic_smem(kern, 200 * 1024, configured)) return rc;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((p.N + 16 * WM - 1) / (16 * WM) * cluster);
+  cfg.gridDim = dim3((p.N + 127) / 128 * p.token_tiles * p.cluster);
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = bytes;
+  cfg.dynamicSmemBytes = smem_bytes;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = cluster;
+  attr[0].val.clusterDim.x = p.cluster;
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = b200host::pdl_enabled() ? 2 : 1;
-  return static_cast<int>(cudaLaunchKernelEx(&cfg, kern, p));
-}
-
-template <int NT>
-int launch_rows(const LinearParams& p, int wm, int cluster, cudaStream_t s) {
-  switch (wm) {
-    case 1:
-      if constexpr (NT <= 2) return launch<NT, 1>(p, cluster, s);
-      return b200host::RC_BAD_SHAPE;
-    case 2: return launch<NT, 2>(p, cluster, s);
-    case 4: return launch<NT, 4>(p, cluster, s);
-    case 8: return launch<NT, 8>(p, cluster, s);
-    default: return b200host::RC_BAD_SHAPE;
-  }
+  return static_cast<int>(cudaLaunchKernelEx(&cfg, kern, tmW, tmX, tmS, p));
 }
 
 }  // namespace
 
-// out [rows, N] (row stride ldo) = x [rows, K] (ldx) * W^T, W as codes [N, width / 8] words and affine [N, width / 64] pairs.
-// Blocks of 16 wm weight rows (wm 1, 2, 4 or 8), `cluster` (1, 2, 4 or 8) slices of K.
+// out [rows, N] (row stride ldo) = x [rows, K] (ldx) * W^T, W as codes [N, width / 8] words and affine [N, width / 64] pairs;
+// rows <= 64, `cluster` (1, 2, 4 or 8) slices of K.  `work` is the call's own: with R = rows rounded up to 16 (up to 16 rows) or
+// 32 and width = K rounded up to 256, 5 * R * width / 2 bytes and then R floats (none of it for up to 64 channels).
 extern "C" int b200_q4_linear(const void* x, long long ldx, const void* codes, const void* affine, void* out,
-                              long long ldo, int rows, int N, int K, int wm, int cluster, void* stream) {
-  if (rows <= 0 || rows > 64 || N <= 0 || K <= 0 || K > (1 << 30)) return b200host::RC_BAD_SHAPE;
-  if (cluster != 1 && cluster != 2 && cluster != 4 && cluster != 8) return b200host::RC_BAD_SHAPE;
-  if ((reinterpret_cast<uintptr_t>(codes) | reinterpret_cast<uintptr_t>(affine)) & 15) return b200host::RC_BAD_ALIGNMENT;
-  LinearParams p{(const __nv_bfloat16*)x, ldx, ldo, (const uint8_t*)codes, (const uint8_t*)affine, (__nv_bfloat16*)out,
-                 rows, N, K, row_width(K), 1, (ldx % 8 == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0) ? 1 : 0};
+                              long long ldo, int rows, int N, int K, int cluster, void* work, void* status,
+                              void* stream) {
+  using namespace b200host;
+  if (rows <= 0 || rows > 64 || N <= 0 || K <= 0 || K > (1 << 30) || !status) return RC_BAD_SHAPE;
+  if (cluster != 1 && cluster != 2 && cluster != 4 && cluster != 8) return RC_BAD_SHAPE;
+  if ((reinterpret_cast<uintptr_t>(codes) | reinterpret_cast<uintptr_t>(affine)) & 15) return RC_BAD_ALIGNMENT;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  if (p.width == 64)
-    return static_cast<int>(b200host::launch_kernel(linear_q4_narrow_kernel, dim3((N + 3) / 4, (rows + 7) / 8), dim3(128), 0,
-                                                    s, b200host::pdl_enabled() != 0, p));
-  if (rows <= 8) return launch_rows<1>(p, wm, cluster, s);
-  if (rows <= 16) return launch_rows<2>(p, wm, cluster, s);
-  if (rows <= 32) return launch_rows<4>(p, wm, cluster, s);
-  return launch_rows<8>(p, wm, cluster, s);
+  const int width = row_width(K);
+  const bool pdl = pdl_enabled() != 0;
+  if (width == 64)
+    return static_cast<int>(launch_kernel(linear_q4_narrow_kernel, dim3((N + 3) / 4, (rows + 7) / 8), dim3(128), 0, s, pdl,
+                                          (const __nv_bfloat16*)x, ldx, (const uint32_t*)codes, (const uint32_t*)affine,
+                                          (__nv_bfloat16*)out, ldo, rows, N, K));
+  if (!work || ((reinterpret_cast<uintptr_t>(work) & 15) | (reinterpret_cast<uintptr_t>(out) & 7))) return RC_BAD_ALIGNMENT;
+  const int NT = rows <= 16 ? 16 : 32, tiles = (rows + NT - 1) / NT, tokens = NT * tiles;
+  const int xwidth = (K + kStage - 1) / kStage * kStage;
+  uint8_t* xq = static_cast<uint8_t*>(work);
+  uint8_t* sums = xq + 2ll * tokens * xwidth;
+  float* xs = reinterpret_cast<float*>(sums + tokens * (xwidth / 2ll));
+  CUtensorMap tmW, tmX, tmS;
+  int rc;
+  if ((rc = make_map_2d(&tmW, CU_TENSOR_MAP_DATA_TYPE_UINT8, codes, width / 2, N, width / 2, 128, 128))) return rc;
+  if ((rc = make_map_2d(&tmX, CU_TENSOR_MAP_DATA_TYPE_UINT8, xq, xwidth, 2 * tokens, xwidth, 128, 2 * NT))) return rc;
+  if ((rc = make_map_2d(&tmS, CU_TENSOR_MAP_DATA_TYPE_UINT8, sums, xwidth / 2, tokens, xwidth / 2, 128, NT))) return rc;
+  const int aligned = ldx % 8 == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0;
+  if (cudaError_t e = launch_kernel(linear_q4_split_kernel, dim3(tokens), dim3(512), 0, s, pdl, (const __nv_bfloat16*)x, ldx,
+                                    rows, K, xwidth, NT, aligned, xq, xs))
+    return static_cast<int>(e);
+  LinearParams p{(const uint8_t*)affine, xs, (__nv_bfloat16*)out, ldo, rows, N, width, cluster, 0, tiles,
+                 (int*)status};
+  return NT == 16 ? launch<16>(tmW, tmX, tmS, p, s) : launch<32>(tmW, tmX, tmS, p, s);
 }

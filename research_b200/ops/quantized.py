@@ -425,24 +425,52 @@ def linear_q4(x: torch.Tensor, w: Q4Rows) -> torch.Tensor:
         if x2.stride(1) != 1:
             x2 = x2.contiguous()
         out = torch.empty(rows, N, dtype=torch.bfloat16, device=x.device)
-        native._check((native._lib or native.load()).b200_q4_linear(x2.data_ptr(), x2.stride(0), w.codes.data_ptr(), w.affine.data_ptr(),
-                                                   out.data_ptr(), N, rows, N, K, *linear_shape(rows, N, K),
-                                                   native._stream()), "b200_q4_linear")
+        work = None
+        if K > GROUP:                                   # x as the kernel multiplies it: two e4m3 parts, a scale per row
+            tokens, width = 16 if rows <= 16 else -(-rows // 32) * 32, -(-K // 256) * 256
+            work = torch.empty(tokens * (2 * width + width // 2 + 4), dtype=torch.uint8, device=x.device)
+        native._check((native._lib or native.load()).b200_q4_linear(
+            x2.data_ptr(), x2.stride(0), w.codes.data_ptr(), w.affine.data_ptr(), out.data_ptr(), N, rows, N, K,
+            linear_slices(rows, N, K), native._ptr(work), native.status_word(x.device).data_ptr(), native._stream()),
+            "b200_q4_linear")
+    native.LAUNCHES += work is not None                 # _check counts one launch; the split of x is another
     return out.view(*x.shape[:-1], N)
 
 
+def _rows_on_16_bytes(x: torch.Tensor) -> torch.Tensor:
+    """``x [rows, K]`` as tensor maps take it: dense rows that start on 16 bytes (a copy where they do not)."""
+
+    if x.stride(1) == 1 and x.stride(0) % 8 == 0 and x.stride(0) >= x.shape[1] and x.data_ptr() % 16 == 0:
+        return x
+    return F.pad(x, (0, -x.shape[1] % 8))[:, :x.shape[1]] if x.shape[1] % 8 else x.clone(memory_format=torch.contiguous_format)
+
+
 @functools.lru_cache(maxsize=4096)
-def linear_shape(rows: int, n: int, k: int) -> tuple[int, int]:
-    return 2, 1
+def linear_slices(rows: int, n: int, k: int, sms: int = 148) -> int:
+    """Slices of K (1, 2, 4 or 8 blocks of a cluster) for a product with 4-bit weights: the count of least estimated time.
+    A stage of 256 channels takes a block 0.65 us (1.4 with more than 16 rows of x) by itself and an SM 0.55 (0.8) where
+    several of its up to four (two) blocks share it; slices add the exchange of partial sums.  Measured with 1 / 32 rows:
+    2048 x 2048 1 / 2 / 4 / 8 slices 10.7 / 8.5 / 6.9 / 6.3 and 15.6 / 11.0 / 8.8 / 8.5 us, 11264 x 2048 11.8 / 10.2 / 9.8 / 13.7
+    and 16.8 / 12.5 / 16.6 / 23.0 us, 28672 x 4096 31.5 / 22.5 / 26.6 / 33.6 and 30.7 / 37.0 / 45.1 / 61.2 us."""
+
+    alone, shared, room = (0.65, 0.55, 4) if rows <= 16 else (1.4, 0.8, 2)
+    tiles, stages = -(-n // 128) * -(-rows // 32), -(-k // 256)
+    best, best_cost = 1, float("inf")
+    for s, exchange in ((1, 0.0), (2, 1.1), (4, 1.6), (8, 2.2)):
+        if s > 1 and stages < s:
+            break
+        per_sm = math.ceil(tiles * s / sms - 0.1)
+        waves = -(-per_sm // room)                      # of blocks, each with 2.5 us to begin and to end
+        cost = -(-stages // s) * max(alone, (per_sm if waves == 1 else waves * room) * shared) + exchange + (waves - 1) * 2.5
+        if cost < best_cost:
+            best, best_cost = s, cost
+    return best
 
 
 def _expanded_linear(x: torch.Tensor, w: Q4Rows) -> torch.Tensor:
     (rows, K), N = x.shape, w.codes.shape[0]
-    full = _expand(w)
-    if x.stride(1) != 1 or x.stride(0) % 8 or x.stride(0) < K or x.data_ptr() % 16:
-        x = F.pad(x, (0, full.shape[1] - K))            # the GEMM's rows start on 16 bytes
-    full = full[:, :x.shape[1]]
+    full = _expand(w)[:, :K]
     ld = -(-N // 8) * 8
     out = torch.empty(rows, ld, dtype=torch.bfloat16, device=x.device)
-    native.gemm(x, full, out=out[:, :N])
+    native.gemm(_rows_on_16_bytes(x), full, out=out[:, :N])
     return out if ld == N else out[:, :N].contiguous()
