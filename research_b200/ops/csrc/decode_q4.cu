@@ -58,15 +58,6 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t v) {
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
   return r;
 }
-// codes P of both halves of w as bf16 128 + n: one shift and one three-input operation (a & b) | c, whose constants are kept
-// in registers, since an instruction has room for one
-template <int P>
-__device__ __forceinline__ uint32_t coded(uint32_t w, uint32_t mask, uint32_t magic) {
-  uint32_t r;
-  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(P ? w >> (4 * P) : w), "r"(mask), "r"(magic));
-  return r;
-}
-
 constexpr uint32_t kOnes = 0x3f803f80u;
 
 // Rows of sequence b that count: [first, end), in tiles of TR rows from tile_lo to tile_hi (none: tile_lo = tile_hi).
@@ -237,8 +228,8 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS) decode_q4_kernel(const __g
     cp_async_commit();
   }
 
-  uint32_t mask = 0x000f000fu, magic = 0x43004300u;
-  asm volatile("" : "+r"(mask), "+r"(magic));
+  uint32_t mask, magic;
+  opaque_masks(mask, magic);
   const int pi = (g & 1) ? 7 - (g >> 1) : g >> 1;
   const float low = (!WIDE && t >= 2) ? 1.f : 0.f;
   uint32_t qf[KW][4];

@@ -1,5 +1,6 @@
 // 4-bit rows (quant4.cuh): a K/V cache that is quantised as it is written and read back, and whole matrices.
 #include <math_constants.h>
+#include <string.h>
 
 #include "quant4.cuh"
 #include "host_util.cuh"
@@ -14,74 +15,122 @@ struct KvParams {
   uint32_t* codes[2];                 // [B, pages, Hkv, page_rows, D / 8] words
   uint32_t* affine[2];                // [B, pages, Hkv, page_rows, D / 64]
   const int* start;                   // [B] or null: first row of each sequence
-  long long row[2], batch[2];         // element strides of src
-  int B, T, Hkv, D, pages, page_rows;
+  long long batch[2];                 // element strides of src
+  int row[2];
+  int T, Hkv, pages, page_rows, blocks;   // blocks of a sequence
+  Divisor per_block, per_token, per_page;
 };
 
-// index of a cache row among the rows of the pool, or -1 outside the cache
-__device__ __forceinline__ long long pool_row(const KvParams& p, int b, int h, int t) {
-  const long long r = (p.start ? p.start[b] : 0) + static_cast<long long>(t);
-  if (r < 0 || r >= static_cast<long long>(p.pages) * p.page_rows) return -1;
-  const int pg = static_cast<int>(r) / p.page_rows, in = static_cast<int>(r) - pg * p.page_rows;
-  return ((static_cast<long long>(b) * p.pages + pg) * p.Hkv + h) * p.page_rows + in;
+constexpr int kItems = 4;             // words of a thread, their loads all under way at once
+constexpr uint32_t kThreads = 256;
+
+// A thread's words among those of a sequence's new rows, counted over (token, head, word): this one, and 256 further on.
+struct Walk {
+  uint32_t token, e;                  // e: word of the token's row over all heads
+  __device__ __forceinline__ Walk(const KvParams& p, uint32_t j) : token(p.per_token.of(j)), e(j - token * p.per_token.d) {}
+  __device__ __forceinline__ void next(const KvParams& p, uint32_t tokens, uint32_t rest) {
+    token += tokens;
+    e += rest;
+    if (e >= p.per_token.d) {
+      e -= p.per_token.d;
+      ++token;
+    }
+  }
+};
+
+// Row of a sequence in its cache as 32 bits without sign: whatever start + token is, it is below the capacity only if it is a
+// row of the cache (both are below 2^31).
+__device__ __forceinline__ uint32_t row_of(int first, const Walk& at) { return static_cast<uint32_t>(first) + at.token; }
+// Pool row of a token's head.
+template <int D>
+__device__ __forceinline__ uint64_t pool_row(const KvParams& p, uint64_t seq_row, uint32_t r, const Walk& at) {
+  constexpr uint32_t WORDS = D / 8;
+  const uint32_t pg = p.per_page.of(r), in = r - pg * p.per_page.d;
+  return seq_row + in + static_cast<uint64_t>(pg * p.Hkv + at.e / WORDS) * p.per_page.d;
+}
+// word of a pool row for word e of the token
+template <int D>
+__device__ __forceinline__ uint32_t word_at(uint32_t e) {
+  const uint32_t c = e % (D / 8);
+  return D == 128 ? 2 * (c & 7) + (c >> 3) : c;
 }
 
-// A lane per word: eight lanes share a group and find its least and largest value.
+// Quantise as it is written: a lane per word, eight lanes share a group and find its least and largest value in bf16 (which
+// they are).  Bound by the reads (2 bytes a channel) as long as the arithmetic stays near 15 instructions a channel: eight
+// prompts of 4096 rows of 8 heads of 128, 172 MB, in KVWRITE us.
+template <int D>
 __global__ void __launch_bounds__(256) kv_write_q4_kernel(const __grid_constant__ KvParams p) {
-  const int per = p.D / 8, which = blockIdx.y;
-  const long long total = static_cast<long long>(p.B) * p.T * p.Hkv * per;
+  const int which = blockIdx.y, b = static_cast<int>(p.per_block.of(blockIdx.x)), block = blockIdx.x - b * p.blocks;
   b200::pdl_launch_dependents();
   b200::pdl_wait();
-  const long long step = static_cast<long long>(gridDim.x) * blockDim.x;
-  for (long long i0 = static_cast<long long>(blockIdx.x) * blockDim.x; i0 < total; i0 += step) {
-    const long long i = min(i0 + threadIdx.x, total - 1);      // whole groups of lanes stay together for the shuffles
-    const int c = static_cast<int>(i % per);
-    const long long token_head = i / per;
-    const int h = static_cast<int>(token_head % p.Hkv);
-    const long long token = token_head / p.Hkv;
-    const int t = static_cast<int>(token % p.T), b = static_cast<int>(token / p.T);
-    float x[8];
-    unpack_bf16(*reinterpret_cast<const uint4*>(p.src[which] + b * p.batch[which] + t * p.row[which] + h * p.D + c * 8), x);
-    float least = x[0], most = x[0];
+  const int first = p.start ? p.start[b] : 0;
+  const uint32_t total = static_cast<uint32_t>(p.T) * p.per_token.d, j0 = block * (kThreads * kItems) + threadIdx.x;
+  const uint32_t tokens = p.per_token.of(kThreads), rest = kThreads - tokens * p.per_token.d;
+  const __nv_bfloat16* src = p.src[which] + b * p.batch[which];
+  uint4 v[kItems];
+  {
+    Walk at(p, j0);
 #pragma unroll
-    for (int j = 1; j < 8; ++j) {
-      least = min_nan(least, x[j]);
-      most = max_nan(most, x[j]);
-    }
+    for (int k = 0; k < kItems; ++k, at.next(p, tokens, rest))   // beyond the rows: the last one's word, whose group is whole too
+      v[k] = *reinterpret_cast<const uint4*>(src + static_cast<long long>(min(at.token, p.T - 1u)) * p.row[which] + at.e * 8);
+  }
+  const uint64_t seq_row = static_cast<uint64_t>(b) * p.pages * p.Hkv * p.page_rows;
+  const uint32_t capacity = static_cast<uint32_t>(p.pages) * p.page_rows;
+  Walk at(p, j0);
 #pragma unroll
-    for (int off = 4; off > 0; off >>= 1) {
-      least = min_nan(least, __shfl_xor_sync(0xffffffffu, least, off));
-      most = max_nan(most, __shfl_xor_sync(0xffffffffu, most, off));
-    }
+  for (int k = 0; k < kItems; ++k, at.next(p, tokens, rest)) {
+    const uint32_t j = j0 + k * kThreads;
+    if (j - (threadIdx.x & 31) >= total) break;           // the whole warp is beyond
+    __nv_bfloat162 w[4];
+    memcpy(w, &v[k], 16);
+    const __nv_bfloat162 lo = __hmin2_nan(__hmin2_nan(w[0], w[1]), __hmin2_nan(w[2], w[3]));
+    const __nv_bfloat162 hi = __hmax2_nan(__hmax2_nan(w[0], w[1]), __hmax2_nan(w[2], w[3]));
+    // (least, -largest), so that one minimum serves both
+    __nv_bfloat162 m = __halves2bfloat162(__hmin_nan(lo.x, lo.y), __hneg(__hmax_nan(hi.x, hi.y)));
+#pragma unroll
+    for (int off = 4; off > 0; off >>= 1) m = __hmin2_nan(m, __shfl_xor_sync(0xffffffffu, m, off));
+    const float least = __low2float(m), most = -__high2float(m);
     const uint32_t affine = (__float_as_uint(least) & 0xffff0000u) | scale_bits(least, most);
+    float x[8];
+    unpack_bf16(v[k], x);
     const uint32_t word = pack(x, affine);
-    const long long r = pool_row(p, b, h, t);
-    if (r < 0 || i0 + threadIdx.x >= total) continue;
-    const int g = c & 7, half = c >> 3;
-    p.codes[which][r * per + (per == 8 ? g : 2 * g + half)] = word;
-    if (g == 0) p.affine[which][r * (per >> 3) + half] = affine;
+    const uint32_t r = row_of(first, at);
+    if (j >= total || r >= capacity) continue;
+    const uint64_t row = pool_row<D>(p, seq_row, r, at);
+    p.codes[which][row * (D / 8) + word_at<D>(at.e)] = word;
+    if ((at.e & 7) == 0) p.affine[which][row * (D / 64) + at.e % (D / 8) / 8] = affine;
   }
 }
 
+// Read back: a lane per word, 16 bytes written.
+template <int D>
 __global__ void __launch_bounds__(256) kv_read_q4_kernel(const __grid_constant__ KvParams p) {
-  const int per = p.D / 8, which = blockIdx.y;
-  const long long total = static_cast<long long>(p.B) * p.T * p.Hkv * per;
+  const int which = blockIdx.y, b = static_cast<int>(p.per_block.of(blockIdx.x)), block = blockIdx.x - b * p.blocks;
   b200::pdl_launch_dependents();
   b200::pdl_wait();
-  const long long step = static_cast<long long>(gridDim.x) * blockDim.x;
-  for (long long i = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x; i < total; i += step) {
-    const int c = static_cast<int>(i % per);
-    const long long token_head = i / per;
-    const int h = static_cast<int>(token_head % p.Hkv);
-    const long long token = token_head / p.Hkv;
-    const int t = static_cast<int>(token % p.T), b = static_cast<int>(token / p.T);
-    const long long r = pool_row(p, b, h, t);
-    const int g = c & 7, half = c >> 3;
-    uint4 v = make_uint4(0, 0, 0, 0);
-    if (r >= 0)
-      v = values_bf16(p.codes[which][r * per + (per == 8 ? g : 2 * g + half)], p.affine[which][r * (per >> 3) + half]);
-    *reinterpret_cast<uint4*>(p.dst[which] + i * 8) = v;
+  const int first = p.start ? p.start[b] : 0;
+  const uint32_t total = static_cast<uint32_t>(p.T) * p.per_token.d, j0 = block * (kThreads * kItems) + threadIdx.x;
+  const uint32_t tokens = p.per_token.of(kThreads), rest = kThreads - tokens * p.per_token.d;
+  const uint64_t seq_row = static_cast<uint64_t>(b) * p.pages * p.Hkv * p.page_rows;
+  const uint32_t capacity = static_cast<uint32_t>(p.pages) * p.page_rows;
+  uint32_t word[kItems], affine[kItems];
+  Walk at(p, j0);
+#pragma unroll
+  for (int k = 0; k < kItems; ++k, at.next(p, tokens, rest)) {
+    word[k] = affine[k] = 0;                              // a row that the cache does not have reads as zeros
+    const uint32_t r = row_of(first, at);
+    if (j0 + k * kThreads < total && r < capacity) {
+      const uint64_t row = pool_row<D>(p, seq_row, r, at);
+      word[k] = p.codes[which][row * (D / 8) + word_at<D>(at.e)];
+      affine[k] = p.affine[which][row * (D / 64) + at.e % (D / 8) / 8];
+    }
   }
+  uint32_t mask, magic;
+  opaque_masks(mask, magic);
+  uint4* to = reinterpret_cast<uint4*>(p.dst[which]) + static_cast<long long>(b) * total;
+#pragma unroll
+  for (int k = 0; k < kItems; ++k)
+    if (j0 + k * kThreads < total) to[j0 + k * kThreads] = values_bf16(word[k], affine[k], mask, magic);
 }
 
 // Whole matrices (weights, once): eight lanes per group, any number of channels and any row stride.
@@ -134,13 +183,15 @@ __global__ void __launch_bounds__(256) dequantize_rows_q4_kernel(const uint32_t*
   const int words = width / 8;
   const long long total = rows * words;
   const long long step = static_cast<long long>(gridDim.x) * blockDim.x;
+  uint32_t mask, magic;
+  opaque_masks(mask, magic);
   b200::pdl_launch_dependents();
   b200::pdl_wait();
   for (long long i = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x; i < total; i += step) {
     const long long row = i / words;
     const int w = static_cast<int>(i - row * words);
     *reinterpret_cast<uint4*>(out + row * width + word_channel(w, width)) =
-        values_bf16(codes[i], affine[row * (width / kGroup) + word_group(w, width)]);
+        values_bf16(codes[i], affine[row * (width / kGroup) + word_group(w, width)], mask, magic);
   }
 }
 
@@ -151,7 +202,20 @@ int blocks_for(long long items) {
 
 bool kv_shape_ok(int B, int T, int Hkv, int D, int pages, int page_rows) {
   return B > 0 && T > 0 && Hkv > 0 && (D == 64 || D == 128) && pages > 0 && page_rows > 0 &&
-         static_cast<long long>(pages) * page_rows <= 0x7fffffffll;
+         static_cast<long long>(pages) * page_rows <= 0x7fffffffll &&
+         static_cast<long long>(pages) * Hkv <= 0x7fffffffll && static_cast<long long>(T) * Hkv * (D / 8) <= 0x7ffff000ll &&
+         static_cast<long long>(B) * (static_cast<long long>(T) * Hkv * (D / 8) / (kThreads * kItems) + 1) <= 0x7fffffffll;
+}
+
+template <typename Kern>
+int launch_kv(Kern* kern64, Kern* kern128, KvParams p, int B, int D, void* stream) {
+  const uint32_t words = static_cast<uint32_t>(p.Hkv) * (D / 8);
+  p.blocks = static_cast<int>((static_cast<uint32_t>(p.T) * words + kThreads * kItems - 1) / (kThreads * kItems));
+  p.per_block = Divisor(p.blocks);
+  p.per_token = Divisor(words);
+  p.per_page = Divisor(p.page_rows);
+  return static_cast<int>(b200host::launch_kernel(D == 64 ? kern64 : kern128, dim3(B * p.blocks, 2), dim3(kThreads), 0,
+                                                  reinterpret_cast<cudaStream_t>(stream), b200host::pdl_enabled() != 0, p));
 }
 
 }  // namespace
@@ -163,16 +227,15 @@ extern "C" int b200_q4_kv_write(const void* k, const void* v, long long k_row, l
                                 const void* start, int B, int T, int Hkv, int D, int pages, int page_rows, void* stream) {
   if (!kv_shape_ok(B, T, Hkv, D, pages, page_rows)) return b200host::RC_BAD_SHAPE;
   if ((k_row | k_batch | v_row | v_batch) & 7) return b200host::RC_BAD_ALIGNMENT;
+  if (k_row < 0 || v_row < 0 || k_row > 0x7fffffff || v_row > 0x7fffffff) return b200host::RC_TOO_LARGE;
   if ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15) return b200host::RC_BAD_ALIGNMENT;
   if ((reinterpret_cast<uintptr_t>(k_codes) | reinterpret_cast<uintptr_t>(v_codes) |
        reinterpret_cast<uintptr_t>(k_affine) | reinterpret_cast<uintptr_t>(v_affine)) & 15)
     return b200host::RC_BAD_ALIGNMENT;
   KvParams p{{(const __nv_bfloat16*)k, (const __nv_bfloat16*)v}, {nullptr, nullptr},
              {(uint32_t*)k_codes, (uint32_t*)v_codes}, {(uint32_t*)k_affine, (uint32_t*)v_affine}, (const int*)start,
-             {k_row, v_row}, {k_batch, v_batch}, B, T, Hkv, D, pages, page_rows};
-  return static_cast<int>(b200host::launch_kernel(
-      kv_write_q4_kernel, dim3(blocks_for((long long)B * T * Hkv * (D / 8)), 2), dim3(256), 0,
-      reinterpret_cast<cudaStream_t>(stream), b200host::pdl_enabled() != 0, p));
+             {k_batch, v_batch}, {(int)k_row, (int)v_row}, T, Hkv, pages, page_rows, 0, {}, {}, {}};
+  return launch_kv(kv_write_q4_kernel<64>, kv_write_q4_kernel<128>, p, B, D, stream);
 }
 
 // The same rows as bf16 into k, v [B, T, Hkv, D] contiguous; rows outside the cache read as zeros.
@@ -185,11 +248,9 @@ extern "C" int b200_q4_kv_read(void* k, void* v, const void* k_codes, const void
        reinterpret_cast<uintptr_t>(v_affine)) & 15)
     return b200host::RC_BAD_ALIGNMENT;
   KvParams p{{nullptr, nullptr}, {(__nv_bfloat16*)k, (__nv_bfloat16*)v}, {(uint32_t*)k_codes, (uint32_t*)v_codes},
-             {(uint32_t*)k_affine, (uint32_t*)v_affine}, (const int*)start, {0, 0}, {0, 0}, B, T, Hkv, D, pages,
-             page_rows};
-  return static_cast<int>(b200host::launch_kernel(
-      kv_read_q4_kernel, dim3(blocks_for((long long)B * T * Hkv * (D / 8)), 2), dim3(256), 0,
-      reinterpret_cast<cudaStream_t>(stream), b200host::pdl_enabled() != 0, p));
+             {(uint32_t*)k_affine, (uint32_t*)v_affine}, (const int*)start, {0, 0}, {0, 0}, T, Hkv, pages,
+             page_rows, 0, {}, {}, {}};
+  return launch_kv(kv_read_q4_kernel<64>, kv_read_q4_kernel<128>, p, B, D, stream);
 }
 
 // x [rows, channels] bf16 with row stride ldx -> codes [rows, width / 8] words, affine [rows, width / 64] pairs.

@@ -47,41 +47,66 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 
 // Scale of a group from its least and largest value, as its bf16 bits: (most - least) / 15; NaN where the spread is no
 // number or beyond fp32 (a NaN or an infinity in the group), 0 where it is below the least normal number.
+// The quotient is x zh + x zl with zh + zl = 1 / 15 to 48 bits, one rounding after the fused sum (Brisebarre, Muller and
+// Raina, "Accelerating Correctly Rounded Floating-Point Division When the Divisor Is Known in Advance", 2004); for 15 it is
+// the correctly rounded one for every 24-bit significand.
 __device__ __forceinline__ uint32_t scale_bits(float least, float most) {
-  const float s = __bfloat162float(__float2bfloat16(__fdiv_rn(most - least, 15.f)));
+  constexpr float zh = 0x1.111112p-4f, zl = -0x1.dddddep-29f;
+  const float w = most - least;
+  const float s = __bfloat162float(__float2bfloat16(fmaf(w, zh, w * zl)));
   if (!(s <= 3.4e38f)) return 0x7fc0u;
   return s < 1.17549435e-38f ? 0u : __float_as_uint(s) >> 16;
 }
 
 // Code of x: (x - least) / s to the nearest whole number, ties to even, of the numbers themselves and not of their fp32
-// quotient.  The quotient by the reciprocal is off by 4e-6 at most, so it decides wherever it is further than that from a
-// border k + 1/2; near one the sign of x - least - (k + 1/2) s decides, which fp32 has exactly: the product has 13 bits
-// and goes into one fused rounding, and what the difference x - least lost (it loses something only where the two are 2^16
-// apart or more) is recovered and counts where the rest is zero.
-__device__ __forceinline__ uint32_t code_of(float x, float least, float s, float inv) {
+// quotient: near a border k + 1/2 the sign of x - least - (k + 1/2) s decides, which fp32 has exactly: the product has 13
+// bits and goes into one fused rounding, and what the difference x - least lost (it loses something only where the two are
+// 2^16 apart or more) is recovered and counts where the rest is zero.
+__device__ __forceinline__ float exact_code(float x, float least, float s, float inv) {
   const float d = x - least;
-  const float q = d * inv;
-  float n = rintf(q);
-  if (fabsf(q - n) > 0.499f) {
-    const float k = floorf(q);
-    const float r = fmaf(-(k + 0.5f), s, d);
-    const float back = d - x;
-    const float lost = (x - (d - back)) - (least + back);
-    const bool above = r > 0.f || (r == 0.f && (lost > 0.f || (lost == 0.f && (static_cast<int>(k) & 1))));
-    n = above ? k + 1.f : k;
-  }
-  return static_cast<uint32_t>(fminf(n, 15.f));
+  const float k = floorf(d * inv);
+  const float r = fmaf(-(k + 0.5f), s, d);
+  const float back = d - x;
+  const float lost = (x - (d - back)) - (least + back);
+  const bool above = r > 0.f || (r == 0.f && (lost > 0.f || (lost == 0.f && (static_cast<int>(k) & 1))));
+  return above ? k + 1.f : k;
 }
 
-// The word of eight channels of a group with the given affine pair.
+// The word of eight channels of a group with the given affine pair.  Where the channels and the least are multiples of G =
+// 2^-17 of the scale's power of two (all but groups of a very wide range are), the differences are exact, of 22 bits at most,
+// and a quotient with one Newton step on the approximate reciprocal, off by little more than 2^-24 of itself, rounds to the
+// right whole number: the borders (k + 1/2) s are multiples of G too, so what is not on a border is G away from it, 2^-22 of
+// it at least, and what is on one comes out as k + 1/2 itself.  Codes come out of the low bits of q + 1.5 2^23, two to a byte by
+// one multiply-add.
 __device__ __forceinline__ uint32_t pack(const float (&x)[8], uint32_t affine) {
+  using namespace b200;
   const float s = scale_of(affine), least = least_of(affine);
   if (!(s > 0.f)) return 0u;   // a constant group, or one without numbers
-  const float inv = __frcp_rn(s);
-  uint32_t word = 0;
+  const float inv = __fdividef(1.f, s);        // 2 ulp
+  constexpr float magic = 12582912.f;
+  // adding 1.5 2^23 G and taking it off again leaves multiples of G, and of what is larger no less (a bf16 above 2^7 G is one)
+  const float grid = __uint_as_float((__float_as_uint(s) & 0x7f800000u)) * 96.f;
+  const uint64_t inv2 = f2_pack(inv, inv), least2 = f2_pack(-least, -least), s2 = f2_pack(-s, -s);
+  const uint64_t magic2 = f2_pack(magic, magic), minus2 = f2_pack(-magic, -magic);
+  const uint64_t grid2 = f2_pack(grid, grid), ungrid2 = f2_pack(-grid, -grid);
+  float n[8];
+  bool coarse = (least + grid) - grid == least;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) word |= code_of(x[i], least, s, inv) << (4 * ((i >> 1) + 4 * (i & 1)));
-  return word;
+  for (int i = 0; i < 8; i += 2) {
+    const uint64_t x2 = f2_pack(x[i], x[i + 1]), d = f2_add(x2, least2), q = f2_mul(d, inv2);
+    f2_unpack(f2_add(f2_add(f2_fma(f2_fma(q, s2, d), inv2, q), magic2), minus2), n[i], n[i + 1]);
+    float u, v;
+    f2_unpack(f2_add(f2_add(x2, grid2), ungrid2), u, v);
+    coarse = coarse && u == x[i] && v == x[i + 1];
+  }
+  if (!coarse) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) n[i] = exact_code(x[i], least, s, inv);
+  }
+  // nibbles 0 .. 7 are channels 0 2 4 6 1 3 5 7; none is above 15: s is at least 1 - 2^-8 of a fifteenth of the spread
+  const uint32_t b0 = __float_as_uint(fmaf(n[2], 16.f, n[0]) + magic), b1 = __float_as_uint(fmaf(n[6], 16.f, n[4]) + magic);
+  const uint32_t b2 = __float_as_uint(fmaf(n[3], 16.f, n[1]) + magic), b3 = __float_as_uint(fmaf(n[7], 16.f, n[5]) + magic);
+  return __byte_perm(__byte_perm(b0, b1, 0x0040), __byte_perm(b2, b3, 0x0040), 0x5410);
 }
 
 __device__ __forceinline__ void unpack_bf16(const uint4& v, float (&f)[8]) {
@@ -93,15 +118,48 @@ __device__ __forceinline__ void unpack_bf16(const uint4& v, float (&f)[8]) {
   }
 }
 
-// Values of a word as eight bf16, rounded once.
-__device__ __forceinline__ uint4 values_bf16(uint32_t word, uint32_t affine) {
-  const float s = scale_of(affine), z = least_of(affine);
-  float n[8];
-  unpack(word, n);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) n[i] = fmaf(n[i], s, z);
-  return make_uint4(b200::pack_bf16x2(n[0], n[1]), b200::pack_bf16x2(n[2], n[3]), b200::pack_bf16x2(n[4], n[5]),
-                    b200::pack_bf16x2(n[6], n[7]));
+// Codes P of both halves of w as bf16 128 + n: one shift and one three-input operation (a & b) | c, whose constants are kept
+// in registers (opaque_masks), since an instruction has room for one.
+template <int P>
+__device__ __forceinline__ uint32_t coded(uint32_t w, uint32_t mask, uint32_t magic) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(P ? w >> (4 * P) : w), "r"(mask), "r"(magic));
+  return r;
 }
+__device__ __forceinline__ void opaque_masks(uint32_t& mask, uint32_t& magic) {
+  mask = 0x000f000fu;
+  magic = 0x43004300u;
+  asm volatile("" : "+r"(mask), "+r"(magic));
+}
+
+// Values of a word as eight bf16, rounded once (after fp32).
+__device__ __forceinline__ uint4 values_bf16(uint32_t word, uint32_t affine, uint32_t mask, uint32_t magic) {
+  const uint64_t s = b200::f2_pack(scale_of(affine), scale_of(affine)), z = b200::f2_pack(least_of(affine), least_of(affine));
+  const uint64_t minus = b200::f2_pack(-128.f, -128.f);
+  const uint32_t pair[4] = {coded<0>(word, mask, magic), coded<1>(word, mask, magic), coded<2>(word, mask, magic),
+                            coded<3>(word, mask, magic)};
+  uint32_t out[4];
+#pragma unroll
+  for (int p = 0; p < 4; ++p) {
+    const uint64_t n = b200::f2_add(b200::f2_pack(__uint_as_float(pair[p] << 16), __uint_as_float(pair[p] & 0xffff0000u)), minus);
+    float u, v;
+    b200::f2_unpack(b200::f2_fma(n, s, z), u, v);
+    out[p] = b200::pack_bf16x2(u, v);
+  }
+  return make_uint4(out[0], out[1], out[2], out[3]);
+}
+
+// n / d by a multiplication: n, d below 2^31 (Granlund and Montgomery, "Division by Invariant Integers using
+// Multiplication", 1994, figure 4.1).
+struct Divisor {
+  uint32_t d, mul, shift;
+  Divisor() = default;
+  __host__ explicit Divisor(uint32_t by) : d(by) {
+    shift = 0;
+    while (shift < 32 && (1ull << shift) < by) ++shift;
+    mul = static_cast<uint32_t>(((1ull << 32) * ((1ull << shift) - by)) / by + 1);
+  }
+  __device__ __forceinline__ uint32_t of(uint32_t n) const { return (__umulhi(mul, n) + n) >> shift; }
+};
 
 }  // namespace q4
