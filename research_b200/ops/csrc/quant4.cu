@@ -21,12 +21,15 @@ struct KvParams {
   Divisor per_block, per_token, per_page;
 };
 
-constexpr int kItems = 4;             // words of a thread, their loads all under way at once
 constexpr uint32_t kThreads = 256;
+// A lane has eight channels of every group of its row (words 2 g and 2 g + 1 of a row of 128), so that placing it, which costs
+// as much as a word's codes, is done once for both.  Lanes of a thread, their loads all under way at once:
+template <int D>
+constexpr int items() { return D == 128 ? 2 : 4; }
 
-// A thread's words among those of a sequence's new rows, counted over (token, head, word): this one, and 256 further on.
+// A thread's items among those of a sequence's new rows, counted over (token, head, g): this one, and 256 further on.
 struct Walk {
-  uint32_t token, e;                  // e: word of the token's row over all heads
+  uint32_t token, e;                  // e: item of the token's row over all heads
   __device__ __forceinline__ Walk(const KvParams& p, uint32_t j) : token(p.per_token.of(j)), e(j - token * p.per_token.d) {}
   __device__ __forceinline__ void next(const KvParams& p, uint32_t tokens, uint32_t rest) {
     token += tokens;
@@ -42,95 +45,112 @@ struct Walk {
 // row of the cache (both are below 2^31).
 __device__ __forceinline__ uint32_t row_of(int first, const Walk& at) { return static_cast<uint32_t>(first) + at.token; }
 // Pool row of a token's head.
-template <int D>
 __device__ __forceinline__ uint64_t pool_row(const KvParams& p, uint64_t seq_row, uint32_t r, const Walk& at) {
-  constexpr uint32_t WORDS = D / 8;
   const uint32_t pg = p.per_page.of(r), in = r - pg * p.per_page.d;
-  return seq_row + in + static_cast<uint64_t>(pg * p.Hkv + at.e / WORDS) * p.per_page.d;
-}
-// word of a pool row for word e of the token
-template <int D>
-__device__ __forceinline__ uint32_t word_at(uint32_t e) {
-  const uint32_t c = e % (D / 8);
-  return D == 128 ? 2 * (c & 7) + (c >> 3) : c;
+  return seq_row + in + static_cast<uint64_t>(pg * p.Hkv + at.e / 8) * p.per_page.d;
 }
 
-// Quantise as it is written: a lane per word, eight lanes share a group and find its least and largest value in bf16 (which
-// they are).  Bound by the reads (2 bytes a channel) as long as the arithmetic stays near 15 instructions a channel: eight
-// prompts of 4096 rows of 8 heads of 128, 172 MB, in KVWRITE us.
+// Quantise as it is written: eight lanes have a row's head and find the least and largest value of its groups in bf16 (which
+// they are).  Bound by the arithmetic, 20 instructions a channel: eight prompts of 4096 rows of 8 heads of 128 (172 MB read
+// and written, 26 us at the copy bandwidth) take 47 us, and 26 us to read back.
 template <int D>
-__global__ void __launch_bounds__(256) kv_write_q4_kernel(const __grid_constant__ KvParams p) {
+__global__ void __launch_bounds__(kThreads) kv_write_q4_kernel(const __grid_constant__ KvParams p) {
+  constexpr int ITEMS = items<D>(), GROUPS = D / 64;
   const int which = blockIdx.y, b = static_cast<int>(p.per_block.of(blockIdx.x)), block = blockIdx.x - b * p.blocks;
   b200::pdl_launch_dependents();
   b200::pdl_wait();
   const int first = p.start ? p.start[b] : 0;
-  const uint32_t total = static_cast<uint32_t>(p.T) * p.per_token.d, j0 = block * (kThreads * kItems) + threadIdx.x;
+  const uint32_t total = static_cast<uint32_t>(p.T) * p.per_token.d, j0 = block * (kThreads * ITEMS) + threadIdx.x;
   const uint32_t tokens = p.per_token.of(kThreads), rest = kThreads - tokens * p.per_token.d;
   const __nv_bfloat16* src = p.src[which] + b * p.batch[which];
-  uint4 v[kItems];
+  uint4 v[ITEMS][GROUPS];
   {
     Walk at(p, j0);
 #pragma unroll
-    for (int k = 0; k < kItems; ++k, at.next(p, tokens, rest))   // beyond the rows: the last one's word, whose group is whole too
-      v[k] = *reinterpret_cast<const uint4*>(src + static_cast<long long>(min(at.token, p.T - 1u)) * p.row[which] + at.e * 8);
+    for (int k = 0; k < ITEMS; ++k, at.next(p, tokens, rest)) {  // beyond the rows: the last one's, whose groups are whole too
+      const __nv_bfloat16* row = src + static_cast<long long>(min(at.token, p.T - 1u)) * p.row[which] + (at.e / 8) * D +
+                                 (at.e & 7) * 8;
+#pragma unroll
+      for (int h = 0; h < GROUPS; ++h) v[k][h] = *reinterpret_cast<const uint4*>(row + 64 * h);
+    }
   }
   const uint64_t seq_row = static_cast<uint64_t>(b) * p.pages * p.Hkv * p.page_rows;
   const uint32_t capacity = static_cast<uint32_t>(p.pages) * p.page_rows;
   Walk at(p, j0);
 #pragma unroll
-  for (int k = 0; k < kItems; ++k, at.next(p, tokens, rest)) {
+  for (int k = 0; k < ITEMS; ++k, at.next(p, tokens, rest)) {
     const uint32_t j = j0 + k * kThreads;
     if (j - (threadIdx.x & 31) >= total) break;           // the whole warp is beyond
-    __nv_bfloat162 w[4];
-    memcpy(w, &v[k], 16);
-    const __nv_bfloat162 lo = __hmin2_nan(__hmin2_nan(w[0], w[1]), __hmin2_nan(w[2], w[3]));
-    const __nv_bfloat162 hi = __hmax2_nan(__hmax2_nan(w[0], w[1]), __hmax2_nan(w[2], w[3]));
-    // (least, -largest), so that one minimum serves both
-    __nv_bfloat162 m = __halves2bfloat162(__hmin_nan(lo.x, lo.y), __hneg(__hmax_nan(hi.x, hi.y)));
+    uint32_t word[GROUPS], affine[GROUPS];
 #pragma unroll
-    for (int off = 4; off > 0; off >>= 1) m = __hmin2_nan(m, __shfl_xor_sync(0xffffffffu, m, off));
-    const float least = __low2float(m), most = -__high2float(m);
-    const uint32_t affine = (__float_as_uint(least) & 0xffff0000u) | scale_bits(least, most);
-    float x[8];
-    unpack_bf16(v[k], x);
-    const uint32_t word = pack(x, affine);
-    const uint32_t r = row_of(first, at);
+    for (int h = 0; h < GROUPS; ++h) {
+      __nv_bfloat162 w[4];
+      memcpy(w, &v[k][h], 16);
+      const __nv_bfloat162 lo = __hmin2_nan(__hmin2_nan(w[0], w[1]), __hmin2_nan(w[2], w[3]));
+      const __nv_bfloat162 hi = __hmax2_nan(__hmax2_nan(w[0], w[1]), __hmax2_nan(w[2], w[3]));
+      // (least, -largest), so that one minimum serves both
+      __nv_bfloat162 m = __halves2bfloat162(__hmin_nan(lo.x, lo.y), __hneg(__hmax_nan(hi.x, hi.y)));
+#pragma unroll
+      for (int off = 4; off > 0; off >>= 1) m = __hmin2_nan(m, __shfl_xor_sync(0xffffffffu, m, off));
+      const float least = __low2float(m), most = -__high2float(m);
+      affine[h] = (__float_as_uint(least) & 0xffff0000u) | scale_bits(least, most);
+      float x[8];
+      unpack_bf16(v[k][h], x);
+      word[h] = pack(x, affine[h]);
+    }
+    const uint32_t r = row_of(first, at), g = at.e & 7;
     if (j >= total || r >= capacity) continue;
-    const uint64_t row = pool_row<D>(p, seq_row, r, at);
-    p.codes[which][row * (D / 8) + word_at<D>(at.e)] = word;
-    if ((at.e & 7) == 0) p.affine[which][row * (D / 64) + at.e % (D / 8) / 8] = affine;
+    const uint64_t row = pool_row(p, seq_row, r, at);
+    if constexpr (GROUPS == 2) {
+      reinterpret_cast<uint2*>(p.codes[which])[row * 8 + g] = make_uint2(word[0], word[1]);
+      if (g == 0) reinterpret_cast<uint2*>(p.affine[which])[row] = make_uint2(affine[0], affine[1]);
+    } else {
+      p.codes[which][row * 8 + g] = word[0];
+      if (g == 0) p.affine[which][row] = affine[0];
+    }
   }
 }
 
-// Read back: a lane per word, 16 bytes written.
+// Read back.
 template <int D>
-__global__ void __launch_bounds__(256) kv_read_q4_kernel(const __grid_constant__ KvParams p) {
+__global__ void __launch_bounds__(kThreads) kv_read_q4_kernel(const __grid_constant__ KvParams p) {
+  constexpr int ITEMS = items<D>(), GROUPS = D / 64;
   const int which = blockIdx.y, b = static_cast<int>(p.per_block.of(blockIdx.x)), block = blockIdx.x - b * p.blocks;
   b200::pdl_launch_dependents();
   b200::pdl_wait();
   const int first = p.start ? p.start[b] : 0;
-  const uint32_t total = static_cast<uint32_t>(p.T) * p.per_token.d, j0 = block * (kThreads * kItems) + threadIdx.x;
+  const uint32_t total = static_cast<uint32_t>(p.T) * p.per_token.d, j0 = block * (kThreads * ITEMS) + threadIdx.x;
   const uint32_t tokens = p.per_token.of(kThreads), rest = kThreads - tokens * p.per_token.d;
   const uint64_t seq_row = static_cast<uint64_t>(b) * p.pages * p.Hkv * p.page_rows;
   const uint32_t capacity = static_cast<uint32_t>(p.pages) * p.page_rows;
-  uint32_t word[kItems], affine[kItems];
+  uint32_t word[ITEMS][GROUPS], affine[ITEMS][GROUPS];
   Walk at(p, j0);
 #pragma unroll
-  for (int k = 0; k < kItems; ++k, at.next(p, tokens, rest)) {
-    word[k] = affine[k] = 0;                              // a row that the cache does not have reads as zeros
-    const uint32_t r = row_of(first, at);
-    if (j0 + k * kThreads < total && r < capacity) {
-      const uint64_t row = pool_row<D>(p, seq_row, r, at);
-      word[k] = p.codes[which][row * (D / 8) + word_at<D>(at.e)];
-      affine[k] = p.affine[which][row * (D / 64) + at.e % (D / 8) / 8];
+  for (int k = 0; k < ITEMS; ++k, at.next(p, tokens, rest)) {
+    const uint32_t r = row_of(first, at), g = at.e & 7;
+    const bool there = j0 + k * kThreads < total && r < capacity;   // a row that the cache does not have reads as zeros
+    const uint64_t row = there ? pool_row(p, seq_row, r, at) : 0;
+    if constexpr (GROUPS == 2) {
+      const uint2 w = there ? reinterpret_cast<const uint2*>(p.codes[which])[row * 8 + g] : make_uint2(0, 0);
+      const uint2 a = there ? reinterpret_cast<const uint2*>(p.affine[which])[row] : make_uint2(0, 0);
+      word[k][0] = w.x, word[k][1] = w.y, affine[k][0] = a.x, affine[k][1] = a.y;
+    } else {
+      word[k][0] = there ? p.codes[which][row * 8 + g] : 0u;
+      affine[k][0] = there ? p.affine[which][row] : 0u;
     }
   }
   uint32_t mask, magic;
   opaque_masks(mask, magic);
-  uint4* to = reinterpret_cast<uint4*>(p.dst[which]) + static_cast<long long>(b) * total;
+  // an item's first chunk of eight channels among the sequence's: the item with the groups' chunks counted in
+  uint4* to = reinterpret_cast<uint4*>(p.dst[which]) + static_cast<long long>(b) * total * GROUPS;
 #pragma unroll
-  for (int k = 0; k < kItems; ++k)
-    if (j0 + k * kThreads < total) to[j0 + k * kThreads] = values_bf16(word[k], affine[k], mask, magic);
+  for (int k = 0; k < ITEMS; ++k) {
+    const uint32_t j = j0 + k * kThreads;
+    if (j >= total) break;
+#pragma unroll
+    for (int h = 0; h < GROUPS; ++h)
+      to[static_cast<uint64_t>(j / 8) * (8 * GROUPS) + 8 * h + (j & 7)] = values_bf16(word[k][h], affine[k][h], mask, magic);
+  }
 }
 
 // Whole matrices (weights, once): eight lanes per group, any number of channels and any row stride.
@@ -204,15 +224,15 @@ bool kv_shape_ok(int B, int T, int Hkv, int D, int pages, int page_rows) {
   return B > 0 && T > 0 && Hkv > 0 && (D == 64 || D == 128) && pages > 0 && page_rows > 0 &&
          static_cast<long long>(pages) * page_rows <= 0x7fffffffll &&
          static_cast<long long>(pages) * Hkv <= 0x7fffffffll && static_cast<long long>(T) * Hkv * (D / 8) <= 0x7ffff000ll &&
-         static_cast<long long>(B) * (static_cast<long long>(T) * Hkv * (D / 8) / (kThreads * kItems) + 1) <= 0x7fffffffll;
+         static_cast<long long>(B) * (static_cast<long long>(T) * Hkv * 8 / (kThreads * 2) + 1) <= 0x7fffffffll;
 }
 
 template <typename Kern>
 int launch_kv(Kern* kern64, Kern* kern128, KvParams p, int B, int D, void* stream) {
-  const uint32_t words = static_cast<uint32_t>(p.Hkv) * (D / 8);
-  p.blocks = static_cast<int>((static_cast<uint32_t>(p.T) * words + kThreads * kItems - 1) / (kThreads * kItems));
+  const uint32_t per = static_cast<uint32_t>(p.Hkv) * 8, block = kThreads * (D == 64 ? items<64>() : items<128>());
+  p.blocks = static_cast<int>((static_cast<uint32_t>(p.T) * per + block - 1) / block);
   p.per_block = Divisor(p.blocks);
-  p.per_token = Divisor(words);
+  p.per_token = Divisor(per);
   p.per_page = Divisor(p.page_rows);
   return static_cast<int>(b200host::launch_kernel(D == 64 ? kern64 : kern128, dim3(B * p.blocks, 2), dim3(kThreads), 0,
                                                   reinterpret_cast<cudaStream_t>(stream), b200host::pdl_enabled() != 0, p));
