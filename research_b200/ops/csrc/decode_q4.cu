@@ -6,12 +6,20 @@
 // be a stream for the memory becomes work for the SM: at the copy bandwidth 46 codes a clock and SM, too many for an FMA per
 // code and head.  Both products therefore go through the tensor cores as m16n8k16 with the cache as the 16-row operand and
 // up to eight query heads as the columns (a tcgen05 product would want the expanded rows in shared or tensor memory first,
-// and its 128 x 16 tile has no more use for eight columns): a code c becomes the bf16 128 + c by one shift and one
-// and-or per two codes, exact, and scales and least values are applied to the sums in fp32:
-//   q . k_r = sum_groups s_r (sum q (128 + n) - 128 sum q) + z_r sum q
-//   o       = sum_r (p_r s_r) (128 + n_r) - 136 sum_r (p_r s_r) + sum_r p_r (z_r + 8 s_r)      (centred: n - 8)
+// and its 128 x 16 tile has no more use for eight columns).  The bits 0 .. 255 are, as bf16, the numbers i 2^-133 (subnormals
+// and the first binade are one straight line), so that a code needs no more than to be masked out: n at the low end of a
+// half word, 16 n four bits further up, one shift for the word's other four.  The other operands make up for the size: queries
+// are brought to 2^126 by a power of two of their head's own (and divided by 16 where the code is not), weights times scales
+// to 2^100 by one that follows the largest scale.  Scales and least values are applied to the sums in fp32:
+//   q . k_r = sum_groups s_r (sum q n) + z_r sum q
+//   o       = sum_r (p_r s_r) n_r + sum_r p_r z_r
 // p s enters the second product as two bf16 parts (up to four heads: in columns 4 .. 7 of the same product, else in a
 // second one), which holds it to 2^-14; a single bf16 would cost as much as the rounding of the result does.
+//
+// Measured (inputs larger than L2 or flushed from it): 64 sequences of 512 .. 4096 rows, 32 heads over 8 of 128, 46.6 us; of
+// 16384 rows 136.5 us, 77 % of the copy bandwidth; one sequence of 131072 rows, 23 us; of 300, 7.3 us, which are two launches
+// and one tile's latency.  With codes as 128 + n (a second operation each, and the 128 taken off again) and a maximum followed
+// tile by tile the first took 53 us.
 #include <math.h>
 #include <math_constants.h>
 
@@ -31,8 +39,8 @@ struct AttnParams {
   __nv_bfloat16* out;                 // [B, Hq, D]
   float *part_o, *part_ml;            // [slots, G, D], [slots, G, 2]: (m in log2 units, l)
   int B, Hq, Hkv, pages, page_rows, warps;
-  float scale_log2;                   // above zero: a negative scale changes the queries' sign
-  uint32_t q_sign;                    // of two bf16
+  float scale_log2;                   // above zero: a negative scale changes the queries' sign, one of zero leaves zeros of them
+  uint32_t q_keep, q_flip;            // bits of two bf16
 };
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
@@ -58,7 +66,19 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t v) {
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
   return r;
 }
-constexpr uint32_t kOnes = 0x3f803f80u;
+// the first product of a chain
+__device__ __forceinline__ void mma_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                          uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+// 2^e, e clamped to what fp32 has as normal numbers
+__device__ __forceinline__ float pow2(int e) { return __uint_as_float(static_cast<uint32_t>(min(max(e, -126), 127) + 127) << 23); }
+
+// codes 0 and 1 (of four) of each half of a word as bf16: n 2^-133 and 16 n 2^-133
+__device__ __forceinline__ uint32_t low_codes(uint32_t w) { return w & 0x000f000fu; }
+__device__ __forceinline__ uint32_t high_codes(uint32_t w) { return w & 0x00f000f0u; }
 
 // Rows of sequence b that count: [first, end), in tiles of TR rows from tile_lo to tile_hi (none: tile_lo = tile_hi).
 template <int TR>
@@ -228,35 +248,63 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS) decode_q4_kernel(const __g
     cp_async_commit();
   }
 
-  uint32_t mask, magic;
-  opaque_masks(mask, magic);
   const int pi = (g & 1) ? 7 - (g >> 1) : g >> 1;
   const float low = (!WIDE && t >= 2) ? 1.f : 0.f;
   uint32_t qf[KW][4];
-  float qsum[GROUPS][2];
+  float qsum[GROUPS][2], scale[2], before[2];  // sums of q, and log2(e) times the scale, in the units of the first product
+  bool huge = false;                           // queries of 2^113 and more: the scale is in two factors
   float o[GROUPS * 4][4], zacc[GROUPS][2], m[2], l[2];
+  int v_exp = 0;                               // of the largest scale of V so far, about
+  float v_up = 1.f, v_limit = -1.f;            // 2^(100 - v_exp), and the scale from which v_exp has to go up
   bool fresh = true;
   for (int i = 0; i < count; ++i) {
     if (fresh) {
       // queries: column g of the first product is head g (WIDE) or g % 4, whose second copy gives the low parts of p s
       fresh = false;
       const int hq = WIDE ? g : (g & 3);
+      uint32_t most = 0;                       // exponent bits of the head's largest value
 #pragma unroll
       for (int j = 0; j < KW; ++j) {
         const int c = D == 128 ? 64 * (j & 1) + 16 * t + 8 * (j >> 1) : 16 * t + 8 * j;
         uint4 v = make_uint4(0, 0, 0, 0);
         if (hq < G)
           v = *reinterpret_cast<const uint4*>(p.q + at.b * p.q_batch + static_cast<long long>(at.h * G + hq) * D + c);
-        qf[j][0] = v.x ^ p.q_sign, qf[j][1] = v.y ^ p.q_sign, qf[j][2] = v.z ^ p.q_sign, qf[j][3] = v.w ^ p.q_sign;
-      }
+        qf[j][0] = v.x, qf[j][1] = v.y, qf[j][2] = v.z, qf[j][3] = v.w;
 #pragma unroll
-      for (int gr = 0; gr < GROUPS; ++gr) {
+        for (int k = 0; k < 4; ++k) most = max(most, max(qf[j][k] & 0x7f80u, (qf[j][k] >> 16) & 0x7f80u));
+      }
+      most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
+      most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
+      // q' = q 2^(126 - e): a sum of q' n 2^-133 stands for 2^(7 + e) times itself, of which what is above 2^119 goes to the
+      // scores first.  A head with an infinity or a NaN has none; else the factor stays a number above zero, so that a masked
+      // row's -inf does.
+      const int e = static_cast<int>(most >> 7) - 127;
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const int ec = __shfl_sync(0xffffffffu, e, 8 * t + 4 * c) + 7;
+        const float f = fminf(fmaxf(p.scale_log2 * pow2(min(ec, 119)), 1.17549435e-38f), 3.402823466e38f);
+        scale[c] = ec == 135 ? CUDART_NAN_F : f;
+        before[c] = pow2(max(ec - 119, 0));
+      }
+      huge = __any_sync(0xffffffffu, before[0] + before[1] > 2.f);
+      // 2^(126 - e) may be more than one factor has room for
+      const float up = pow2((126 - e) / 2), up2 = pow2(126 - e - (126 - e) / 2);
+#pragma unroll
+      for (int j = 0; j < KW; ++j)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float f = (k & 1) ? up2 * 0.0625f : up2;
+          const uint32_t v = (qf[j][k] & p.q_keep) ^ p.q_flip;
+          qf[j][k] = b200::pack_bf16x2(__uint_as_float(v << 16) * up * f, __uint_as_float(v & 0xffff0000u) * up * f);
+        }
+#pragma unroll
+      for (int gr = 0; gr < GROUPS; ++gr) {    // sums of q': the product with a row of ones
         float c[4] = {};
 #pragma unroll
         for (int j = 0; j < KW; ++j)
           if (GROUPS == 1 || (j & 1) == gr) {
-            mma(c, kOnes, kOnes, kOnes, kOnes, qf[j][0], qf[j][1]);
-            mma(c, kOnes, kOnes, kOnes, kOnes, qf[j][2], qf[j][3]);
+            mma(c, 0x00010001u, 0x00010001u, 0x00100010u, 0x00100010u, qf[j][0], qf[j][1]);
+            mma(c, 0x00010001u, 0x00010001u, 0x00100010u, 0x00100010u, qf[j][2], qf[j][3]);
           }
         qsum[gr][0] = c[0], qsum[gr][1] = c[1];
         zacc[gr][0] = zacc[gr][1] = 0.f;
@@ -301,24 +349,23 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS) decode_q4_kernel(const __g
       }
       float acc[GROUPS][4];
 #pragma unroll
-      for (int gr = 0; gr < GROUPS; ++gr)
-#pragma unroll
-        for (int c = 0; c < 4; ++c) acc[gr][c] = 0.f;
-#pragma unroll
       for (int j = 0; j < KW; ++j) {
-        float(&a)[4] = acc[GROUPS == 1 ? 0 : (j & 1)];
-        mma(a, coded<0>(ka[j], mask, magic), coded<0>(kb[j], mask, magic), coded<1>(ka[j], mask, magic), coded<1>(kb[j], mask, magic), qf[j][0], qf[j][1]);
-        mma(a, coded<2>(ka[j], mask, magic), coded<2>(kb[j], mask, magic), coded<3>(ka[j], mask, magic), coded<3>(kb[j], mask, magic), qf[j][2], qf[j][3]);
+        const int gr = GROUPS == 1 ? 0 : (j & 1);
+        const uint32_t wa = ka[j] >> 8, wb = kb[j] >> 8;
+        if (j < GROUPS)
+          mma_first(acc[gr], low_codes(ka[j]), low_codes(kb[j]), high_codes(ka[j]), high_codes(kb[j]), qf[j][0], qf[j][1]);
+        else
+          mma(acc[gr], low_codes(ka[j]), low_codes(kb[j]), high_codes(ka[j]), high_codes(kb[j]), qf[j][0], qf[j][1]);
+        mma(acc[gr], low_codes(wa), low_codes(wb), high_codes(wa), high_codes(wb), qf[j][2], qf[j][3]);
       }
-#pragma unroll
-      for (int c = 0; c < 4; ++c) sc[mt][c] = 0.f;
 #pragma unroll
       for (int gr = 0; gr < GROUPS; ++gr) {
         const float sa = scale_of(aa[gr]), sb = scale_of(ab[gr]);
-        const float za = fmaf(-128.f, sa, least_of(aa[gr])), zb = fmaf(-128.f, sb, least_of(ab[gr]));
+        const float za = least_of(aa[gr]), zb = least_of(ab[gr]);
 #pragma unroll
         for (int c = 0; c < 4; ++c)
-          sc[mt][c] = fmaf(c < 2 ? sa : sb, acc[gr][c], fmaf(c < 2 ? za : zb, qsum[gr][c & 1], sc[mt][c]));
+          sc[mt][c] = fmaf(c < 2 ? sa : sb, acc[gr][c],
+                           gr ? fmaf(c < 2 ? za : zb, qsum[gr][c & 1], sc[mt][c]) : (c < 2 ? za : zb) * qsum[gr][c & 1]);
       }
       if (edge) {
         const bool seen_a = r0 + ja >= first && r0 + ja < end, seen_b = r0 + jb >= first && r0 + jb < end;
@@ -328,31 +375,71 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS) decode_q4_kernel(const __g
       }
     }
 
-    float alpha[2];
+    if (huge) {
+#pragma unroll
+      for (int mt = 0; mt < STEPS; ++mt)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) sc[mt][c] *= before[c & 1];
+    }
+    // Exponentials are taken relative to a reference that follows the maximum only where a score is 2^8 above it (or there
+    // is none yet): what they add up to stays far inside fp32, and nothing has to be rescaled for most tiles.
+    float top[2];
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      float mx = m[e];
+      top[e] = fmaxf(sc[0][e], sc[0][e + 2]);
 #pragma unroll
-      for (int mt = 0; mt < STEPS; ++mt) mx = fmaxf(mx, fmaxf(sc[mt][e], sc[mt][e + 2]));
+      for (int mt = 1; mt < STEPS; ++mt) top[e] = fmaxf(top[e], fmaxf(sc[mt][e], sc[mt][e + 2]));
+    }
+    // the largest scale of the tile's V rows, two rows a lane (a scale that is no number counts for nothing here)
+    float v_top = 0.f;
 #pragma unroll
-      for (int off = 4; off < 32; off <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
-      const float use = mx == -CUDART_INF_F ? 0.f : mx * p.scale_log2;
-      alpha[e] = b200::ex2_approx(fmaf(m[e], p.scale_log2, -use));
-      m[e] = mx;
-      float sum = 0.f;
+    for (int k = 0; k < TR / 32; ++k) {
+      const int j = lane + 32 * k;
+#pragma unroll
+      for (int gr = 0; gr < GROUPS; ++gr) {
+        const float s = scale_of(*reinterpret_cast<const uint32_t*>(slot + OFF_VA + j * PAIR_BYTES + gr * 4));
+        if (!edge || (r0 + j >= first && r0 + j < end)) v_top = fmaxf(v_top, fabsf(s));
+      }
+    }
+    if (__any_sync(0xffffffffu, fmaf(top[0], scale[0], -m[0]) > 8.f || fmaf(top[1], scale[1], -m[1]) > 8.f ||
+                                    v_top > v_limit)) {
+      v_top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(v_top)));
+      float down = 1.f;
+      if (v_top > v_limit) {                   // weights go up to 2^8, scales to 2^9 above v_exp: far from 2^127 together
+        const int now = max(static_cast<int>(__float_as_uint(v_top) >> 23) - 127, -27);
+        down = v_limit < 0.f ? 1.f : pow2(v_exp - now);
+        v_exp = now;
+        v_up = pow2(100 - now);
+        v_limit = pow2(now + 9);
+      }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float mx = top[e];
+#pragma unroll
+        for (int off = 4; off < 32; off <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+        mx = fmaxf(m[e], mx * scale[e]);
+        const float alpha = mx == -CUDART_INF_F ? 1.f : b200::ex2_approx(m[e] - mx);
+        m[e] = mx;
+        l[e] *= alpha;
+#pragma unroll
+        for (int gr = 0; gr < GROUPS; ++gr) zacc[gr][e] *= alpha;
+#pragma unroll
+        for (int v = 0; v < GROUPS * 4; ++v) o[v][e] *= alpha * down, o[v][e + 2] *= alpha * down;
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const float use = m[e] == -CUDART_INF_F ? 0.f : m[e];     // no number yet: nothing but zeros (or NaN) comes out
 #pragma unroll
       for (int mt = 0; mt < STEPS; ++mt) {
-        sc[mt][e] = b200::ex2_approx(fmaf(sc[mt][e], p.scale_log2, -use));
-        sc[mt][e + 2] = b200::ex2_approx(fmaf(sc[mt][e + 2], p.scale_log2, -use));
-        sum += sc[mt][e] + sc[mt][e + 2];
+        sc[mt][e] = b200::ex2_approx(fmaf(sc[mt][e], scale[e], -use));
+        sc[mt][e + 2] = b200::ex2_approx(fmaf(sc[mt][e + 2], scale[e], -use));
+        l[e] += sc[mt][e] + sc[mt][e + 2];
       }
-      l[e] = fmaf(l[e], alpha[e], sum);
     }
 
     // p s in two parts, as the column operand of the second product
     uint32_t bh_[GROUPS][STEPS][2], bl_[WIDE ? GROUPS : 1][STEPS][2];
-#pragma unroll
-    for (int gr = 0; gr < GROUPS; ++gr) zacc[gr][0] *= alpha[0], zacc[gr][1] *= alpha[1];
 #pragma unroll
     for (int mt = 0; mt < STEPS; ++mt) {
       const int ja = 16 * mt + pi, jb = ja + 8;
@@ -375,8 +462,8 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS) decode_q4_kernel(const __g
       }
 #pragma unroll
       for (int gr = 0; gr < GROUPS; ++gr) {
-        const float sa = scale_of(aa[gr]), sb = scale_of(ab[gr]);
-        const float za = fmaf(8.f, sa, least_of(aa[gr])), zb = fmaf(8.f, sb, least_of(ab[gr]));
+        const float sa = scale_of(aa[gr]) * v_up, sb = scale_of(ab[gr]) * v_up;
+        const float za = least_of(aa[gr]), zb = least_of(ab[gr]);
         zacc[gr][0] = fmaf(sc[mt][0], za, fmaf(sc[mt][2], zb, zacc[gr][0]));
         zacc[gr][1] = fmaf(sc[mt][1], za, fmaf(sc[mt][3], zb, zacc[gr][1]));
         const float u[4] = {sc[mt][0] * sa, sc[mt][1] * sa, sc[mt][2] * sb, sc[mt][3] * sb};
@@ -396,21 +483,6 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS) decode_q4_kernel(const __g
           bh_[gr][mt][1] = transpose8(__byte_perm(__float_as_uint(rest[2]), __float_as_uint(rest[3]), 0x7632));
         }
       }
-    }
-    // a tile's sums start at -136 sum p s and are added to the running ones in fp32
-    float acc[GROUPS * 4][4];
-#pragma unroll
-    for (int gr = 0; gr < GROUPS; ++gr) {
-      float c[4] = {};
-#pragma unroll
-      for (int mt = 0; mt < STEPS; ++mt) {
-        mma(c, kOnes, kOnes, kOnes, kOnes, bh_[gr][mt][0], bh_[gr][mt][1]);
-        if constexpr (WIDE) mma(c, kOnes, kOnes, kOnes, kOnes, bl_[gr][mt][0], bl_[gr][mt][1]);
-      }
-#pragma unroll
-      for (int v = 0; v < 4; ++v)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) acc[gr * 4 + v][e] = -136.f * c[e & 1];
     }
 #pragma unroll
     for (int mt = 0; mt < STEPS; ++mt) {
@@ -434,22 +506,19 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS) decode_q4_kernel(const __g
           mma(c, x0, x1, x2, x3, bh_[gr][mt][0], bh_[gr][mt][1]);
           if constexpr (WIDE) mma(c, x0, x1, x2, x3, bl_[gr][mt][0], bl_[gr][mt][1]);
         };
-        step(acc[gr * 4 + 0], coded<0>(a0, mask, magic), coded<0>(a1, mask, magic), coded<0>(a2, mask, magic), coded<0>(a3, mask, magic));
-        step(acc[gr * 4 + 1], coded<1>(a0, mask, magic), coded<1>(a1, mask, magic), coded<1>(a2, mask, magic), coded<1>(a3, mask, magic));
-        step(acc[gr * 4 + 2], coded<2>(a0, mask, magic), coded<2>(a1, mask, magic), coded<2>(a2, mask, magic), coded<2>(a3, mask, magic));
-        step(acc[gr * 4 + 3], coded<3>(a0, mask, magic), coded<3>(a1, mask, magic), coded<3>(a2, mask, magic), coded<3>(a3, mask, magic));
+        step(o[gr * 4 + 0], low_codes(a0), low_codes(a1), low_codes(a2), low_codes(a3));
+        step(o[gr * 4 + 1], high_codes(a0), high_codes(a1), high_codes(a2), high_codes(a3));
+        step(o[gr * 4 + 2], low_codes(a0 >> 8), low_codes(a1 >> 8), low_codes(a2 >> 8), low_codes(a3 >> 8));
+        step(o[gr * 4 + 3], high_codes(a0 >> 8), high_codes(a1 >> 8), high_codes(a2 >> 8), high_codes(a3 >> 8));
       }
     }
-#pragma unroll
-    for (int v = 0; v < GROUPS * 4; ++v)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) o[v][e] = fmaf(o[v][e], alpha[e & 1], acc[v][e]);
-
     const int b = at.b, h = at.h;
     fresh = i + 1 == count || at.tile + 1 == at.tile_hi;
     at.next(p);
     if (!fresh) continue;
     // the run leaves the pair: its state goes to the pair's slot
+    const float v_back = pow2(v_exp);          // and 2^33, or 2^29 where codes were 16 n
+    v_limit = -1.f;
     const long long place = static_cast<long long>(run) + static_cast<long long>(b) * p.Hkv + h;
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
@@ -461,12 +530,13 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS) decode_q4_kernel(const __g
       }
       const int hq = WIDE ? 2 * t + e : (2 * t + e) & 3;
       if (g == 0 && low == 0.f && hq < G)
-        *reinterpret_cast<float2*>(p.part_ml + (place * G + hq) * 2) = make_float2(m[e] * p.scale_log2, l[e]);
+        *reinterpret_cast<float2*>(p.part_ml + (place * G + hq) * 2) = make_float2(m[e], l[e]);
 #pragma unroll
       for (int gr = 0; gr < GROUPS; ++gr)
 #pragma unroll
         for (int v = 0; v < 4; ++v) {
-          float x = o[gr * 4 + v][e], y = o[gr * 4 + v][e + 2];
+          const float back = (v & 1) ? 536870912.f : 8589934592.f;
+          float x = o[gr * 4 + v][e] * back * v_back, y = o[gr * 4 + v][e + 2] * back * v_back;
           if constexpr (!WIDE) {      // the low parts are two lanes further
             x += __shfl_xor_sync(0xffffffffu, x, 2);
             y += __shfl_xor_sync(0xffffffffu, y, 2);
@@ -485,9 +555,10 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS) decode_q4_kernel(const __g
 constexpr int kMergeThreads = 256;
 template <int D, int TR>
 __global__ void __launch_bounds__(kMergeThreads) decode_q4_merge_kernel(const __grid_constant__ AttnParams p) {
-  constexpr int PARTS = kMergeThreads / D, WARPS = kMergeThreads / 32;
+  constexpr int PARTS = kMergeThreads / (D / 4), WARPS = kMergeThreads / 32;
   __shared__ long long s_sum[2][WARPS];
-  __shared__ float s_max[WARPS], s_w[kMergeThreads], s_l[WARPS], s_o[PARTS][D];
+  __shared__ float s_max[WARPS], s_w[kMergeThreads], s_l[WARPS];
+  __shared__ __align__(16) float s_o[PARTS][D];
   const int b = blockIdx.x / p.Hq, hq = blockIdx.x - b * p.Hq, G = p.Hq / p.Hkv, h = hq / G;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   b200::pdl_launch_dependents();
@@ -512,10 +583,10 @@ __global__ void __launch_bounds__(kMergeThreads) decode_q4_merge_kernel(const __
 #pragma unroll
     for (int w = 0; w < WARPS; ++w) sum[k] += s_sum[k][w];
   }
-  const int d = threadIdx.x % D, part = threadIdx.x / D;
-  __nv_bfloat16* out = p.out + (static_cast<long long>(b) * p.Hq + hq) * D + d;
+  const int d = threadIdx.x % (D / 4) * 4, part = threadIdx.x / (D / 4);     // four channels, every PARTS-th piece
+  uint2* out = reinterpret_cast<uint2*>(p.out + (static_cast<long long>(b) * p.Hq + hq) * D + d);
   if (tiles == 0) {
-    if (part == 0) *out = __float2bfloat16(0.f);
+    if (part == 0) *out = make_uint2(0, 0);
     return;
   }
   const Deal deal(sum[0] * p.Hkv, p.warps);
@@ -524,54 +595,78 @@ __global__ void __launch_bounds__(kMergeThreads) decode_q4_merge_kernel(const __
   const long long place = first + static_cast<long long>(b) * p.Hkv + h;
   const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + place * G + (hq - h * G);
   const float* o = p.part_o + (place * G + (hq - h * G)) * D + d;
+  // the first pieces' channels are on their way while the weights are made
+  float4 ahead[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    ahead[k] = part + k * PARTS < pieces ? *reinterpret_cast<const float4*>(o + static_cast<long long>(part + k * PARTS) * G * D)
+                                         : make_float4(0.f, 0.f, 0.f, 0.f);
   float mm = -CUDART_INF_F;
-  for (int i = threadIdx.x; i < pieces; i += kMergeThreads) mm = fmaxf(mm, ml[static_cast<long long>(i) * G].x);
+  float2 mine = make_float2(-CUDART_INF_F, 0.f);
+  for (int i = threadIdx.x; i < pieces; i += kMergeThreads) {
+    const float2 v = ml[static_cast<long long>(i) * G];
+    if (i < kMergeThreads) mine = v;
+    mm = fmaxf(mm, v.x);
+  }
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, off));
   if (lane == 0) s_max[warp] = mm;
   __syncthreads();
 #pragma unroll
   for (int w = 0; w < WARPS; ++w) mm = fmaxf(mm, s_max[w]);
-  float acc = 0.f, l = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  float l = 0.f;
+  auto add = [&](const float4& v, float w) {
+    acc.x = fmaf(v.x, w, acc.x);
+    acc.y = fmaf(v.y, w, acc.y);
+    acc.z = fmaf(v.z, w, acc.z);
+    acc.w = fmaf(v.w, w, acc.w);
+  };
   for (int i0 = 0; i0 < pieces; i0 += kMergeThreads) {
     const int n = min(pieces - i0, kMergeThreads);
     if (threadIdx.x < n) {
-      const float2 v = ml[static_cast<long long>(i0 + threadIdx.x) * G];
+      const float2 v = i0 ? ml[static_cast<long long>(i0 + threadIdx.x) * G] : mine;
       const float w = v.x == -CUDART_INF_F ? (v.y == 0.f ? 0.f : 1.f) : b200::ex2_approx(v.x - mm);
       s_w[threadIdx.x] = w;
       l = fmaf(v.y, w, l);
     }
     __syncthreads();
-#pragma unroll 8
-    for (int i = part; i < n; i += PARTS) acc = fmaf(o[static_cast<long long>(i0 + i) * G * D], s_w[i], acc);
+    int i = part;
+    if (i0 == 0) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k, i += PARTS)
+        if (i < n) add(ahead[k], s_w[i]);
+    }
+#pragma unroll 4
+    for (; i < n; i += PARTS) add(*reinterpret_cast<const float4*>(o + static_cast<long long>(i0 + i) * G * D), s_w[i]);
     __syncthreads();
   }
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
   if (lane == 0) s_l[warp] = l;
-  s_o[part][d] = acc;
+  *reinterpret_cast<float4*>(&s_o[part][d]) = acc;
   __syncthreads();
   if (part == 0) {
     l = 0.f;
 #pragma unroll
     for (int w = 0; w < WARPS; ++w) l += s_l[w];
 #pragma unroll
-    for (int k = 1; k < PARTS; ++k) acc += s_o[k][d];
-    *out = __float2bfloat16(acc / l);
+    for (int k = 1; k < PARTS; ++k) add(*reinterpret_cast<const float4*>(&s_o[k][d]), 1.f);
+    *out = make_uint2(b200::pack_bf16x2(acc.x / l, acc.y / l), b200::pack_bf16x2(acc.z / l, acc.w / l));
   }
 }
 
-#ifndef VROWS
-#define VROWS 64
-#define VSTAGES 3
-#define VBLOCKS 2
-#endif
-constexpr int kWarps = 4, kRows = VROWS, kStages = VSTAGES, kBlocks = VBLOCKS;
+// Warps of a block, rows of a tile, blocks an SM; the ring takes the shared memory.  64 sequences of 512 .. 4096 / 16384 rows,
+// heads of 128: 64 rows and 3 blocks 46.6 / 136.5 us, 2 blocks 48.4 / 144.8, 32 rows and 4 blocks 50.8 / 154.5 (what a tile costs
+// besides its rows weighs more than the fourth warp of a scheduler gives).
+constexpr int kWarps = 4, kRows = 64, kBlocks = 3;
+template <int D>
+constexpr int stages() { return D == 128 ? 2 : 4; }
 
 template <int D, bool WIDE>
 int launch(const AttnParams& p, cudaStream_t s) {
-  constexpr int bytes = kWarps * kStages * kRows * (D + D / 8);
-  auto* kern = decode_q4_kernel<D, WIDE, kWarps, kRows, kStages, kBlocks>;
+  constexpr int bytes = kWarps * stages<D>() * kRows * (D + D / 8);
+  auto* kern = decode_q4_kernel<D, WIDE, kWarps, kRows, stages<D>(), kBlocks>;
   static bool configured[b200host::kMaxDevices] = {};
   if (int rc = b200host::ensure_dynamic_smem(kern, bytes, configured)) return rc;
   const bool pdl = b200host::pdl_enabled() != 0;
@@ -609,10 +704,8 @@ extern "C" int b200_q4_decode_attn(const void* q, long long q_batch, const void*
     return b200host::RC_BAD_ALIGNMENT;
   AttnParams p{(const __nv_bfloat16*)q, q_batch, (const uint8_t*)k_codes, (const uint8_t*)k_affine,
                (const uint8_t*)v_codes, (const uint8_t*)v_affine, (const int*)lengths, (const int*)lo,
-               (__nv_bfloat16*)out, (float*)part_o, (float*)part_ml, B, Hq, Hkv, pages, page_rows, runs, fabsf(scale) * kLog2e,
-               scale < 0.f ? 0x80008000u : 0u};
-  // a scale of zero weighs all rows alike, as one does that no score is large enough for; infinite scores stay none
-  if (p.scale_log2 < 1e-36f) p.scale_log2 = 1e-36f;
+               (__nv_bfloat16*)out, (float*)part_o, (float*)part_ml, B, Hq, Hkv, pages, page_rows, runs,
+               scale == 0.f ? 1.f : fabsf(scale) * kLog2e, scale == 0.f ? 0u : ~0u, scale < 0.f ? 0x80008000u : 0u};
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   const bool wide = Hq / Hkv > 4;
   if (D == 128) return wide ? launch<128, true>(p, s) : launch<128, false>(p, s);

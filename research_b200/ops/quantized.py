@@ -365,6 +365,9 @@ def decode_attention_paged_q4(q: torch.Tensor, k_pool: Q4Rows, v_pool: Q4Rows, l
     lengths, lo = _per_sequence(what, "lengths", lengths, B, q), _per_sequence(what, "lo", lo, B, q)
     if lengths is None:
         raise KernelError(f"{what} needs the lengths of the sequences")
+    scale = float(D ** -0.5 if scale is None else scale)
+    if not math.isfinite(scale):
+        raise KernelError(f"{what}: the scale is a finite number, got {scale}")
     _no_gradient(what, q)
     if not q.is_cuda:
         return decode_attention_paged_q4_reference(q, k_pool, v_pool, lengths, lo, scale)
@@ -388,7 +391,7 @@ def decode_attention_paged_q4(q: torch.Tensor, k_pool: Q4Rows, v_pool: Q4Rows, l
             q.data_ptr(), q.stride(0), k_pool.codes.data_ptr(), k_pool.affine.data_ptr(), v_pool.codes.data_ptr(),
             v_pool.affine.data_ptr(), lengths.data_ptr(), native._ptr(lo), out.data_ptr(), parts.data_ptr(),
             parts.data_ptr() + 4 * slots * D, B, Hq, Hkv, D, pages, page_rows, runs,
-            float(D ** -0.5 if scale is None else scale), native._stream()), "b200_q4_decode_attn")
+            scale, native._stream()), "b200_q4_decode_attn")
     native.LAUNCHES += 1                                # _check counts one launch; joining the runs is the second
     return out
 

@@ -199,6 +199,9 @@ def test_refusals_of_attention_and_linear():
                        ((q, *pools, n, n[:1]), "lo is"), ((q.clone().requires_grad_(), *pools, n), "has no gradient")]:
         with pytest.raises(KernelError, match=words):
             q4.decode_attention_paged_q4(*bad)
+    for scale in (float("nan"), float("inf")):
+        with pytest.raises(KernelError, match="finite"):
+            q4.decode_attention_paged_q4(q, *pools, n, scale=scale)
     w = q4.quantize_rows_q4(torch.randn(5, 70))
     x = torch.zeros(2, 70)
     for bad, words in [((x[:, :64], w), "rows of 64 channels"), ((x.int(), w), "x is"), ((torch.zeros(2, 0), w), "x is"),

@@ -1,8 +1,13 @@
 """4-bit rows on the GPU: codes bit for bit against the restatement, attention and linears against 64 bits.
 
 Tolerances count roundings.  A bf16 result is off by 2^-8 of itself at most (half a step).  In front of that, sums of
-products ``x (128 + n)`` are formed in fp32, in the tensor cores' order: a chain of at most 8 additions per group of 64, each off
-by 2^-23 of a running sum that is at most ``sum |x| (144 s + |z|)`` in the result's units, hence 2^-20 of that.
+products ``x n`` are formed in fp32, in the tensor cores' order: a chain of at most 8 additions per group of 64, each off by
+2^-23 of a running sum that is at most ``sum |x| (16 s + |z|)`` in the result's units, hence 2^-20 of that.
+
+A linear's row of x is split into two e4m3 numbers after a power of two has brought its largest value X to 128 .. 256.  A bf16
+of 2^-2 and more is their sum exactly (its 8 bits are 4 in the first and, of what is left, 4 in the second, whose last place
+is 2^-9 or more); a smaller one, below X / 512, is off by half of 2^-9, which is 2^-17 X, times a code of up to 15.  The sum over
+a group is held as 16 a + b + c + d + e, a quarter of it: what is left over is half of 2^-9 again, four times that 2^-15 X.
 """
 
 import math
@@ -121,7 +126,7 @@ def test_write_takes_rows_of_any_layout():
 # ------------------------------------------------------------------------------------------------- attention
 def _attention64(q, k_pool, v_pool, lengths, lo, scale):
     """Result in 64 bits, and the tolerance of the kernel's (see above): ``2^-8 |o|`` for the result, and for what a score is
-    off by, ``d = 2^-20 scale sum |q| (144 s + |z|)``, 2 d of every weight, plus 2^-13 for the weights' own roundings (two
+    off by, ``d = 2^-20 scale sum |q| (16 s + |z|)``, 2 d of every weight, plus 2^-13 for the weights' own roundings (two
     bf16 parts: 2^-15; exponential, sums, tile-wise rescaling)."""
 
     B, Hq, D = q.shape
@@ -129,7 +134,7 @@ def _attention64(q, k_pool, v_pool, lengths, lo, scale):
     G, rows = Hq // Hkv, pages * ps
     dense = [q4.dequantize_rows_reference(p, D, torch.float64).transpose(2, 3).reshape(B, rows, Hkv, D) for p in (k_pool, v_pool)]
     most = [(p.affine[..., 0].double().abs() * m + p.affine[..., 1].double().abs()).repeat_interleave(64, -1)
-            .transpose(2, 3).reshape(B, rows, Hkv, D) for p, m in ((k_pool, 144), (v_pool, 15))]
+            .transpose(2, 3).reshape(B, rows, Hkv, D) for p, m in ((k_pool, 16), (v_pool, 15))]
     out, tol = torch.zeros(B, Hq, D, dtype=torch.float64, device="cuda"), torch.zeros(B, Hq, D, dtype=torch.float64, device="cuda")
     for b in range(B):
         first = 0 if lo is None else max(int(lo[b]), 0)
@@ -237,6 +242,27 @@ def test_rows_of_very_different_size():
     assert (want.abs().max() < 1e-5) and ((got.double() - want).abs() <= tol).all()
 
 
+@pytest.mark.parametrize("D,G", [(128, 4), (64, 8)])
+@pytest.mark.parametrize("q_size,k_size,scale", [(5e37, 1e-37, 0.09), (1e-37, 1e37, 0.1), (1.0, 1.0, 0.0), (5e37, 1.0, 0.0),
+                                                 (1e-37, 1.0, 1e-38), (3e30, 1e-4, -1e-27), (1.0, 1e35, 1e-36)])
+def test_attention_of_extreme_numbers(D, G, q_size, k_size, scale):
+    g = _gen(D)
+    pages, ps = 3, 40
+    q = (torch.randn(3, G, D, generator=g, device="cuda") * q_size).to(BF16)
+    q[:, 1] = 0.0
+    q[:, 2, D // 2:] = 0.0
+    k = q4.quantize_rows_reference((torch.randn(3, pages, 1, ps, D, generator=g, device="cuda") * k_size).to(BF16))
+    v_rows = torch.randn(3, pages, 1, ps, D, generator=g, device="cuda")
+    v_rows[0] *= 1e37
+    v_rows[1, :, :, ::7] *= 1e-30
+    v = q4.quantize_rows_reference(v_rows.to(BF16))
+    lengths = torch.tensor([70, 120, 1], device="cuda", dtype=torch.int32)
+    lo = torch.tensor([66, 0, 0], device="cuda", dtype=torch.int32)
+    want, tol = _attention64(q, k, v, lengths, lo, scale)
+    off = (q4.decode_attention_paged_q4(q, k, v, lengths, lo, scale).double() - want).abs()
+    assert (off <= tol).all(), (off - tol).max()
+
+
 def test_offsets_past_32_bits():
     """Two caches whose words number more than 2^31."""
 
@@ -262,12 +288,18 @@ def test_offsets_past_32_bits():
 
 # ------------------------------------------------------------------------------------------------- linear
 def _linear64(x, w, K):
-    a = w.affine.double()
-    xd = torch.nn.functional.pad(x.double().abs(), (0, w.codes.shape[1] * 2 - K)).unflatten(-1, (-1, 64)).sum(-1)   # per group
+    """Result in 64 bits, what the tolerance of up to 64 rows adds to its rounding, and ``|x| |W|^T``."""
+
+    a, width = w.affine.double(), w.codes.shape[1] * 2
+    s, z = a[..., 0].abs(), a[..., 1].abs()
+    xd = torch.nn.functional.pad(x.double().abs(), (0, width - K)).unflatten(-1, (-1, 64))          # rows, groups, 64
     full = q4.dequantize_rows_reference(w, K, torch.float64)
     want = x.double() @ full.t()
-    sums = xd @ (144 * a[..., 0].abs() + a[..., 1].abs()).t()
-    return want, sums, x.double().abs() @ full.abs().t()
+    most = xd.amax((1, 2), keepdim=True)
+    small = (xd < most / 512).double().sum(-1)
+    sums = xd.sum(-1) @ (16 * s + z).t()                    # 2^-20 per group, and 2^-23 for each of K / 64 additions of groups
+    split = most[:, 0] * (2.0 ** -17 * small @ (15 * s).t() + 2.0 ** -15 * z.sum(-1))
+    return want, sums * (2.0 ** -20 + 2.0 ** -23 * (K / 64)) + split, x.double().abs() @ full.abs().t()
 
 
 @pytest.mark.parametrize("rows", [1, 2, 7, 8, 9, 16, 17, 31, 33, 48, 64, 65, 200])
@@ -277,9 +309,8 @@ def test_linear_against_64_bits(rows, N, K):
     x = torch.randn(rows, K, generator=g, device="cuda").to(BF16)
     w = q4.quantize_rows_q4(torch.randn(N, K, generator=g, device="cuda") * 0.05)
     want, sums, plain = _linear64(x, w, K)
-    # the result's rounding, the products' sums of a group (2^-20), the sum over K / 64 groups in fp32 (2^-23 each, of at most
-    # sum |x| (15 s + |z|)); from 65 rows the weights are rounded to bf16 and the sums run over K in one accumulator
-    tol = 2.0 ** -8 * want.abs() + sums * (2.0 ** -20 + 2.0 ** -23 * (K / 64))
+    # from 65 rows the weights are rounded to bf16 and the sums run over K in one accumulator
+    tol = 2.0 ** -8 * want.abs() + sums
     if rows > 64:
         tol = 2.0 ** -8 * want.abs() + plain * (1.01 * 2.0 ** -8 + 2.0 ** -23 * K)
     got = q4.linear_q4(x, w)
@@ -290,6 +321,27 @@ def test_linear_against_64_bits(rows, N, K):
     wider = torch.zeros(rows, K + 5, device="cuda", dtype=BF16)
     wider[:, 3:K + 3] = x
     assert torch.equal(q4.linear_q4(wider[:, 3:K + 3], w), got)                     # rows on odd addresses
+
+
+@pytest.mark.parametrize("rows", [3, 20, 50])
+def test_linear_rows_of_uneven_size(rows):
+    """A channel of 2^12 times the others' size, a row of tiny values, a row of zeros, one of huge values."""
+
+    g = _gen(rows)
+    N, K = 260, 1100
+    x = torch.randn(rows, K, generator=g, device="cuda")
+    x[0, 77] = 5000.0
+    x[1] *= 1e-30
+    x[2] = 0.0
+    if rows > 3:
+        x[rows - 1] *= 1e25
+        x[rows - 2] *= torch.pow(2.0, torch.randint(-40, 1, (K,), generator=g, device="cuda").float())
+    x = x.to(BF16)
+    w = q4.quantize_rows_q4(torch.randn(N, K, generator=g, device="cuda") * 0.05)
+    want, tol, _ = _linear64(x, w, K)
+    off = (q4.linear_q4(x, w).double() - want).abs()
+    assert (off <= 2.0 ** -8 * want.abs() + tol).all(), (off - 2.0 ** -8 * want.abs() - tol).max()
+    assert torch.count_nonzero(q4.linear_q4(x, w)[2]) == 0
 
 
 def test_linear_shapes_and_broadcast_rows():
@@ -351,7 +403,7 @@ def test_a_step_of_all_of_them_and_its_graph():
     o = q4.decode_attention_paged_q4(q, *pools, position + 1)
     assert ((o.double() - want).abs() <= tol).all()
     y, sums, _ = _linear64(o, wo, 1024)
-    assert ((got.double() - y).abs() <= 2.0 ** -8 * y.abs() + sums * (2.0 ** -20 + 16 * 2.0 ** -23)).all()
+    assert ((got.double() - y).abs() <= 2.0 ** -8 * y.abs() + sums).all()
 
     # two graphs of the same step on caches of their own, replayed at the same time on two streams with new inputs
     sides, graphs = [], []
