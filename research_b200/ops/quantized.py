@@ -153,13 +153,10 @@ def linear_q4_reference(x: torch.Tensor, w: Q4Rows) -> torch.Tensor:
 # --------------------------------------------------------------------------------------------------
 # argument checks
 # --------------------------------------------------------------------------------------------------
-def _records(*tensors: torch.Tensor) -> bool:
-    return torch.is_grad_enabled() and any(t.requires_grad for t in tensors)
-
-
 def _no_gradient(what: str, *tensors: torch.Tensor) -> None:
-    if _records(*tensors):
-        raise KernelError(f"{what} has no gradient: call it under torch.no_grad() or on detached tensors")
+    for t in tensors:
+        if t.requires_grad and torch.is_grad_enabled():
+            raise KernelError(f"{what} has no gradient: call it under torch.no_grad() or on detached tensors")
 
 
 def _same_device(what: str, first: torch.Tensor, *others: torch.Tensor | None) -> None:
@@ -181,9 +178,10 @@ def _on(t: torch.Tensor):
 def _check_rows(what: str, rows: Q4Rows, channels: int) -> None:
     width = row_width(channels)
     codes, affine = rows
-    if (codes.dtype is torch.uint8 and affine.dtype is torch.bfloat16 and codes.shape[-1] * 2 == width
-            and affine.shape == codes.shape[:-1] + (width // GROUP, 2) and codes.is_contiguous()
-            and affine.is_contiguous() and codes.get_device() == affine.get_device()):
+    *shape, half = codes.shape
+    if (half * 2 == width and affine.shape == (*shape, width // GROUP, 2) and codes.dtype is torch.uint8
+            and affine.dtype is torch.bfloat16 and codes.is_contiguous() and affine.is_contiguous()
+            and codes.get_device() == affine.get_device()):
         return
     if codes.dtype != torch.uint8 or affine.dtype != torch.bfloat16:
         raise KernelError(f"{what}: 4-bit rows are uint8 codes and bf16 pairs, got {codes.dtype} and {affine.dtype}")
@@ -196,15 +194,20 @@ def _check_rows(what: str, rows: Q4Rows, channels: int) -> None:
 
 
 def _check_pools(what: str, k_pool: Q4Rows, v_pool: Q4Rows, B: int, Hkv: int | None, D: int) -> tuple[int, int, int]:
-    for pool in (k_pool, v_pool):
-        if pool.codes.dim() != 5:
-            raise KernelError(f"{what}: a cache has codes [B, pages, Hkv, page_rows, D / 2], got {tuple(pool.codes.shape)}")
-        _check_rows(what, pool, D)
-    shape = k_pool.codes.shape
-    if shape != v_pool.codes.shape:
-        raise KernelError(f"{what}: the K and the V cache must have one shape, got {tuple(shape)} and "
-                          f"{tuple(v_pool.codes.shape)}")
-    _same_device(what, k_pool.codes, v_pool.codes)
+    (kc, ka), (vc, va) = k_pool, v_pool
+    shape, pairs, width, at = kc.shape, ka.shape, row_width(D), kc.get_device()
+    if not (len(shape) == 5 and shape[4] * 2 == width and pairs == (*shape[:4], width // GROUP, 2) and vc.shape == shape
+            and va.shape == pairs and kc.dtype is vc.dtype is torch.uint8 and ka.dtype is va.dtype is torch.bfloat16
+            and kc.is_contiguous() and ka.is_contiguous() and vc.is_contiguous() and va.is_contiguous()
+            and at == ka.get_device() == vc.get_device() == va.get_device()):
+        for pool in (k_pool, v_pool):                   # says what is wrong
+            if pool.codes.dim() != 5:
+                raise KernelError(f"{what}: a cache has codes [B, pages, Hkv, page_rows, D / 2], got "
+                                  f"{tuple(pool.codes.shape)}")
+            _check_rows(what, pool, D)
+        if shape != vc.shape:
+            raise KernelError(f"{what}: the K and the V cache must have one shape, got {tuple(shape)} and {tuple(vc.shape)}")
+        _same_device(what, kc, vc)
     seqs, pages, heads, page_rows, _ = shape
     if seqs != B or (Hkv is not None and heads != Hkv):
         raise KernelError(f"{what}: a cache {tuple(shape)} does not hold {B} sequences"
@@ -279,9 +282,13 @@ def _expand(rows: Q4Rows) -> torch.Tensor:
 # --------------------------------------------------------------------------------------------------
 # cache
 # --------------------------------------------------------------------------------------------------
-def _heads_apart(t: torch.Tensor) -> bool:
+def _heads_apart(t: torch.Tensor, Hkv: int, D: int) -> tuple[torch.Tensor, int, int]:
+    """``t [B, T, Hkv, D]`` as the kernel reads it (a copy where heads are not D apart), with the strides of rows and sequences."""
+
     batch, row, head, one = t.stride()
-    return one == 1 and head == t.shape[3] and row % 8 == 0 and batch % 8 == 0 and t.data_ptr() % 16 == 0
+    if one == 1 and head == D and row % 8 == 0 and batch % 8 == 0 and t.data_ptr() % 16 == 0:
+        return t, row, batch
+    return t.contiguous(), Hkv * D, t.shape[1] * Hkv * D
 
 
 def kv_write_paged_q4(k: torch.Tensor, v: torch.Tensor, k_pool: Q4Rows, v_pool: Q4Rows,
@@ -309,11 +316,11 @@ def kv_write_paged_q4(k: torch.Tensor, v: torch.Tensor, k_pool: Q4Rows, v_pool: 
     _head_dim(what, D)
     if k.dtype != torch.bfloat16:
         raise KernelError(f"{what} quantises bf16 rows on a CUDA device, got {k.dtype}")
-    k = k if _heads_apart(k) else k.contiguous()
-    v = v if _heads_apart(v) else v.contiguous()
+    k, k_row, k_batch = _heads_apart(k, Hkv, D)
+    v, v_row, v_batch = _heads_apart(v, Hkv, D)
     with _on(k):
         native._check((native._lib or native.load()).b200_q4_kv_write(
-            k.data_ptr(), v.data_ptr(), k.stride(1), k.stride(0), v.stride(1), v.stride(0), k_pool.codes.data_ptr(),
+            k.data_ptr(), v.data_ptr(), k_row, k_batch, v_row, v_batch, k_pool.codes.data_ptr(),
             k_pool.affine.data_ptr(), v_pool.codes.data_ptr(), v_pool.affine.data_ptr(), native._ptr(start), B, T, Hkv,
             D, pages, page_rows, native._stream()), "b200_q4_kv_write")
 
@@ -336,16 +343,16 @@ def kv_read_paged_q4(k_pool: Q4Rows, v_pool: Q4Rows, rows: int, start: torch.Ten
     _head_dim(what, D)
     if dtype != torch.bfloat16:
         raise KernelError(f"{what} writes bf16 on a CUDA device, got {dtype}")
-    out = torch.empty(2, B, rows, Hkv, D, dtype=torch.bfloat16, device=k_pool.codes.device)
+    out = k_pool.affine.new_empty(2, B, rows, Hkv, D)
     if out.numel() and pages * page_rows:
         with _on(out):
             native._check((native._lib or native.load()).b200_q4_kv_read(
-                out[0].data_ptr(), out[1].data_ptr(), k_pool.codes.data_ptr(), k_pool.affine.data_ptr(),
+                out.data_ptr(), out.data_ptr() + out.numel(), k_pool.codes.data_ptr(), k_pool.affine.data_ptr(),
                 v_pool.codes.data_ptr(), v_pool.affine.data_ptr(), native._ptr(start), B, rows, Hkv, D, pages,
                 page_rows, native._stream()), "b200_q4_kv_read")
     else:
         out.zero_()
-    return out[0], out[1]
+    return out.unbind(0)
 
 
 def decode_attention_paged_q4(q: torch.Tensor, k_pool: Q4Rows, v_pool: Q4Rows, lengths: torch.Tensor,
@@ -375,20 +382,21 @@ def decode_attention_paged_q4(q: torch.Tensor, k_pool: Q4Rows, v_pool: Q4Rows, l
     if q.dtype != torch.bfloat16 or Hq // Hkv > 8:
         raise KernelError(f"{what} supports bf16 queries and up to 8 query heads to a K/V head on a CUDA device, got "
                           f"{q.dtype}, Hq={Hq}, Hkv={Hkv}")
-    if q.stride(2) != 1 or q.stride(1) != D or q.stride(0) % 8 or q.data_ptr() % 16:
-        q = q.contiguous()
-    out = torch.empty(B, Hq * D, dtype=torch.bfloat16, device=q.device)
+    per_row, per_head, one = q.stride()
+    if one != 1 or per_head != D or per_row % 8 or q.data_ptr() % 16:
+        q, per_row = q.contiguous(), Hq * D
+    out = q.new_empty(B, Hq * D)
     if out.numel() == 0:
         return out
     if pages * page_rows == 0:
         return out.zero_()
     lib = native._lib or native.load()
     with _on(q):
-        runs = lib.b200_q4_decode_attn_runs(B, Hkv, pages * page_rows)
+        runs = _attention_runs(B, Hkv, pages * page_rows, q.get_device())
         slots = (runs + B * Hkv) * (Hq // Hkv)
         parts = torch.empty(slots * (D + 2), dtype=torch.float32, device=q.device)
         native._check(lib.b200_q4_decode_attn(
-            q.data_ptr(), q.stride(0), k_pool.codes.data_ptr(), k_pool.affine.data_ptr(), v_pool.codes.data_ptr(),
+            q.data_ptr(), per_row, k_pool.codes.data_ptr(), k_pool.affine.data_ptr(), v_pool.codes.data_ptr(),
             v_pool.affine.data_ptr(), lengths.data_ptr(), native._ptr(lo), out.data_ptr(), parts.data_ptr(),
             parts.data_ptr() + 4 * slots * D, B, Hq, Hkv, D, pages, page_rows, runs,
             scale, native._stream()), "b200_q4_decode_attn")
@@ -396,13 +404,19 @@ def decode_attention_paged_q4(q: torch.Tensor, k_pool: Q4Rows, v_pool: Q4Rows, l
     return out
 
 
+@functools.lru_cache(maxsize=4096)
+def _attention_runs(B: int, Hkv: int, rows: int, device: int) -> int:
+    return native.load().b200_q4_decode_attn_runs(B, Hkv, rows)
+
+
 # --------------------------------------------------------------------------------------------------
 # linear
 # --------------------------------------------------------------------------------------------------
 def linear_q4(x: torch.Tensor, w: Q4Rows) -> torch.Tensor:
     """``y = x W^T`` for ``x [..., K]`` and weights ``w`` of ``N`` 4-bit rows of K channels; ``y [..., N]`` in x's type.  Up to
-    64 rows of x the weights are read as they are (sums of exact products in fp32); for more they are expanded to bf16
-    once, which rounds each to 2^-8 of itself at most, and go through the GEMM."""
+    64 rows of x the weights are read as they are, and x counts to 2^-17 of its row's largest value (a row with an infinity or
+    a NaN gives NaN); for more rows the weights are expanded to bf16 once, which rounds each to 2^-8 of itself at most, and
+    go through the GEMM."""
 
     what = "linear_q4"
     if x.dim() < 1 or not x.is_floating_point() or x.shape[-1] < 1:
@@ -418,26 +432,34 @@ def linear_q4(x: torch.Tensor, w: Q4Rows) -> torch.Tensor:
     if x.dtype != torch.bfloat16:
         raise KernelError(f"{what} takes bf16 rows on a CUDA device, got {x.dtype}")
     N = w.codes.shape[0]
-    x2 = x.reshape(-1, K)
+    x2 = x if x.dim() == 2 else x.reshape(-1, K)
     rows = x2.shape[0]
     if rows == 0 or N == 0:
         return torch.empty(*x.shape[:-1], N, dtype=x.dtype, device=x.device)
     with _on(x):
         if rows > LINEAR_ROWS:
-            return _expanded_linear(x2, w).view(*x.shape[:-1], N)
-        if x2.stride(1) != 1:
-            x2 = x2.contiguous()
-        out = torch.empty(rows, N, dtype=torch.bfloat16, device=x.device)
-        work = None
-        if K > GROUP:                                   # x as the kernel multiplies it: two e4m3 parts, a scale per row
-            tokens, width = 16 if rows <= 16 else -(-rows // 32) * 32, -(-K // 256) * 256
-            work = torch.empty(tokens * (2 * width + width // 2 + 4), dtype=torch.uint8, device=x.device)
-        native._check((native._lib or native.load()).b200_q4_linear(
-            x2.data_ptr(), x2.stride(0), w.codes.data_ptr(), w.affine.data_ptr(), out.data_ptr(), N, rows, N, K,
-            linear_slices(rows, N, K), native._ptr(work), native.status_word(x.device).data_ptr(), native._stream()),
-            "b200_q4_linear")
+            out = _expanded_linear(x2, w)
+        else:
+            out = _few_rows_linear(x2, w, rows, N, K)
+    return out if x2 is x else out.view(*x.shape[:-1], N)
+
+
+def _few_rows_linear(x: torch.Tensor, w: Q4Rows, rows: int, N: int, K: int) -> torch.Tensor:
+    ld, one = x.stride()
+    if one != 1:
+        x, ld = x.contiguous(), K
+    device = x.device
+    out = x.new_empty(rows, N)
+    work = None
+    if K > GROUP:                                       # x as the kernel multiplies it: two e4m3 parts, a scale per row
+        tokens, width = 16 if rows <= 16 else -(-rows // 32) * 32, -(-K // 256) * 256
+        work = w.codes.new_empty(tokens * (2 * width + width // 2 + 4))
+    native._check((native._lib or native.load()).b200_q4_linear(
+        x.data_ptr(), ld, w.codes.data_ptr(), w.affine.data_ptr(), out.data_ptr(), N, rows, N, K,
+        linear_slices(rows, N, K), native._ptr(work), native.status_word(device).data_ptr(), native._stream()),
+        "b200_q4_linear")
     native.LAUNCHES += work is not None                 # _check counts one launch; the split of x is another
-    return out.view(*x.shape[:-1], N)
+    return out
 
 
 def _rows_on_16_bytes(x: torch.Tensor) -> torch.Tensor:
