@@ -26,6 +26,7 @@
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 #include <math_constants.h>
+#include <type_traits>
 
 #include "quant4.cuh"
 #include "host_util.cuh"
@@ -44,7 +45,7 @@ constexpr int ERR_Q4_A = 41, ERR_Q4_D = 42;    // status codes: operands or prod
 
 struct LinearParams {
   const uint8_t* affine;
-  const float* xs;                    // [rows]: what a row of x was divided by
+  const float* xs;                    // [rows]: what a row of x was divided by; null: nothing
   __nv_bfloat16* out;
   long long ldo;
   int rows, N, width, cluster, stages, token_tiles;
@@ -212,6 +213,49 @@ __global__ void __launch_bounds__(512) linear_q4_split_kernel(const __nv_bfloat1
       *reinterpret_cast<uint4*>(at) = make_uint4(all, all, all, all);
       *reinterpret_cast<uint4*>(at + 16) = make_uint4(part[1] | part[2] << 8 | part[3] << 16 | part[4] << 24, 0, 0, 0);
     }
+  }
+}
+
+// Writes the block's part of the result: weight rows [rank, rank + 1) * 128 / cluster of every token of the tile, from the
+// sums red[token][128] of the cluster's blocks, added in rank order.
+template <int NT>
+__device__ __forceinline__ void finish(float* red, const LinearParams& p, int tile, int tokens0, int rank, int threads) {
+  pdl_wait();   // what the output replaces may still be read by the predecessor
+  const int width = 128 / p.cluster, vecs = width >> 2;
+  const int rows = min(p.rows - tokens0 * NT, NT);
+  for (int it = threadIdx.x; it < rows * vecs; it += threads) {
+    const int token = it / vecs, nl = rank * width + (it - token * vecs) * 4, n = tile * 128 + nl;
+    if (n >= p.N) continue;
+    const float* at = red + token * 128 + nl;
+    float4 v = *reinterpret_cast<const float4*>(at);
+    if (p.cluster > 1) {
+      v = ld_cluster4(smem_u32(at), 0);
+      for (int r = 1; r < p.cluster; ++r) {
+        const float4 w = ld_cluster4(smem_u32(at), r);
+        v.x += w.x;
+        v.y += w.y;
+        v.z += w.z;
+        v.w += w.w;
+      }
+    }
+    const float scale = p.xs ? p.xs[tokens0 * NT + token] : 1.f;
+    v.x *= scale;
+    v.y *= scale;
+    v.z *= scale;
+    v.w *= scale;
+    __nv_bfloat16* dst = p.out + (tokens0 * NT + token) * p.ldo + n;
+    if (((p.N | p.ldo) & 3) == 0) {
+      *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16x2(v.x, v.y), pack_bf16x2(v.z, v.w));
+    } else {
+      const float e[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (n + i < p.N) dst[i] = __float2bfloat16(e[i]);
+    }
+  }
+  if (p.cluster > 1) {
+    __syncwarp();
+    cluster_sync();   // peers may still read this block's sums
   }
 }
 
@@ -439,44 +483,212 @@ linear_q4_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant_
     tmem_dealloc(tmem, TMEM_COLUMNS);
   }
 
-  // weight rows [rank, rank + 1) * 128 / cluster, summed over the cluster in rank order
-  pdl_wait();   // what the output replaces may still be read by the predecessor
-  const int width = 128 / p.cluster, vecs = width >> 2;
-  const int rows = min(p.rows - tokens0 * NT, NT);
-  for (int it = threadIdx.x; it < rows * vecs; it += kThreads) {
-    const int token = it / vecs, nl = rank * width + (it - token * vecs) * 4, n = tile * 128 + nl;
-    if (n >= p.N) continue;
-    const float* at = red + token * 128 + nl;
-    float4 v = *reinterpret_cast<const float4*>(at);
-    if (p.cluster > 1) {
-      v = ld_cluster4(smem_u32(at), 0);
-      for (int r = 1; r < p.cluster; ++r) {
-        const float4 w = ld_cluster4(smem_u32(at), r);
-        v.x += w.x;
-        v.y += w.y;
-        v.z += w.z;
-        v.w += w.w;
+  finish<NT>(red, p, tile, tokens0, rank, kThreads);
+}
+
+// More than 64 rows of x: y = x W^T in bf16, tiles of 128 weight rows and 128 tokens, one block an SM, the weights expanded into
+// tensor memory on their way.  The products of 128 x 128 x 128 take the tensor cores 512 clocks, expanding the codes for them
+// takes each scheduler about 300 issue slots (a mask and a shift, 128 + n - 128, n s + z for two channels, rounded once), so that
+// a matrix of bf16 weights need be neither written nor read.  (Taking the groups' products by themselves, as above, would
+// need an FMA and a read of tensor memory for each of them and each group: 46 us for 777 rows of 5632 x 2048 channels.)
+//   warp 0      TMA: codes of 256 channels, x of 128 channels, in the order of use
+//   warp 1      MMA issuer
+//   warps 4-11  two for a quadrant's 32 weight rows: each expands half of a step's channels
+constexpr int kManyTokens = 128, kManyThreads = 384;
+constexpr int kManyX = 2 * kManyTokens * 128, kManyXStages = 5, kManyCodeStages = 3;
+constexpr int kManyWeights = 4, kManySums = 256;   // tensor memory: 4 x 64 columns of weights, 128 of sums
+
+// Place in a ring of N, and the parity of its round.
+template <int N>
+struct Place {
+  int at = 0;
+  uint32_t round = 0;
+  __device__ __forceinline__ void on() {
+    if (++at == N) at = 0, round ^= 1;
+  }
+};
+
+// Values of a word as eight bf16 in channel order, n s + z rounded once; s2 and z2 hold s and z twice.
+__device__ __forceinline__ void values(uint32_t word, uint32_t s2, uint32_t z2, uint32_t mask, uint32_t magic, uint32_t* to) {
+  const uint32_t coded_pairs[4] = {coded<0>(word, mask, magic), coded<1>(word, mask, magic), coded<2>(word, mask, magic),
+                                   coded<3>(word, mask, magic)};
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    uint32_t n;
+    asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(n) : "r"(coded_pairs[k]), "r"(magic));      // magic: 128, twice
+    asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(to[k]) : "r"(n), "r"(s2), "r"(z2));
+  }
+}
+
+__global__ void __launch_bounds__(kManyThreads, 1)
+linear_q4_many_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX,
+                      const __grid_constant__ LinearParams p) {
+  constexpr int NT = kManyTokens;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* codes = smem + kManyXStages * kManyX;
+  __shared__ uint64_t x_full[kManyXStages], x_empty[kManyXStages], c_full[kManyCodeStages], c_empty[kManyCodeStages];
+  __shared__ uint64_t w_full[kManyWeights], w_empty[kManyWeights], done[1];
+  __shared__ uint32_t tmem_slot[1];
+  __shared__ int abort_word;
+  pdl_launch_dependents();
+  volatile int* abort_flag = &abort_word;
+  const AbortCtx ab{abort_flag, p.status};
+  const int warp = warp_uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
+  const int rank = blockIdx.x % p.cluster;
+  const int tokens0 = blockIdx.x / p.cluster % p.token_tiles, tile = blockIdx.x / p.cluster / p.token_tiles;
+  const int blocks = (p.width + kStage - 1) / kStage, per = (blocks + p.cluster - 1) / p.cluster;
+  const int step0 = 2 * rank * per;                                         // steps of 128 channels, two groups each
+  const int steps = max(min(2 * per, p.width / 128 - step0), 0);
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kManyXStages; ++s) mbar_init(&x_full[s], 1), mbar_init(&x_empty[s], 1);
+    for (int s = 0; s < kManyCodeStages; ++s) mbar_init(&c_full[s], 1), mbar_init(&c_empty[s], 8);
+    for (int s = 0; s < kManyWeights; ++s) mbar_init(&w_full[s], 8), mbar_init(&w_empty[s], 1);
+    mbar_init(done, 1);
+    *abort_flag = 0;
+    mbar_fence_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  float* red = reinterpret_cast<float*>(smem);   // [token][128], over the ring of x once everything has been read
+
+  if (warp == 0) {
+    if (elect_one()) {
+      tma_prefetch_desc(&tmW);
+      tma_prefetch_desc(&tmX);
+      for (int i = 0; i < min((steps + 1) / 2, 4); ++i) tma_prefetch_l2_2d(&tmW, (step0 + 2 * i) * 64, tile * 128);
+      pdl_wait();
+      bool ok = true;
+      Place<kManyXStages> x;
+      Place<kManyCodeStages> c;
+      for (int j = 0; j < steps; ++j) {
+        if ((j & 1) == 0) {
+          ok = wait(&c_empty[c.at], c.round ^ 1, ab, ERR_WAIT_EMPTY);
+          if (!ok) break;
+          mbar_expect_tx(&c_full[c.at], kCodeBytes);
+          tma_load_2d(codes + c.at * kCodeBytes, &tmW, &c_full[c.at], (step0 + j) * 64, tile * 128);
+          c.on();
+        }
+        ok = wait(&x_empty[x.at], x.round ^ 1, ab, ERR_WAIT_EMPTY);
+        if (!ok) break;
+        uint8_t* to = smem + x.at * kManyX;
+        mbar_expect_tx(&x_full[x.at], kManyX);
+        tma_load_2d(to, &tmX, &x_full[x.at], (step0 + j) * 128, tokens0 * NT);
+        tma_load_2d(to + kManyX / 2, &tmX, &x_full[x.at], (step0 + j) * 128 + 64, tokens0 * NT);
+        x.on();
+      }
+      if (!ok) {
+        // give copies already in flight time to land before the CTA's shared memory goes away
+        const uint64_t t0 = globaltimer_ns();
+        while (globaltimer_ns() - t0 < 200000ull) __nanosleep(1000);
       }
     }
-    const float scale = p.xs[tokens0 * NT + token];
-    v.x *= scale;
-    v.y *= scale;
-    v.z *= scale;
-    v.w *= scale;
-    __nv_bfloat16* dst = p.out + (tokens0 * NT + token) * p.ldo + n;
-    if (((p.N | p.ldo) & 3) == 0) {
-      *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16x2(v.x, v.y), pack_bf16x2(v.z, v.w));
-    } else {
-      const float e[4] = {v.x, v.y, v.z, v.w};
+  } else if (warp == 1) {
+    if (elect_one()) {
+      constexpr uint32_t idesc = make_idesc_bf16(128, NT, false, false);
+      bool ok = true;
+      Place<kManyXStages> x;
+      Place<kManyWeights> w;
+      for (int j = 0; j < steps; ++j) {
+        ok = wait(&x_full[x.at], x.round, ab, ERR_WAIT_FULL) && wait(&w_full[w.at], w.round, ab, ERR_Q4_A);
+        if (!ok) break;
+        tc_fence_after();
+        const uint64_t xdesc = make_smem_desc_sw128(smem_u32(smem + x.at * kManyX), 16, 1024);
+        const uint32_t weights = tmem + w.at * 64;
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (n + i < p.N) dst[i] = __float2bfloat16(e[i]);
+        for (int k = 0; k < 8; ++k)              // 16 channels each, 64 to a box of x
+          tc_mma_ts(tmem + kManySums, weights + k * 8, xdesc + (uint64_t)(((k >> 2) * (kManyX / 2) + (k & 3) * 32) >> 4), idesc,
+                    (j | k) != 0 ? 1u : 0u);
+        tc_commit(&x_empty[x.at]);
+        tc_commit(&w_empty[w.at]);
+        x.on();
+        w.on();
+      }
+      if (ok && steps > 0) tc_commit(done);
+    }
+  } else if (warp >= 4) {
+    const int quad = warp & 3, row = quad * 32 + lane, side = (warp - 4) >> 2;
+    const uint32_t lane_sel = static_cast<uint32_t>(quad * 32) << 16;
+    const uint2* pairs = reinterpret_cast<const uint2*>(
+        p.affine + static_cast<long long>(min(tile * 128 + row, p.N - 1)) * (p.width / 16)) + step0;
+    uint32_t mask, magic;
+    opaque_masks(mask, magic);
+    pdl_wait();
+    bool ok = true;
+    uint2 f[2] = {steps > 0 ? __ldg(pairs) : make_uint2(0, 0), steps > 1 ? __ldg(pairs + 1) : make_uint2(0, 0)};
+    Place<kManyCodeStages> c;
+    Place<kManyWeights> w;
+    for (int j0 = 0; j0 < steps && ok; j0 += 2) {
+      ok = wait_warp(&c_full[c.at], c.round, ab, ERR_WAIT_FULL);
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const int j = j0 + half;
+        if (j >= steps || !ok) break;
+        const uint2 pair = f[half];
+        f[half] = j + 2 < steps ? __ldg(pairs + j + 2) : make_uint2(0, 0);
+        uint32_t r[2][16];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {            // word 4 c + k: channels 64 (k & 1) + 8 (2 c + k / 2) ..
+          const uint4 v = *reinterpret_cast<const uint4*>(codes + c.at * kCodeBytes + sw128_offset(row, half * 4 + 2 * side + k));
+          const uint32_t s0 = __byte_perm(pair.x, pair.x, 0x1010), z0 = __byte_perm(pair.x, pair.x, 0x3232);
+          const uint32_t s1 = __byte_perm(pair.y, pair.y, 0x1010), z1 = __byte_perm(pair.y, pair.y, 0x3232);
+          values(v.x, s0, z0, mask, magic, &r[0][8 * k]);
+          values(v.y, s1, z1, mask, magic, &r[1][8 * k]);
+          values(v.z, s0, z0, mask, magic, &r[0][8 * k + 4]);
+          values(v.w, s1, z1, mask, magic, &r[1][8 * k + 4]);
+        }
+        ok = wait_warp(&w_empty[w.at], w.round ^ 1, ab, ERR_Q4_D);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t to = tmem + w.at * 64 + side * 16 + lane_sel;
+        tmem_st16(to, r[0]);
+        tmem_st16(to + 32, r[1]);
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&w_full[w.at]);
+          if (half || j + 1 == steps) mbar_arrive(&c_empty[c.at]);
+        }
+        w.on();
+      }
+      c.on();
+    }
+    if (steps > 0) ok = ok && wait_warp(done, 0, ab, ERR_Q4_D);
+    tc_fence_after();
+    // every product has been made, so every copy has landed and every operand has been used: the ring is free
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      uint32_t v[32];
+      if (steps > 0 && ok) {
+        tmem_ld_32x32b_x32(tmem + kManySums + side * 64 + k * 32 + lane_sel, v);
+        tmem_ld_wait();
+      } else {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) v[i] = 0;
+      }
+#pragma unroll
+      for (int i = 0; i < 32; ++i) red[(side * 64 + k * 32 + i) * 128 + row] = __uint_as_float(v[i]);
     }
   }
-  if (p.cluster > 1) {
-    __syncwarp();
-    cluster_sync();   // peers may still read this block's sums
+  __syncwarp();
+  tc_fence_before();
+  if (p.cluster > 1)
+    cluster_sync();
+  else
+    __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
   }
+  finish<NT>(red, p, tile, tokens0, rank, kManyThreads);
 }
 
 // Rows of up to 64 channels (one group, words in channel order): one warp per weight row and eight rows of x, a lane per word.
@@ -508,21 +720,12 @@ __global__ void __launch_bounds__(128) linear_q4_narrow_kernel(const __nv_bfloat
   }
 }
 
-template <int NT>
-int launch(const CUtensorMap& tmW, const CUtensorMap& tmX, const CUtensorMap& tmS, LinearParams p, cudaStream_t stream) {
-  auto* kern = linear_q4_kernel<NT>;
-  const int blocks = (p.width + kStage - 1) / kStage, slice = (blocks + p.cluster - 1) / p.cluster;
-  p.stages = (222 * 1024 / blocks_per_sm<NT>() - 2048) / stage_bytes<NT>();
-  if (p.stages > kMaxStages) p.stages = kMaxStages;
-  if (p.stages > slice) p.stages = slice;
-  if (p.stages < 2) p.stages = 2;
-  const int ring = p.stages * stage_bytes<NT>(), sums = NT * 128 * 4;   // the partial sums reuse the ring
-  const int smem_bytes = (ring > sums ? ring : sums) + 1024;
-  static bool configured[b200host::kMaxDevices] = {};
-  if (int rc = b200host::ensure_dynamic_smem(kern, 200 * 1024, configured)) return rc;
+template <typename... Args>
+int launch_cluster(void (*kern)(Args...), const LinearParams& p, int threads, int smem_bytes, cudaStream_t stream,
+                   const std::common_type_t<Args>&... args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((p.N + 127) / 128 * p.token_tiles * p.cluster);
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = smem_bytes;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
@@ -533,7 +736,29 @@ int launch(const CUtensorMap& tmW, const CUtensorMap& tmX, const CUtensorMap& tm
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = b200host::pdl_enabled() ? 2 : 1;
-  return static_cast<int>(cudaLaunchKernelEx(&cfg, kern, tmW, tmX, tmS, p));
+  return static_cast<int>(cudaLaunchKernelEx(&cfg, kern, args...));
+}
+
+template <int NT>
+int launch(const CUtensorMap& tmW, const CUtensorMap& tmX, const CUtensorMap& tmS, LinearParams p, cudaStream_t stream) {
+  const int blocks = (p.width + kStage - 1) / kStage, slice = (blocks + p.cluster - 1) / p.cluster;
+  p.stages = (222 * 1024 / blocks_per_sm<NT>() - 2048) / stage_bytes<NT>();
+  if (p.stages > kMaxStages) p.stages = kMaxStages;
+  if (p.stages > slice) p.stages = slice;
+  if (p.stages < 2) p.stages = 2;
+  const int ring = p.stages * stage_bytes<NT>(), sums = NT * 128 * 4;   // the partial sums reuse the ring
+  const int smem_bytes = (ring > sums ? ring : sums) + 1024;
+  static bool configured[b200host::kMaxDevices] = {};
+  if (int rc = b200host::ensure_dynamic_smem(linear_q4_kernel<NT>, 200 * 1024, configured)) return rc;
+  return launch_cluster(linear_q4_kernel<NT>, p, kThreads, smem_bytes, stream, tmW, tmX, tmS, p);
+}
+
+int launch_many(const CUtensorMap& tmW, const CUtensorMap& tmX, const LinearParams& p, cudaStream_t stream) {
+  constexpr int bytes = kManyXStages * kManyX + kManyCodeStages * kCodeBytes + 1024;
+  static_assert(kManyXStages * kManyX >= kManyTokens * 128 * 4 && bytes <= 226 * 1024, "shared memory");
+  static bool configured[b200host::kMaxDevices] = {};
+  if (int rc = b200host::ensure_dynamic_smem(linear_q4_many_kernel, bytes, configured)) return rc;
+  return launch_cluster(linear_q4_many_kernel, p, kManyThreads, bytes, stream, tmW, tmX, p);
 }
 
 }  // namespace
@@ -545,7 +770,7 @@ extern "C" int b200_q4_linear(const void* x, long long ldx, const void* codes, c
                               long long ldo, int rows, int N, int K, int cluster, void* work, void* status,
                               void* stream) {
   using namespace b200host;
-  if (rows <= 0 || rows > 64 || N <= 0 || K <= 0 || K > (1 << 30) || !status) return RC_BAD_SHAPE;
+  if (rows <= 0 || rows > 4096 || N <= 0 || K <= 0 || K > (1 << 30) || !status) return RC_BAD_SHAPE;
   if (cluster != 1 && cluster != 2 && cluster != 4 && cluster != 8) return RC_BAD_SHAPE;
   if ((reinterpret_cast<uintptr_t>(codes) | reinterpret_cast<uintptr_t>(affine)) & 15) return RC_BAD_ALIGNMENT;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
@@ -555,15 +780,21 @@ extern "C" int b200_q4_linear(const void* x, long long ldx, const void* codes, c
     return static_cast<int>(launch_kernel(linear_q4_narrow_kernel, dim3((N + 3) / 4, (rows + 7) / 8), dim3(128), 0, s, pdl,
                                           (const __nv_bfloat16*)x, ldx, (const uint32_t*)codes, (const uint32_t*)affine,
                                           (__nv_bfloat16*)out, ldo, rows, N, K));
-  if (!work || ((reinterpret_cast<uintptr_t>(work) & 15) | (reinterpret_cast<uintptr_t>(out) & 7))) return RC_BAD_ALIGNMENT;
+  if (reinterpret_cast<uintptr_t>(out) & 7) return RC_BAD_ALIGNMENT;
+  CUtensorMap tmW, tmX, tmS;
+  int rc;
+  if ((rc = make_map_2d(&tmW, CU_TENSOR_MAP_DATA_TYPE_UINT8, codes, width / 2, N, width / 2, 128, 128))) return rc;
+  if (rows > 64) {
+    if ((rc = make_map_2d(&tmX, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, x, K, rows, ldx * 2, 64, kManyTokens))) return rc;
+    return launch_many(tmW, tmX, LinearParams{(const uint8_t*)affine, nullptr, (__nv_bfloat16*)out, ldo, rows, N, width, cluster,
+                                              0, (rows + kManyTokens - 1) / kManyTokens, (int*)status}, s);
+  }
+  if (!work || (reinterpret_cast<uintptr_t>(work) & 15)) return RC_BAD_ALIGNMENT;
   const int NT = rows <= 16 ? 16 : 32, tiles = (rows + NT - 1) / NT, tokens = NT * tiles;
   const int xwidth = (K + kStage - 1) / kStage * kStage;
   uint8_t* xq = static_cast<uint8_t*>(work);
   uint8_t* sums = xq + 2ll * tokens * xwidth;
   float* xs = reinterpret_cast<float*>(sums + tokens * (xwidth / 2ll));
-  CUtensorMap tmW, tmX, tmS;
-  int rc;
-  if ((rc = make_map_2d(&tmW, CU_TENSOR_MAP_DATA_TYPE_UINT8, codes, width / 2, N, width / 2, 128, 128))) return rc;
   if ((rc = make_map_2d(&tmX, CU_TENSOR_MAP_DATA_TYPE_UINT8, xq, xwidth, 2 * tokens, xwidth, 128, 2 * NT))) return rc;
   if ((rc = make_map_2d(&tmS, CU_TENSOR_MAP_DATA_TYPE_UINT8, sums, xwidth / 2, tokens, xwidth / 2, 128, NT))) return rc;
   const int aligned = ldx % 8 == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0;

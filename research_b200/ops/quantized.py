@@ -30,7 +30,7 @@ from research_b200.ops import native
 
 GROUP = 64
 #: Rows up to which a product reads the 4-bit weights themselves; above, they are expanded once for the GEMM.
-LINEAR_ROWS = 64
+LINEAR_ROWS = 2048
 
 
 class Q4Rows(NamedTuple):
@@ -437,26 +437,30 @@ def linear_q4(x: torch.Tensor, w: Q4Rows) -> torch.Tensor:
     if rows == 0 or N == 0:
         return torch.empty(*x.shape[:-1], N, dtype=x.dtype, device=x.device)
     with _on(x):
-        if rows > LINEAR_ROWS:
+        if rows > LINEAR_ROWS or (rows > 64 and K <= GROUP):
             out = _expanded_linear(x2, w)
         else:
-            out = _few_rows_linear(x2, w, rows, N, K)
+            out = _coded_linear(x2, w, rows, N, K)
     return out if x2 is x else out.view(*x.shape[:-1], N)
 
 
-def _few_rows_linear(x: torch.Tensor, w: Q4Rows, rows: int, N: int, K: int) -> torch.Tensor:
+def _coded_linear(x: torch.Tensor, w: Q4Rows, rows: int, N: int, K: int) -> torch.Tensor:
+    work = None
+    if rows > 64:
+        x, slices = _rows_on_16_bytes(x), many_rows_slices(rows, N, K)
+    else:
+        slices = linear_slices(rows, N, K)
+        if K > GROUP:                                   # x as the kernel multiplies it: two e4m3 parts, a scale per row
+            tokens, width = 16 if rows <= 16 else -(-rows // 32) * 32, -(-K // 256) * 256
+            work = w.codes.new_empty(tokens * (2 * width + width // 2 + 4))
     ld, one = x.stride()
     if one != 1:
         x, ld = x.contiguous(), K
     device = x.device
     out = x.new_empty(rows, N)
-    work = None
-    if K > GROUP:                                       # x as the kernel multiplies it: two e4m3 parts, a scale per row
-        tokens, width = 16 if rows <= 16 else -(-rows // 32) * 32, -(-K // 256) * 256
-        work = w.codes.new_empty(tokens * (2 * width + width // 2 + 4))
     native._check((native._lib or native.load()).b200_q4_linear(
         x.data_ptr(), ld, w.codes.data_ptr(), w.affine.data_ptr(), out.data_ptr(), N, rows, N, K,
-        linear_slices(rows, N, K), native._ptr(work), native.status_word(device).data_ptr(), native._stream()),
+        slices, native._ptr(work), native.status_word(device).data_ptr(), native._stream()),
         "b200_q4_linear")
     native.LAUNCHES += work is not None                 # _check counts one launch; the split of x is another
     return out
@@ -487,6 +491,21 @@ def linear_slices(rows: int, n: int, k: int, sms: int = 148) -> int:
         per_sm = math.ceil(tiles * s / sms - 0.1)
         waves = -(-per_sm // room)                      # of blocks, each with 2.5 us to begin and to end
         cost = -(-stages // s) * max(alone, (per_sm if waves == 1 else waves * room) * shared) + exchange + (waves - 1) * 2.5
+        if cost < best_cost:
+            best, best_cost = s, cost
+    return best
+
+
+@functools.lru_cache(maxsize=4096)
+def many_rows_slices(rows: int, n: int, k: int, sms: int = 148) -> int:
+    """Slices of K as above, for more than 64 rows."""
+
+    tiles, stages = -(-n // 128) * -(-rows // 128), -(-k // 256)
+    best, best_cost = 1, float("inf")
+    for s in (1, 2, 4, 8):
+        if s > 1 and stages < s:
+            break
+        cost = math.ceil(tiles * s / sms) * (-(-stages // s) * 0.6 + 3.0)
         if cost < best_cost:
             best, best_cost = s, cost
     return best
