@@ -1,15 +1,15 @@
-// y = x W^T for up to 64 rows of x and weights held in 4 bits (quant4.cuh): x [rows, K] bf16, W [N, K], y [rows, N] bf16 with
-// fp32 sums.  The time is that of streaming the codes once (0.56 bytes a weight), as long as expanding them keeps up: at the
+// y = x W^T with weights held in 4 bits (quant4.cuh): x [rows, K] bf16, W [N, K], y [rows, N] bf16 with fp32 sums.  For more
+// than 64 rows of x see linear_q4_many_kernel; what follows is up to 64.  The time is that of streaming the codes once (0.56 bytes a weight), as long as expanding them keeps up: at the
 // copy bandwidth an SM gets 46 codes a clock, which is what the arrangement below is for.
 //
 // The weights are the 128-row operand of tcgen05.mma, from tensor memory, the rows of x its columns (16 or 32 at a time), both in
 // e4m3.  The bytes 0 .. 15 are, as e4m3, the numbers n 2^-9 (subnormals and the first binade are one straight line), so that a
 // word of eight codes becomes eight operands by two masks and a shift, a third of what bf16 operands take, in half the tensor
 // memory.  A row of x is brought to [128, 256) by a power of two and split into two e4m3 numbers, high + low, which go into
-// one accumulator: the eight bits of a bf16 are two times four, so that is exact down to 2^-10 of the row's largest value, and
-// below that off by 2^-19 of it at most.  The product of each group is taken by itself.  The sum X_g of x over a group gets
+// one accumulator: the eight bits of a bf16 are two times four, so that is exact down to 2^-9 of the row's largest value, and
+// below that off by 2^-17 of it at most.  The product of each group is taken by itself.  The sum X_g of x over a group gets
 // into every lane as a product too, of fours with 32 e4m3 numbers that add up to a quarter of it (16 times its sixteenth, then
-// what is left: to 2^-16 of the row's largest value); scales and least values are applied to both in fp32:
+// what is left: to 2^-15 of the row's largest value); scales and least values are applied to both in fp32:
 //   y = x_max (sum_g s_g (sum_k x'_k n_k) + z_g X'_g),   x' = x / x_max
 // (weights rounded to bf16 instead would cost as much precision again as the result's own rounding; sums and scales of x from
 // shared memory, the same word for all lanes, take one pass a word: 16 passes a column and 128 x 128 block, 85 us for 28672 x
@@ -492,11 +492,13 @@ linear_q4_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant_
 // a matrix of bf16 weights need be neither written nor read.  (Taking the groups' products by themselves, as above, would
 // need an FMA and a read of tensor memory for each of them and each group: 46 us for 777 rows of 5632 x 2048 channels.)
 //   warp 0      TMA: codes of 256 channels, x of 128 channels, in the order of use
-//   warp 1      MMA issuer
-//   warps 4-11  two for a quadrant's 32 weight rows: each expands half of a step's channels
-constexpr int kManyTokens = 128, kManyThreads = 384;
-constexpr int kManyX = 2 * kManyTokens * 128, kManyXStages = 5, kManyCodeStages = 3;
-constexpr int kManyWeights = 4, kManySums = 256;   // tensor memory: 4 x 64 columns of weights, 128 of sums
+//   warp 1      MMA issuer: one wait and one commit a step (each takes the thread a good 100 clocks in which it issues nothing:
+//               with barriers of their own for weights and x, 777 rows of 5632 x 2048 channels took 28.0 us instead of 23.1)
+//   warps 4-19  four for a quadrant's 32 weight rows: each expands half of every second step's channels
+constexpr int kManyTokens = 128, kManyThreads = 640;
+constexpr int kManyX = 2 * kManyTokens * 128, kManyCodeStages = 5;
+constexpr int kManySteps = 4;         // steps whose operands are there at a time, with one barrier for both operands
+constexpr int kManySums = kManySteps * 64;   // tensor memory: 4 x 64 columns of weights, 128 of sums
 
 // Place in a ring of N, and the parity of its round.
 template <int N>
@@ -505,6 +507,10 @@ struct Place {
   uint32_t round = 0;
   __device__ __forceinline__ void on() {
     if (++at == N) at = 0, round ^= 1;
+  }
+  __device__ __forceinline__ void on2() {
+    at += 2;
+    if (at >= N) at -= N, round ^= 1;
   }
 };
 
@@ -526,9 +532,8 @@ linear_q4_many_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_cons
   constexpr int NT = kManyTokens;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* codes = smem + kManyXStages * kManyX;
-  __shared__ uint64_t x_full[kManyXStages], x_empty[kManyXStages], c_full[kManyCodeStages], c_empty[kManyCodeStages];
-  __shared__ uint64_t w_full[kManyWeights], w_empty[kManyWeights], done[1];
+  uint8_t* codes = smem + kManySteps * kManyX;
+  __shared__ uint64_t full[kManySteps], empty[kManySteps], c_full[kManyCodeStages], c_empty[kManyCodeStages], done[1];
   __shared__ uint32_t tmem_slot[1];
   __shared__ int abort_word;
   pdl_launch_dependents();
@@ -542,9 +547,8 @@ linear_q4_many_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_cons
   const int steps = max(min(2 * per, p.width / 128 - step0), 0);
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < kManyXStages; ++s) mbar_init(&x_full[s], 1), mbar_init(&x_empty[s], 1);
-    for (int s = 0; s < kManyCodeStages; ++s) mbar_init(&c_full[s], 1), mbar_init(&c_empty[s], 8);
-    for (int s = 0; s < kManyWeights; ++s) mbar_init(&w_full[s], 8), mbar_init(&w_empty[s], 1);
+    for (int s = 0; s < kManySteps; ++s) mbar_init(&full[s], 8 + 1), mbar_init(&empty[s], 1);   // expanders' warps, x
+    for (int s = 0; s < kManyCodeStages; ++s) mbar_init(&c_full[s], 1), mbar_init(&c_empty[s], 16);
     mbar_init(done, 1);
     *abort_flag = 0;
     mbar_fence_init();
@@ -566,7 +570,7 @@ linear_q4_many_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_cons
       for (int i = 0; i < min((steps + 1) / 2, 4); ++i) tma_prefetch_l2_2d(&tmW, (step0 + 2 * i) * 64, tile * 128);
       pdl_wait();
       bool ok = true;
-      Place<kManyXStages> x;
+      Place<kManySteps> x;
       Place<kManyCodeStages> c;
       for (int j = 0; j < steps; ++j) {
         if ((j & 1) == 0) {
@@ -576,12 +580,12 @@ linear_q4_many_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_cons
           tma_load_2d(codes + c.at * kCodeBytes, &tmW, &c_full[c.at], (step0 + j) * 64, tile * 128);
           c.on();
         }
-        ok = wait(&x_empty[x.at], x.round ^ 1, ab, ERR_WAIT_EMPTY);
+        ok = wait(&empty[x.at], x.round ^ 1, ab, ERR_WAIT_EMPTY);
         if (!ok) break;
         uint8_t* to = smem + x.at * kManyX;
-        mbar_expect_tx(&x_full[x.at], kManyX);
-        tma_load_2d(to, &tmX, &x_full[x.at], (step0 + j) * 128, tokens0 * NT);
-        tma_load_2d(to + kManyX / 2, &tmX, &x_full[x.at], (step0 + j) * 128 + 64, tokens0 * NT);
+        mbar_expect_tx(&full[x.at], kManyX);
+        tma_load_2d(to, &tmX, &full[x.at], (step0 + j) * 128, tokens0 * NT);
+        tma_load_2d(to + kManyX / 2, &tmX, &full[x.at], (step0 + j) * 128 + 64, tokens0 * NT);
         x.on();
       }
       if (!ok) {
@@ -594,27 +598,24 @@ linear_q4_many_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_cons
     if (elect_one()) {
       constexpr uint32_t idesc = make_idesc_bf16(128, NT, false, false);
       bool ok = true;
-      Place<kManyXStages> x;
-      Place<kManyWeights> w;
+      Place<kManySteps> x;
       for (int j = 0; j < steps; ++j) {
-        ok = wait(&x_full[x.at], x.round, ab, ERR_WAIT_FULL) && wait(&w_full[w.at], w.round, ab, ERR_Q4_A);
+        ok = wait(&full[x.at], x.round, ab, ERR_WAIT_FULL);
         if (!ok) break;
         tc_fence_after();
         const uint64_t xdesc = make_smem_desc_sw128(smem_u32(smem + x.at * kManyX), 16, 1024);
-        const uint32_t weights = tmem + w.at * 64;
+        const uint32_t weights = tmem + x.at * 64;
 #pragma unroll
         for (int k = 0; k < 8; ++k)              // 16 channels each, 64 to a box of x
           tc_mma_ts(tmem + kManySums, weights + k * 8, xdesc + (uint64_t)(((k >> 2) * (kManyX / 2) + (k & 3) * 32) >> 4), idesc,
                     (j | k) != 0 ? 1u : 0u);
-        tc_commit(&x_empty[x.at]);
-        tc_commit(&w_empty[w.at]);
+        tc_commit(&empty[x.at]);
         x.on();
-        w.on();
       }
       if (ok && steps > 0) tc_commit(done);
     }
   } else if (warp >= 4) {
-    const int quad = warp & 3, row = quad * 32 + lane, side = (warp - 4) >> 2;
+    const int quad = warp & 3, row = quad * 32 + lane, side = (warp - 4) >> 2 & 1, half = (warp - 4) >> 3;
     const uint32_t lane_sel = static_cast<uint32_t>(quad * 32) << 16;
     const uint2* pairs = reinterpret_cast<const uint2*>(
         p.affine + static_cast<long long>(min(tile * 128 + row, p.N - 1)) * (p.width / 16)) + step0;
@@ -622,61 +623,56 @@ linear_q4_many_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_cons
     opaque_masks(mask, magic);
     pdl_wait();
     bool ok = true;
-    uint2 f[2] = {steps > 0 ? __ldg(pairs) : make_uint2(0, 0), steps > 1 ? __ldg(pairs + 1) : make_uint2(0, 0)};
+    // a step takes a warp longer than it takes the tensor cores, mostly by waits: half of the warps have the odd steps
     Place<kManyCodeStages> c;
-    Place<kManyWeights> w;
-    for (int j0 = 0; j0 < steps && ok; j0 += 2) {
+    Place<kManySteps> w;
+    if (half) w.on();
+    uint2 pair = half < steps ? __ldg(pairs + half) : make_uint2(0, 0);
+    for (int j = half; j < steps; j += 2) {
       ok = wait_warp(&c_full[c.at], c.round, ab, ERR_WAIT_FULL);
+      if (!ok) break;
+      uint32_t r[2][16];
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const int j = j0 + half;
-        if (j >= steps || !ok) break;
-        const uint2 pair = f[half];
-        f[half] = j + 2 < steps ? __ldg(pairs + j + 2) : make_uint2(0, 0);
-        uint32_t r[2][16];
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {            // word 4 c + k: channels 64 (k & 1) + 8 (2 c + k / 2) ..
-          const uint4 v = *reinterpret_cast<const uint4*>(codes + c.at * kCodeBytes + sw128_offset(row, half * 4 + 2 * side + k));
-          const uint32_t s0 = __byte_perm(pair.x, pair.x, 0x1010), z0 = __byte_perm(pair.x, pair.x, 0x3232);
-          const uint32_t s1 = __byte_perm(pair.y, pair.y, 0x1010), z1 = __byte_perm(pair.y, pair.y, 0x3232);
-          values(v.x, s0, z0, mask, magic, &r[0][8 * k]);
-          values(v.y, s1, z1, mask, magic, &r[1][8 * k]);
-          values(v.z, s0, z0, mask, magic, &r[0][8 * k + 4]);
-          values(v.w, s1, z1, mask, magic, &r[1][8 * k + 4]);
-        }
-        ok = wait_warp(&w_empty[w.at], w.round ^ 1, ab, ERR_Q4_D);
-        if (!ok) break;
-        tc_fence_after();
-        const uint32_t to = tmem + w.at * 64 + side * 16 + lane_sel;
-        tmem_st16(to, r[0]);
-        tmem_st16(to + 32, r[1]);
-        tmem_st_wait();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) {
-          mbar_arrive(&w_full[w.at]);
-          if (half || j + 1 == steps) mbar_arrive(&c_empty[c.at]);
-        }
-        w.on();
+      for (int k = 0; k < 2; ++k) {              // word 4 c + k: channels 64 (k & 1) + 8 (2 c + k / 2) ..
+        const uint4 v = *reinterpret_cast<const uint4*>(codes + c.at * kCodeBytes + sw128_offset(row, half * 4 + 2 * side + k));
+        const uint32_t s0 = __byte_perm(pair.x, pair.x, 0x1010), z0 = __byte_perm(pair.x, pair.x, 0x3232);
+        const uint32_t s1 = __byte_perm(pair.y, pair.y, 0x1010), z1 = __byte_perm(pair.y, pair.y, 0x3232);
+        values(v.x, s0, z0, mask, magic, &r[0][8 * k]);
+        values(v.y, s1, z1, mask, magic, &r[1][8 * k]);
+        values(v.z, s0, z0, mask, magic, &r[0][8 * k + 4]);
+        values(v.w, s1, z1, mask, magic, &r[1][8 * k + 4]);
       }
+      pair = j + 2 < steps ? __ldg(pairs + j + 2) : make_uint2(0, 0);
+      ok = wait_warp(&empty[w.at], w.round ^ 1, ab, ERR_Q4_D);
+      if (!ok) break;
+      tc_fence_after();
+      const uint32_t to = tmem + w.at * 64 + side * 16 + lane_sel;
+      tmem_st16(to, r[0]);
+      tmem_st16(to + 32, r[1]);
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(&full[w.at]);
+        mbar_arrive(&c_empty[c.at]);
+      }
+      w.on2();
       c.on();
     }
-    if (steps > 0) ok = ok && wait_warp(done, 0, ab, ERR_Q4_D);
+    if (steps > 0) ok = wait_warp(done, 0, ab, ERR_Q4_D) && ok;
     tc_fence_after();
     // every product has been made, so every copy has landed and every operand has been used: the ring is free
+    const int token = (half * 2 + side) * 32;
+    uint32_t v[32];
+    if (steps > 0 && ok) {
+      tmem_ld_32x32b_x32(tmem + kManySums + token + lane_sel, v);
+      tmem_ld_wait();
+    } else {
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      uint32_t v[32];
-      if (steps > 0 && ok) {
-        tmem_ld_32x32b_x32(tmem + kManySums + side * 64 + k * 32 + lane_sel, v);
-        tmem_ld_wait();
-      } else {
-#pragma unroll
-        for (int i = 0; i < 32; ++i) v[i] = 0;
-      }
-#pragma unroll
-      for (int i = 0; i < 32; ++i) red[(side * 64 + k * 32 + i) * 128 + row] = __uint_as_float(v[i]);
+      for (int i = 0; i < 32; ++i) v[i] = 0;
     }
+#pragma unroll
+    for (int i = 0; i < 32; ++i) red[(token + i) * 128 + row] = __uint_as_float(v[i]);
   }
   __syncwarp();
   tc_fence_before();
@@ -754,8 +750,8 @@ int launch(const CUtensorMap& tmW, const CUtensorMap& tmX, const CUtensorMap& tm
 }
 
 int launch_many(const CUtensorMap& tmW, const CUtensorMap& tmX, const LinearParams& p, cudaStream_t stream) {
-  constexpr int bytes = kManyXStages * kManyX + kManyCodeStages * kCodeBytes + 1024;
-  static_assert(kManyXStages * kManyX >= kManyTokens * 128 * 4 && bytes <= 226 * 1024, "shared memory");
+  constexpr int bytes = kManySteps * kManyX + kManyCodeStages * kCodeBytes + 1024;
+  static_assert(kManySteps * kManyX >= kManyTokens * 128 * 4 && bytes <= 226 * 1024, "shared memory");
   static bool configured[b200host::kMaxDevices] = {};
   if (int rc = b200host::ensure_dynamic_smem(linear_q4_many_kernel, bytes, configured)) return rc;
   return launch_cluster(linear_q4_many_kernel, p, kManyThreads, bytes, stream, tmW, tmX, p);
@@ -764,13 +760,14 @@ int launch_many(const CUtensorMap& tmW, const CUtensorMap& tmX, const LinearPara
 }  // namespace
 
 // out [rows, N] (row stride ldo) = x [rows, K] (ldx) * W^T, W as codes [N, width / 8] words and affine [N, width / 64] pairs;
-// rows <= 64, `cluster` (1, 2, 4 or 8) slices of K.  `work` is the call's own: with R = rows rounded up to 16 (up to 16 rows) or
-// 32 and width = K rounded up to 256, 5 * R * width / 2 bytes and then R floats (none of it for up to 64 channels).
+// `cluster` (1, 2, 4 or 8) slices of K.  Up to 64 rows `work` is the call's own: with R = rows rounded up to 16 (up to 16 rows)
+// or 32 and width = K rounded up to 256, 5 * R * width / 2 bytes and then R floats (none of it for up to 64 channels).  With more
+// rows there are more than 64 channels, and rows of x start on 16 bytes.
 extern "C" int b200_q4_linear(const void* x, long long ldx, const void* codes, const void* affine, void* out,
                               long long ldo, int rows, int N, int K, int cluster, void* work, void* status,
                               void* stream) {
   using namespace b200host;
-  if (rows <= 0 || rows > 4096 || N <= 0 || K <= 0 || K > (1 << 30) || !status) return RC_BAD_SHAPE;
+  if (rows <= 0 || rows > (1 << 24) || N <= 0 || K <= 0 || K > (1 << 30) || !status) return RC_BAD_SHAPE;
   if (cluster != 1 && cluster != 2 && cluster != 4 && cluster != 8) return RC_BAD_SHAPE;
   if ((reinterpret_cast<uintptr_t>(codes) | reinterpret_cast<uintptr_t>(affine)) & 15) return RC_BAD_ALIGNMENT;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
@@ -785,6 +782,7 @@ extern "C" int b200_q4_linear(const void* x, long long ldx, const void* codes, c
   int rc;
   if ((rc = make_map_2d(&tmW, CU_TENSOR_MAP_DATA_TYPE_UINT8, codes, width / 2, N, width / 2, 128, 128))) return rc;
   if (rows > 64) {
+    if (((long long)(rows + 127) / 128) * ((N + 127) / 128) * cluster > 0x7fffffffll) return RC_BAD_SHAPE;
     if ((rc = make_map_2d(&tmX, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, x, K, rows, ldx * 2, 64, kManyTokens))) return rc;
     return launch_many(tmW, tmX, LinearParams{(const uint8_t*)affine, nullptr, (__nv_bfloat16*)out, ldo, rows, N, width, cluster,
                                               0, (rows + kManyTokens - 1) / kManyTokens, (int*)status}, s);

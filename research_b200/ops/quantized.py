@@ -29,8 +29,8 @@ from research_b200.errors import KernelError
 from research_b200.ops import native
 
 GROUP = 64
-#: Rows up to which a product reads the 4-bit weights themselves; above, they are expanded once for the GEMM.
-LINEAR_ROWS = 2048
+#: Rows of x up to which a linear multiplies the codes themselves; above, bf16 weights, expanded on their way or before.
+FEW_ROWS = 64
 
 
 class Q4Rows(NamedTuple):
@@ -414,9 +414,8 @@ def _attention_runs(B: int, Hkv: int, rows: int, device: int) -> int:
 # --------------------------------------------------------------------------------------------------
 def linear_q4(x: torch.Tensor, w: Q4Rows) -> torch.Tensor:
     """``y = x W^T`` for ``x [..., K]`` and weights ``w`` of ``N`` 4-bit rows of K channels; ``y [..., N]`` in x's type.  Up to
-    64 rows of x the weights are read as they are, and x counts to 2^-17 of its row's largest value (a row with an infinity or
-    a NaN gives NaN); for more rows the weights are expanded to bf16 once, which rounds each to 2^-8 of itself at most, and
-    go through the GEMM."""
+    64 rows of x the weights count as they are, and x to 2^-17 of its row's largest value (a row with an infinity or a NaN
+    gives NaN); for more rows x counts as it is, and each weight as a bf16."""
 
     what = "linear_q4"
     if x.dim() < 1 or not x.is_floating_point() or x.shape[-1] < 1:
@@ -437,22 +436,18 @@ def linear_q4(x: torch.Tensor, w: Q4Rows) -> torch.Tensor:
     if rows == 0 or N == 0:
         return torch.empty(*x.shape[:-1], N, dtype=x.dtype, device=x.device)
     with _on(x):
-        if rows > LINEAR_ROWS or (rows > 64 and K <= GROUP):
-            out = _expanded_linear(x2, w)
-        else:
-            out = _coded_linear(x2, w, rows, N, K)
+        slices = linear_slices(rows, N, K)
+        out = _coded_linear(x2, w, rows, N, K, slices) if slices else _expanded_linear(x2, w)
     return out if x2 is x else out.view(*x.shape[:-1], N)
 
 
-def _coded_linear(x: torch.Tensor, w: Q4Rows, rows: int, N: int, K: int) -> torch.Tensor:
+def _coded_linear(x: torch.Tensor, w: Q4Rows, rows: int, N: int, K: int, slices: int) -> torch.Tensor:
     work = None
-    if rows > 64:
-        x, slices = _rows_on_16_bytes(x), many_rows_slices(rows, N, K)
-    else:
-        slices = linear_slices(rows, N, K)
-        if K > GROUP:                                   # x as the kernel multiplies it: two e4m3 parts, a scale per row
-            tokens, width = 16 if rows <= 16 else -(-rows // 32) * 32, -(-K // 256) * 256
-            work = w.codes.new_empty(tokens * (2 * width + width // 2 + 4))
+    if rows > FEW_ROWS:
+        x = _rows_on_16_bytes(x)
+    elif K > GROUP:                                     # x as the kernel multiplies it: two e4m3 parts, a scale per row
+        tokens, width = 16 if rows <= 16 else -(-rows // 32) * 32, -(-K // 256) * 256
+        work = w.codes.new_empty(tokens * (2 * width + width // 2 + 4))
     ld, one = x.stride()
     if one != 1:
         x, ld = x.contiguous(), K
@@ -476,39 +471,44 @@ def _rows_on_16_bytes(x: torch.Tensor) -> torch.Tensor:
 
 @functools.lru_cache(maxsize=4096)
 def linear_slices(rows: int, n: int, k: int, sms: int = 148) -> int:
-    """Slices of K (1, 2, 4 or 8 blocks of a cluster) for a product with 4-bit weights: the count of least estimated time.
-    A stage of 256 channels takes a block 0.65 us (1.4 with more than 16 rows of x) by itself and an SM 0.55 (0.8) where
-    several of its up to four (two) blocks share it; slices add the exchange of partial sums.  Measured with 1 / 32 rows:
-    2048 x 2048 1 / 2 / 4 / 8 slices 10.7 / 8.5 / 6.9 / 6.3 and 15.6 / 11.0 / 8.8 / 8.5 us, 11264 x 2048 11.8 / 10.2 / 9.8 / 13.7
-    and 16.8 / 12.5 / 16.6 / 23.0 us, 28672 x 4096 31.5 / 22.5 / 26.6 / 33.6 and 30.7 / 37.0 / 45.1 / 61.2 us."""
+    """Slices of K (1, 2, 4 or 8 blocks of a cluster) for a product with 4-bit weights: the count of least estimated time, or 0
+    where that is to expand the weights first.
 
-    alone, shared, room = (0.65, 0.55, 4) if rows <= 16 else (1.4, 0.8, 2)
-    tiles, stages = -(-n // 128) * -(-rows // 32), -(-k // 256)
+    Up to 64 rows a stage of 256 channels takes a block 0.65 us (1.4 with more than 16 rows of x) by itself and an SM 0.55 (0.8)
+    where several of its up to four (two) blocks share it; slices add the exchange of partial sums.  Measured with 1 / 32
+    rows: 2048 x 2048 1 / 2 / 4 / 8 slices 10.7 / 8.5 / 6.9 / 6.3 and 15.6 / 11.0 / 8.8 / 8.5 us, 11264 x 2048 11.8 / 10.2 / 9.8 /
+    13.7 and 16.8 / 12.5 / 16.6 / 23.0 us, 28672 x 4096 31.5 / 22.5 / 26.6 / 33.6 and 30.7 / 37.0 / 45.1 / 61.2 us.
+
+    With more rows a tile of 128 x 128 has an SM for itself, for 5 us and 0.36 us per 128 channels, and clusters of 4 and 8 find
+    no room on some of the SMs.  Expanding takes 1.5 us and 0.48 us a million weights, and the GEMM then 0.4 us per 64 channels
+    of its tiles of 128 x 256.  Measured 1 / 2 / 4 / 8 slices, expanded: 128 rows, 2048 x 2048 11.1 / 8.7 / 7.5 / 16.5, 17.6 us; 65 rows,
+    4096 x 4096 16.4 / 11.0 / 9.5 / 22.6, 31.7 us; 777 rows, 2048 x 5632 22.8 / 29.8 / 44.7 / 80.6, 38.2 us; 1024 rows, 4096 x 4096
+    36.9 / 52.3 / 81.1 / 172.9, 36.2 us; 2048 rows, 2048 x 2048 23.9 / 38.7 / 66.3 / 156.5, 19.0 us."""
+
+    stages = -(-k // 256)
     best, best_cost = 1, float("inf")
-    for s, exchange in ((1, 0.0), (2, 1.1), (4, 1.6), (8, 2.2)):
-        if s > 1 and stages < s:
-            break
-        per_sm = math.ceil(tiles * s / sms - 0.1)
-        waves = -(-per_sm // room)                      # of blocks, each with 2.5 us to begin and to end
-        cost = -(-stages // s) * max(alone, (per_sm if waves == 1 else waves * room) * shared) + exchange + (waves - 1) * 2.5
-        if cost < best_cost:
-            best, best_cost = s, cost
-    return best
-
-
-@functools.lru_cache(maxsize=4096)
-def many_rows_slices(rows: int, n: int, k: int, sms: int = 148) -> int:
-    """Slices of K as above, for more than 64 rows."""
-
-    tiles, stages = -(-n // 128) * -(-rows // 128), -(-k // 256)
-    best, best_cost = 1, float("inf")
-    for s in (1, 2, 4, 8):
-        if s > 1 and stages < s:
-            break
-        cost = math.ceil(tiles * s / sms) * (-(-stages // s) * 0.6 + 3.0)
-        if cost < best_cost:
-            best, best_cost = s, cost
-    return best
+    if rows <= FEW_ROWS:
+        alone, shared, room = (0.65, 0.55, 4) if rows <= 16 else (1.4, 0.8, 2)
+        tiles = -(-n // 128) * -(-rows // 32)
+        for s, exchange in ((1, 0.0), (2, 1.1), (4, 1.6), (8, 2.2)):
+            if s > 1 and stages < s:
+                break
+            per_sm = math.ceil(tiles * s / sms - 0.1)
+            waves = -(-per_sm // room)                  # of blocks, each with 2.5 us to begin and to end
+            cost = -(-stages // s) * max(alone, (per_sm if waves == 1 else waves * room) * shared) + exchange + (waves - 1) * 2.5
+            if cost < best_cost:
+                best, best_cost = s, cost
+        return best
+    if k > GROUP:
+        tiles = -(-n // 128) * -(-rows // 128)
+        for s, exchange, blocks in ((1, 0.0, sms), (2, 0.5, sms), (4, 0.7, sms * 0.9), (8, 1.5, sms * 0.75)):
+            if s > 1 and stages < s:
+                break
+            cost = math.ceil(tiles * s / blocks) * (5.0 + 0.72 * -(-stages // s)) + 1.7 + exchange
+            if cost < best_cost:
+                best, best_cost = s, cost
+    waves = math.ceil(-(-n // 256) * -(-rows // 128) / sms)
+    return best if best_cost < 3.5 + 0.48e-6 * n * k + waves * (2.0 + 0.4 * -(-k // 64)) else 0
 
 
 def _expanded_linear(x: torch.Tensor, w: Q4Rows) -> torch.Tensor:

@@ -323,6 +323,29 @@ def test_linear_against_64_bits(rows, N, K):
     assert torch.equal(q4.linear_q4(wider[:, 3:K + 3], w), got)                     # rows on odd addresses
 
 
+@pytest.mark.parametrize("rows,N,K,slices", [(777, 512, 1100, 4), (129, 333, 705, 2), (100, 1000, 4000, 8), (65, 1000, 130, 0),
+                                             (1000, 4096, 300, 0), (70, 50, 64, 0), (300, 2600, 520, 2), (128, 9, 16000, 8), (150, 9001, 1000, 1)])
+def test_linear_of_many_rows(rows, N, K, slices):
+    """Products on tiles of 128 x 128, in each cut of K, and with the weights expanded first."""
+
+    assert q4.linear_slices(rows, N, K) == slices
+    g = _gen(rows + K)
+    x = torch.randn(rows, K, generator=g, device="cuda").to(BF16)
+    x[rows - 1] *= 1e30
+    x[0, 5], x[1, 6] = math.nan, math.inf
+    w = q4.quantize_rows_q4(torch.randn(N, K, generator=g, device="cuda") * 0.05)
+    w.affine[N - 2, 0] = math.nan
+    got = q4.linear_q4(x, w)
+    assert torch.equal(got[2:, :N - 2], q4.linear_q4(x, w)[2:, :N - 2])                 # the same bits again
+    assert got[0].isnan().all() and not got[1].isfinite().any() and got[:, N - 2].isnan().all()
+    w.affine[N - 2, 0] = 0.0
+    want, _, plain = _linear64(x[2:], w, K)
+    off = (got[2:].double() - want).abs()
+    off[:, N - 2] = 0.0
+    tol = 2.0 ** -8 * want.abs() + plain * (1.01 * 2.0 ** -8 + 2.0 ** -23 * K)
+    assert (off <= tol).all(), (off - tol).max()
+
+
 @pytest.mark.parametrize("rows", [3, 20, 50])
 def test_linear_rows_of_uneven_size(rows):
     """A channel of 2^12 times the others' size, a row of tiny values, a row of zeros, one of huge values."""
