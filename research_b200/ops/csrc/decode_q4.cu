@@ -16,10 +16,10 @@
 // p s enters the second product as two bf16 parts (up to four heads: in columns 4 .. 7 of the same product, else in a
 // second one), which holds it to 2^-14; a single bf16 would cost as much as the rounding of the result does.
 //
-// Measured (inputs larger than L2 or flushed from it): 64 sequences of 512 .. 4096 rows, 32 heads over 8 of 128, 46.6 us; of
-// 16384 rows 136.5 us, 77 % of the copy bandwidth; one sequence of 131072 rows, 23 us; of 300, 7.3 us, which are two launches
-// and one tile's latency.  With codes as 128 + n (a second operation each, and the 128 taken off again) and a maximum followed
-// tile by tile the first took 53 us.
+// Measured (inputs of several sets in turn, larger than L2), heads of 128: 64 sequences of 512 .. 4096 rows, 16 heads over 8,
+// 46.6 us, of 16384 rows 136.7 us, 77 % of the copy bandwidth; 2 sequences of 32768 rows, 32 heads over 8, 21.8 us; one of 777
+// rows 7.3 us, which are two launches and one tile's latency.  With codes as 128 + n (a second operation each, and the 128
+// taken off again) and a maximum followed tile by tile the first took 53 us.
 #include <math.h>
 #include <math_constants.h>
 
@@ -552,18 +552,17 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS) decode_q4_kernel(const __g
 
 // Joins the pieces of a head: out = sum_i w_i o_i / sum_i w_i l_i, w_i = 2^(m_i - max m); a piece that met no number has
 // m = -inf and l = NaN, which counts.  The threads of a channel share the pieces.
-constexpr int kMergeThreads = 256;
-template <int D, int TR>
-__global__ void __launch_bounds__(kMergeThreads) decode_q4_merge_kernel(const __grid_constant__ AttnParams p) {
-  constexpr int PARTS = kMergeThreads / (D / 4), WARPS = kMergeThreads / 32;
+template <int D, int TR, int THREADS>
+__global__ void __launch_bounds__(THREADS) decode_q4_merge_kernel(const __grid_constant__ AttnParams p) {
+  constexpr int PARTS = THREADS / (D / 4), WARPS = THREADS / 32;
   __shared__ long long s_sum[2][WARPS];
-  __shared__ float s_max[WARPS], s_w[kMergeThreads], s_l[WARPS];
+  __shared__ float s_max[WARPS], s_w[THREADS], s_l[WARPS];
   __shared__ __align__(16) float s_o[PARTS][D];
   const int b = blockIdx.x / p.Hq, hq = blockIdx.x - b * p.Hq, G = p.Hq / p.Hkv, h = hq / G;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   b200::pdl_launch_dependents();
   long long sum[2] = {0, 0};    // tiles of one head: of all sequences, of those before b
-  for (int i = threadIdx.x; i < p.B; i += kMergeThreads) {
+  for (int i = threadIdx.x; i < p.B; i += THREADS) {
     const int n = Span<TR>(p, i).tiles();
     sum[0] += n;
     if (i < b) sum[1] += n;
@@ -603,9 +602,9 @@ __global__ void __launch_bounds__(kMergeThreads) decode_q4_merge_kernel(const __
                                          : make_float4(0.f, 0.f, 0.f, 0.f);
   float mm = -CUDART_INF_F;
   float2 mine = make_float2(-CUDART_INF_F, 0.f);
-  for (int i = threadIdx.x; i < pieces; i += kMergeThreads) {
+  for (int i = threadIdx.x; i < pieces; i += THREADS) {
     const float2 v = ml[static_cast<long long>(i) * G];
-    if (i < kMergeThreads) mine = v;
+    if (i < THREADS) mine = v;
     mm = fmaxf(mm, v.x);
   }
 #pragma unroll
@@ -622,8 +621,8 @@ __global__ void __launch_bounds__(kMergeThreads) decode_q4_merge_kernel(const __
     acc.z = fmaf(v.z, w, acc.z);
     acc.w = fmaf(v.w, w, acc.w);
   };
-  for (int i0 = 0; i0 < pieces; i0 += kMergeThreads) {
-    const int n = min(pieces - i0, kMergeThreads);
+  for (int i0 = 0; i0 < pieces; i0 += THREADS) {
+    const int n = min(pieces - i0, THREADS);
     if (threadIdx.x < n) {
       const float2 v = i0 ? ml[static_cast<long long>(i0 + threadIdx.x) * G] : mine;
       const float w = v.x == -CUDART_INF_F ? (v.y == 0.f ? 0.f : 1.f) : b200::ex2_approx(v.x - mm);
@@ -673,8 +672,12 @@ int launch(const AttnParams& p, cudaStream_t s) {
   // fewer runs than the device has blocks: one warp of a block each, on as many SMs
   const int most = kBlocks * b200host::sm_count(), grid = p.warps < most ? p.warps : most;
   if (cudaError_t e = b200host::launch_kernel(kern, dim3(grid), dim3(kWarps * 32), bytes, s, pdl, p)) return static_cast<int>(e);
-  return static_cast<int>(b200host::launch_kernel(decode_q4_merge_kernel<D, kRows>, dim3(p.B * p.Hq), dim3(kMergeThreads), 0,
-                                                  s, pdl, p));
+  // where a head has many pieces, more threads read them at once: 64 heads in 111 pieces each, both kernels,
+  // 256 threads 23.1 us, 512 21.8, 1024 26.0; 7 pieces of 512 heads, 256 threads 46.6 us, and 512 find less room beside the
+  // first kernel
+  const bool many = p.warps > 32 * p.B * p.Hkv;
+  return static_cast<int>(b200host::launch_kernel(many ? decode_q4_merge_kernel<D, kRows, 512> : decode_q4_merge_kernel<D, kRows, 256>,
+                                                  dim3(p.B * p.Hq), dim3(many ? 512 : 256), 0, s, pdl, p));
 }
 
 }  // namespace
