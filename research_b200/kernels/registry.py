@@ -28,6 +28,9 @@ KERNEL_CANDIDATES = (
     {"op": "optimizer_matrix_update", "source": "gemm.cu", "symbol": "b200_gemm_bf16", "engine": "tcgen05 (Newton-Schulz)"},
     {"op": "decode_attention", "source": "decode.cu", "symbol": "b200_decode_attn", "engine": "SIMT split-KV"},
     {"op": "kv_cache_append", "source": "decode.cu", "symbol": "b200_kv_append", "engine": "SIMT 128-bit"},
+    {"op": "quantized_kv_cache", "source": "quant4.cu", "symbol": "b200_q4_kv_write", "engine": "SIMT 128-bit"},
+    {"op": "quantized_decode_attention", "source": "decode_q4.cu", "symbol": "b200_q4_decode_attn", "engine": "mma.sync split-KV"},
+    {"op": "quantized_linear", "source": "linear_q4.cu", "symbol": "b200_q4_linear", "engine": "tcgen05+TMA+TMEM"},
     {"op": "sampler", "source": "sampler.cu", "symbol": "b200_sample_topk", "engine": "SIMT radix select"},
     {"op": "moe_dispatch_combine", "source": "moe.cu", "symbol": "b200_moe_gather", "engine": "SIMT + NVLink peer stores/loads"},
     {"op": "moe_routing_plan", "source": "moe.cu", "symbol": "b200_moe_rank", "engine": "SIMT match_any"},
@@ -39,7 +42,8 @@ KERNEL_CANDIDATES = (
 )
 
 # ops that only some runs need (generation, multi-GPU layouts, MoE): never a reason for kernels.strict to refuse
-OPTIONAL_OPS = ("decode_attention", "kv_cache_append", "sampler", "moe_dispatch_combine", "moe_routing_plan",
+OPTIONAL_OPS = ("decode_attention", "kv_cache_append", "quantized_kv_cache", "quantized_decode_attention",
+                "quantized_linear", "sampler", "moe_dispatch_combine", "moe_routing_plan",
                 "gemm_allgather", "gemm_reduce_scatter", "grad_reduce_scatter", "weight_all_gather",
                 "grouped_expert_gemm")
 
