@@ -16,8 +16,8 @@
 // 4096 with 64 rows).  K is cut over the blocks of a cluster, which add up their partial sums in rank order: the same bits
 // every time.
 //
-// A first kernel splits x once for all blocks, while the second one, launched as its dependent, brings its first codes into
-// L2.  The second one's warps:
+// Blocks of short slices split x themselves (see own_stages); else a first kernel does once for all blocks, while the second
+// one, launched as its dependent, brings its first codes into L2.  The second one's warps:
 //   warp 0     TMA: 256 channels of codes (128 x 128 bytes) and of the split x through a ring of stages
 //   warp 1     MMA issuer: for each group the products with the high and the low parts
 //   warps 2-5  a weight row per thread: expand the next half stage's codes, then scale and add up the current one's products
@@ -40,6 +40,9 @@ constexpr int kThreads = 192;
 constexpr int kStage = 256;                    // channels of a stage
 constexpr int kCodeBytes = 128 * kStage / 2;
 constexpr int kMaxStages = 8;
+// Stages of a slice of x up to which a block splits it itself: with 1 and 16 rows of 2048 x 2048 5.7 and 6.3 us instead of 6.4 and
+// 7.0 with the kernel before (one stage), and 4 us less on the host; two stages of 32 rows take 11.2 us instead of 8.8.
+constexpr int own_stages(int tokens) { return tokens == 16 ? 2 : 1; }
 constexpr int kFours = 32, kProducts = 48;     // tensor memory: half a stage's codes (128 bytes a row), 32 fours, products
 constexpr int ERR_Q4_A = 41, ERR_Q4_D = 42;    // status codes: operands or products that never came
 
@@ -50,6 +53,9 @@ struct LinearParams {
   long long ldo;
   int rows, N, width, cluster, stages, token_tiles;
   int* status;
+  const __nv_bfloat16* x;             // where blocks split it themselves: [rows, K], `aligned` where 16 bytes may be read at once
+  long long ldx;
+  int K, aligned;
 };
 
 // D[tmem] (+)= A[tmem] * B[smem], both e4m3, fp32 accumulate; 32 channels
@@ -122,34 +128,88 @@ __device__ __forceinline__ float4 ld_cluster4(uint32_t saddr, uint32_t rank) {
 template <int NT>
 constexpr int stage_bytes() { return kCodeBytes + (2 * 2 + 1) * NT * 128; }   // codes; [half][high, low] of x; its sums
 
+// 16 channels of row r from channel c on, zeros where there are none
+__device__ __forceinline__ void load16(const __nv_bfloat16* x, long long ldx, int rows, int K, int aligned, int r, int c,
+                                       float (&f)[16]) {
+  const bool there = r < rows;
+  if (there && aligned && c + 16 <= K) {
+    const uint4* at = reinterpret_cast<const uint4*>(x + r * ldx + c);
+    float lo[8], hi[8];
+    unpack_bf16(at[0], lo);
+    unpack_bf16(at[1], hi);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) f[k] = lo[k], f[8 + k] = hi[k];
+  } else {
+#pragma unroll
+    for (int k = 0; k < 16; ++k) f[k] = there && c + k < K ? __bfloat162float(x[r * ldx + c + k]) : 0.f;
+  }
+}
+
+// What a row whose largest exponent bits are `most` is multiplied by, and what undoes it: 2^(7 - e) brings the largest to
+// [128, 256).  A row with an infinity or a NaN counts as NaN.
+__device__ __forceinline__ void row_scale(uint32_t most, float& up, float& back) {
+  const int e = max(static_cast<int>(most >> 23), 8);
+  up = e == 255 ? CUDART_NAN_F : __uint_as_float(static_cast<uint32_t>(261 - e) << 23);
+  back = e == 255 ? CUDART_NAN_F : __uint_as_float(static_cast<uint32_t>(e - 7) << 23);
+}
+
+// 16 channels as two e4m3 parts, in the order in which a word's codes fall into its low and its high nibbles: 0 4 1 5 2 6 3 7.
+__device__ __forceinline__ void split16(const float (&f)[16], uint4& high, uint4& low) {
+  uint32_t hi[4], lo[4];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    constexpr int order[8] = {0, 4, 1, 5, 2, 6, 3, 7};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float a0 = f[8 * h + order[2 * k]], a1 = f[8 * h + order[2 * k + 1]];
+      const __nv_fp8x2_storage_t u = __nv_cvt_float2_to_fp8x2(make_float2(a0, a1), __NV_SATFINITE, __NV_E4M3);
+      const __half2 back(__nv_cvt_fp8x2_to_halfraw2(u, __NV_E4M3));
+      const __nv_fp8x2_storage_t l =
+          __nv_cvt_float2_to_fp8x2(make_float2(a0 - __low2float(back), a1 - __high2float(back)), __NV_SATFINITE, __NV_E4M3);
+      if (k & 1) {
+        hi[2 * h + (k >> 1)] |= static_cast<uint32_t>(u) << 16;
+        lo[2 * h + (k >> 1)] |= static_cast<uint32_t>(l) << 16;
+      } else {
+        hi[2 * h + (k >> 1)] = u;
+        lo[2 * h + (k >> 1)] = l;
+      }
+    }
+  }
+  high = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+  low = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+}
+
+// A group's sum as 32 e4m3 numbers that add up to a quarter of it: 16 times its sixteenth, then what is left, and zeros.
+__device__ __forceinline__ void split_sum(float sum, uint4& first, uint4& second) {
+  float rest = sum * 0.25f;
+  uint32_t part[5];
+#pragma unroll
+  for (int k = 0; k < 5; ++k) {
+    const float of = k ? rest : rest * 0.0625f;
+    const __nv_fp8_storage_t v = __nv_cvt_float_to_fp8(of, __NV_SATFINITE, __NV_E4M3);
+    const float back = __half2float(__half(__nv_cvt_fp8_to_halfraw(v, __NV_E4M3)));
+    rest -= k ? back : 16.f * back;
+    part[k] = v;
+  }
+  const uint32_t all = part[0] * 0x01010101u;
+  first = make_uint4(all, all, all, all);
+  second = make_uint4(part[1] | part[2] << 8 | part[3] << 16 | part[4] << 24, 0, 0, 0);
+}
+
 // x [rows, K] -> per NT rows xq [high, low][NT][width] e4m3, behind all of them the groups' sums [rows][width / 64][32], and
-// xs [rows] fp32, rows rounded up to NT; a block per row.  Channels go into the order in which a word's codes fall into its low and its high nibbles: 0 4 1 5 2 6 3 7.
+// xs [rows] fp32, rows rounded up to NT; a block per row.
 __global__ void __launch_bounds__(512) linear_q4_split_kernel(const __nv_bfloat16* __restrict__ x, long long ldx, int rows,
                                                               int K, int width, int NT, int aligned,
                                                               uint8_t* __restrict__ xq,
                                                               float* __restrict__ xs) {
   __shared__ uint32_t s_most[16];
   const int r = blockIdx.x;
-  const bool there = r < rows;
   pdl_launch_dependents();
   pdl_wait();
-  auto load = [&](int c, float (&f)[16]) {
-    if (there && aligned && c + 16 <= K) {
-      const uint4* at = reinterpret_cast<const uint4*>(x + r * ldx + c);
-      float lo[8], hi[8];
-      unpack_bf16(at[0], lo);
-      unpack_bf16(at[1], hi);
-#pragma unroll
-      for (int k = 0; k < 8; ++k) f[k] = lo[k], f[8 + k] = hi[k];
-    } else {
-#pragma unroll
-      for (int k = 0; k < 16; ++k) f[k] = there && c + k < K ? __bfloat162float(x[r * ldx + c + k]) : 0.f;
-    }
-  };
   uint32_t most = 0;
   for (int c = threadIdx.x * 16; c < width; c += 512 * 16) {
     float f[16];
-    load(c, f);
+    load16(x, ldx, rows, K, aligned, r, c, f);
 #pragma unroll
     for (int k = 0; k < 16; ++k) most = max(most, __float_as_uint(f[k]) & 0x7f800000u);
   }
@@ -158,60 +218,32 @@ __global__ void __launch_bounds__(512) linear_q4_split_kernel(const __nv_bfloat1
   __syncthreads();
 #pragma unroll
   for (int w = 0; w < 16; ++w) most = max(most, s_most[w]);
-  // times 2^(7 - e): the largest is in [128, 256).  A row with an infinity or a NaN counts as NaN.
-  const int e = max(static_cast<int>(most >> 23), 8);
-  const float up = e == 255 ? CUDART_NAN_F : __uint_as_float(static_cast<uint32_t>(261 - e) << 23);
-  if (threadIdx.x == 0) xs[r] = e == 255 ? CUDART_NAN_F : __uint_as_float(static_cast<uint32_t>(e - 7) << 23);
+  float up, back;
+  row_scale(most, up, back);
+  if (threadIdx.x == 0) xs[r] = back;
   for (int c0 = 0; c0 < width; c0 += 512 * 16) {
     const int c = c0 + threadIdx.x * 16;       // four threads have a group; beyond the row they have zeros
     float f[16], sum = 0.f;
-    load(c, f);
-    uint32_t hi[4], lo[4];
+    load16(x, ldx, rows, K, aligned, r, c, f);
 #pragma unroll
     for (int k = 0; k < 16; ++k) {
       f[k] *= up;
       sum += f[k];
     }
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      constexpr int order[8] = {0, 4, 1, 5, 2, 6, 3, 7};
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const float a0 = f[8 * h + order[2 * k]], a1 = f[8 * h + order[2 * k + 1]];
-        const __nv_fp8x2_storage_t u = __nv_cvt_float2_to_fp8x2(make_float2(a0, a1), __NV_SATFINITE, __NV_E4M3);
-        const __half2 back(__nv_cvt_fp8x2_to_halfraw2(u, __NV_E4M3));
-        const __nv_fp8x2_storage_t l =
-            __nv_cvt_float2_to_fp8x2(make_float2(a0 - __low2float(back), a1 - __high2float(back)), __NV_SATFINITE, __NV_E4M3);
-        if (k & 1) {
-          hi[2 * h + (k >> 1)] |= static_cast<uint32_t>(u) << 16;
-          lo[2 * h + (k >> 1)] |= static_cast<uint32_t>(l) << 16;
-        } else {
-          hi[2 * h + (k >> 1)] = u;
-          lo[2 * h + (k >> 1)] = l;
-        }
-      }
-    }
     sum += __shfl_xor_sync(0xffffffffu, sum, 1);
     sum += __shfl_xor_sync(0xffffffffu, sum, 2);
     if (c >= width) continue;                  // no shuffles below
+    uint4 high, low;
+    split16(f, high, low);
     uint8_t* to = xq + (static_cast<long long>(r / NT) * 2 * NT + r % NT) * width + c;
-    *reinterpret_cast<uint4*>(to) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-    *reinterpret_cast<uint4*>(to + static_cast<long long>(NT) * width) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+    *reinterpret_cast<uint4*>(to) = high;
+    *reinterpret_cast<uint4*>(to + static_cast<long long>(NT) * width) = low;
     if ((threadIdx.x & 3) == 0) {
-      float rest = sum * 0.25f;
-      uint32_t part[5];
-#pragma unroll
-      for (int k = 0; k < 5; ++k) {
-        const float of = k ? rest : rest * 0.0625f;
-        const __nv_fp8_storage_t v = __nv_cvt_float_to_fp8(of, __NV_SATFINITE, __NV_E4M3);
-        const float back = __half2float(__half(__nv_cvt_fp8_to_halfraw(v, __NV_E4M3)));
-        rest -= k ? back : 16.f * back;
-        part[k] = v;
-      }
-      const uint32_t all = part[0] * 0x01010101u;
+      uint4 first, second;
+      split_sum(sum, first, second);
       uint8_t* at = xq + 2ll * gridDim.x * width + (static_cast<long long>(r) * width + c) / 2;
-      *reinterpret_cast<uint4*>(at) = make_uint4(all, all, all, all);
-      *reinterpret_cast<uint4*>(at + 16) = make_uint4(part[1] | part[2] << 8 | part[3] << 16 | part[4] << 24, 0, 0, 0);
+      *reinterpret_cast<uint4*>(at) = first;
+      *reinterpret_cast<uint4*>(at + 16) = second;
     }
   }
 }
@@ -263,7 +295,9 @@ __device__ __forceinline__ void finish(float* red, const LinearParams& p, int ti
 template <int NT>
 constexpr int blocks_per_sm() { return NT == 16 ? 4 : 2; }
 
-template <int NT>
+// SPLIT: x comes split from the kernel before.  Else the block's slice has no more stages than there are slots, and its workers
+// split x themselves, with scales of the slice's own: a launch less.
+template <int NT, bool SPLIT>
 __global__ void __launch_bounds__(kThreads, blocks_per_sm<NT>())
 linear_q4_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX,
                  const __grid_constant__ CUtensorMap tmS, const __grid_constant__ LinearParams p) {
@@ -276,6 +310,7 @@ linear_q4_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant_
   __shared__ uint64_t full[kMaxStages], empty[kMaxStages], go[1], done[1];
   __shared__ uint32_t tmem_slot[1];
   __shared__ int abort_word;
+  __shared__ float s_back[NT];                 // what undoes a token's scale, where it is the block's own
   pdl_launch_dependents();
   volatile int* abort_flag = &abort_word;
   const AbortCtx ab{abort_flag, p.status};
@@ -308,7 +343,7 @@ linear_q4_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant_
   if (warp == 0) {
     if (elect_one()) {
       tma_prefetch_desc(&tmW);
-      tma_prefetch_desc(&tmX);
+      if (SPLIT) tma_prefetch_desc(&tmX);
       // what runs before may be what writes the weights: they are read after the wait, and only brought into L2 ahead of it
       for (int i = 0; i < min(n_kb, 4); ++i) tma_prefetch_l2_2d(&tmW, (kb0 + i) * (kStage / 2), tile * 128);
       pdl_wait();
@@ -316,8 +351,12 @@ linear_q4_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant_
       for (int i = 0, s = 0, ph = 1; i < n_kb; ++i) {
         if (!wait(&empty[s], ph, ab, ERR_WAIT_EMPTY)) { ok = false; break; }
         uint8_t* to = smem + s * STAGE;
-        mbar_expect_tx(&full[s], STAGE);
+        mbar_expect_tx(&full[s], SPLIT ? STAGE : kCodeBytes);
         tma_load_2d(to, &tmW, &full[s], (kb0 + i) * (kStage / 2), tile * 128);
+        if constexpr (!SPLIT) {
+          if (++s == p.stages) s = 0, ph ^= 1;
+          continue;
+        }
         tma_load_2d(to + kCodeBytes, &tmX, &full[s], (kb0 + i) * kStage, tokens0 * 2 * NT);
         tma_load_2d(to + kCodeBytes + 2 * NT * 128, &tmX, &full[s], (kb0 + i) * kStage + 128, tokens0 * 2 * NT);
         tma_load_2d(to + kCodeBytes + 4 * NT * 128, &tmS, &full[s], (kb0 + i) * (kStage / 2), tokens0 * NT);
@@ -400,6 +439,52 @@ linear_q4_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant_
       tmem_st16(tmem + kFours + lane_sel, fours);
     }
     pdl_wait();
+    if constexpr (!SPLIT) {
+      // PER threads for a token, of which thread q has every PER-th chunk of 16 channels: four neighbours have a group
+      constexpr int PER = 128 / NT, MOST = own_stages(NT) * 16 / PER;
+      const int t = threadIdx.x - 64, token = t / PER, q = t % PER;
+      float x[MOST][16];
+      uint32_t most = 0;
+#pragma unroll
+      for (int it = 0; it < MOST; ++it) {
+        const int c = it * PER + q;
+        if (it * PER >= n_kb * 16) break;        // a stage less
+        load16(p.x, p.ldx, p.rows, p.K, p.aligned, tokens0 * NT + token, kb0 * kStage + c * 16, x[it]);
+#pragma unroll
+        for (int k = 0; k < 16; ++k) most = max(most, __float_as_uint(x[it][k]) & 0x7f800000u);
+      }
+#pragma unroll
+      for (int off = 1; off < PER; off <<= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, off));
+      float up, back;
+      row_scale(most, up, back);
+      if (q == 0) s_back[token] = back;
+#pragma unroll
+      for (int it = 0; it < MOST; ++it) {
+        const int c = it * PER + q, half = c >> 3 & 1;
+        if (it * PER >= n_kb * 16) break;
+        float sum = 0.f;
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+          x[it][k] *= up;
+          sum += x[it][k];
+        }
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+        uint8_t* to = smem + (c >> 4) * STAGE + kCodeBytes;
+        uint4 high, low;
+        split16(x[it], high, low);
+        *reinterpret_cast<uint4*>(to + half * 2 * NT * 128 + sw128_offset(token, c & 7)) = high;
+        *reinterpret_cast<uint4*>(to + half * 2 * NT * 128 + sw128_offset(NT + token, c & 7)) = low;
+        if ((q & 3) == 0) {
+          uint4 first, second;
+          split_sum(sum, first, second);
+          *reinterpret_cast<uint4*>(to + 4 * NT * 128 + sw128_offset(token, (c >> 2 & 3) * 2)) = first;
+          *reinterpret_cast<uint4*>(to + 4 * NT * 128 + sw128_offset(token, (c >> 2 & 3) * 2 + 1)) = second;
+        }
+      }
+      fence_proxy_async_smem();                  // the first hand-over lets the issuer read it
+      asm volatile("bar.sync 1, 128;" ::: "memory");   // and s_back the workers
+    }
     uint2 f[2] = {0 < n_pairs ? __ldg(pairs) : make_uint2(0, 0), 1 < n_pairs ? __ldg(pairs + 1) : make_uint2(0, 0)};
     bool ok = true;
     if (n_kb > 0) {
@@ -468,8 +553,8 @@ linear_q4_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant_
     for (int c = 0; c < NT; c += 2) {
       float u, v;
       f2_unpack(y[c / 2], u, v);
-      red[c * 128 + row] = u;
-      red[(c + 1) * 128 + row] = v;
+      red[c * 128 + row] = SPLIT ? u : u * s_back[c];
+      red[(c + 1) * 128 + row] = SPLIT ? v : v * s_back[c + 1];
     }
   }
   __syncwarp();
@@ -735,7 +820,7 @@ int launch_cluster(void (*kern)(Args...), const LinearParams& p, int threads, in
   return static_cast<int>(cudaLaunchKernelEx(&cfg, kern, args...));
 }
 
-template <int NT>
+template <int NT, bool SPLIT>
 int launch(const CUtensorMap& tmW, const CUtensorMap& tmX, const CUtensorMap& tmS, LinearParams p, cudaStream_t stream) {
   const int blocks = (p.width + kStage - 1) / kStage, slice = (blocks + p.cluster - 1) / p.cluster;
   p.stages = (222 * 1024 / blocks_per_sm<NT>() - 2048) / stage_bytes<NT>();
@@ -745,8 +830,9 @@ int launch(const CUtensorMap& tmW, const CUtensorMap& tmX, const CUtensorMap& tm
   const int ring = p.stages * stage_bytes<NT>(), sums = NT * 128 * 4;   // the partial sums reuse the ring
   const int smem_bytes = (ring > sums ? ring : sums) + 1024;
   static bool configured[b200host::kMaxDevices] = {};
-  if (int rc = b200host::ensure_dynamic_smem(linear_q4_kernel<NT>, 200 * 1024, configured)) return rc;
-  return launch_cluster(linear_q4_kernel<NT>, p, kThreads, smem_bytes, stream, tmW, tmX, tmS, p);
+  static_assert((222 * 1024 / blocks_per_sm<NT>() - 2048) / stage_bytes<NT>() >= own_stages(NT), "slots");
+  if (int rc = b200host::ensure_dynamic_smem(linear_q4_kernel<NT, SPLIT>, 200 * 1024, configured)) return rc;
+  return launch_cluster(linear_q4_kernel<NT, SPLIT>, p, kThreads, smem_bytes, stream, tmW, tmX, tmS, p);
 }
 
 int launch_many(const CUtensorMap& tmW, const CUtensorMap& tmX, const LinearParams& p, cudaStream_t stream) {
@@ -760,9 +846,9 @@ int launch_many(const CUtensorMap& tmW, const CUtensorMap& tmX, const LinearPara
 }  // namespace
 
 // out [rows, N] (row stride ldo) = x [rows, K] (ldx) * W^T, W as codes [N, width / 8] words and affine [N, width / 64] pairs;
-// `cluster` (1, 2, 4 or 8) slices of K.  Up to 64 rows `work` is the call's own: with R = rows rounded up to 16 (up to 16 rows)
-// or 32 and width = K rounded up to 256, 5 * R * width / 2 bytes and then R floats (none of it for up to 64 channels).  With more
-// rows there are more than 64 channels, and rows of x start on 16 bytes.
+// `cluster` (1, 2, 4 or 8) slices of K.  `work` is the call's own: with R = rows rounded up to 16 (up to 16 rows) or
+// 32 and width = K rounded up to 256, 5 * R * width / 2 bytes and then R floats; none with more than 64 rows, and none where a
+// slice has up to 512 (256) channels.  With more than 64 rows there are more than 64 channels, and rows of x start on 16 bytes.
 extern "C" int b200_q4_linear(const void* x, long long ldx, const void* codes, const void* affine, void* out,
                               long long ldo, int rows, int N, int K, int cluster, void* work, void* status,
                               void* stream) {
@@ -787,19 +873,22 @@ extern "C" int b200_q4_linear(const void* x, long long ldx, const void* codes, c
     return launch_many(tmW, tmX, LinearParams{(const uint8_t*)affine, nullptr, (__nv_bfloat16*)out, ldo, rows, N, width, cluster,
                                               0, (rows + kManyTokens - 1) / kManyTokens, (int*)status}, s);
   }
-  if (!work || (reinterpret_cast<uintptr_t>(work) & 15)) return RC_BAD_ALIGNMENT;
   const int NT = rows <= 16 ? 16 : 32, tiles = (rows + NT - 1) / NT, tokens = NT * tiles;
+  const int aligned = ldx % 8 == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0;
   const int xwidth = (K + kStage - 1) / kStage * kStage;
+  LinearParams p{(const uint8_t*)affine, nullptr, (__nv_bfloat16*)out, ldo, rows, N, width, cluster, 0, tiles,
+                 (int*)status, (const __nv_bfloat16*)x, ldx, K, aligned};
+  if ((xwidth / kStage + cluster - 1) / cluster <= own_stages(NT))
+    return NT == 16 ? launch<16, false>(tmW, tmW, tmW, p, s) : launch<32, false>(tmW, tmW, tmW, p, s);
+  if (!work || (reinterpret_cast<uintptr_t>(work) & 15)) return RC_BAD_ALIGNMENT;
   uint8_t* xq = static_cast<uint8_t*>(work);
   uint8_t* sums = xq + 2ll * tokens * xwidth;
   float* xs = reinterpret_cast<float*>(sums + tokens * (xwidth / 2ll));
   if ((rc = make_map_2d(&tmX, CU_TENSOR_MAP_DATA_TYPE_UINT8, xq, xwidth, 2 * tokens, xwidth, 128, 2 * NT))) return rc;
   if ((rc = make_map_2d(&tmS, CU_TENSOR_MAP_DATA_TYPE_UINT8, sums, xwidth / 2, tokens, xwidth / 2, 128, NT))) return rc;
-  const int aligned = ldx % 8 == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0;
   if (cudaError_t e = launch_kernel(linear_q4_split_kernel, dim3(tokens), dim3(512), 0, s, pdl, (const __nv_bfloat16*)x, ldx,
                                     rows, K, xwidth, NT, aligned, xq, xs))
     return static_cast<int>(e);
-  LinearParams p{(const uint8_t*)affine, xs, (__nv_bfloat16*)out, ldo, rows, N, width, cluster, 0, tiles,
-                 (int*)status};
-  return NT == 16 ? launch<16>(tmW, tmX, tmS, p, s) : launch<32>(tmW, tmX, tmS, p, s);
+  p.xs = xs;
+  return NT == 16 ? launch<16, true>(tmW, tmX, tmS, p, s) : launch<32, true>(tmW, tmX, tmS, p, s);
 }

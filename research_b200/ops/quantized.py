@@ -445,7 +445,7 @@ def _coded_linear(x: torch.Tensor, w: Q4Rows, rows: int, N: int, K: int, slices:
     work = None
     if rows > FEW_ROWS:
         x = _rows_on_16_bytes(x)
-    elif K > GROUP:                                     # x as the kernel multiplies it: two e4m3 parts, a scale per row
+    elif K > (512 if rows <= 16 else 256) * slices:     # x as the kernel multiplies it, for slices that blocks do not split
         tokens, width = 16 if rows <= 16 else -(-rows // 32) * 32, -(-K // 256) * 256
         work = w.codes.new_empty(tokens * (2 * width + width // 2 + 4))
     ld, one = x.stride()
@@ -475,9 +475,10 @@ def linear_slices(rows: int, n: int, k: int, sms: int = 148) -> int:
     where that is to expand the weights first.
 
     Up to 64 rows a stage of 256 channels takes a block 0.65 us (1.4 with more than 16 rows of x) by itself and an SM 0.55 (0.8)
-    where several of its up to four (two) blocks share it; slices add the exchange of partial sums.  Measured with 1 / 32
-    rows: 2048 x 2048 1 / 2 / 4 / 8 slices 10.7 / 8.5 / 6.9 / 6.3 and 15.6 / 11.0 / 8.8 / 8.5 us, 11264 x 2048 11.8 / 10.2 / 9.8 /
-    13.7 and 16.8 / 12.5 / 16.6 / 23.0 us, 28672 x 4096 31.5 / 22.5 / 26.6 / 33.6 and 30.7 / 37.0 / 45.1 / 61.2 us.
+    where several of its up to four (two) blocks share it; slices add the exchange of partial sums.  Where a block splits its
+    slice of x itself, that is most of its time.  Measured with 1 / 32 rows, 1 / 2 / 4 / 8 slices: 2048 x 2048 10.7 / 8.3 / 7.4 / 5.7
+    and 15.6 / 10.9 / 8.8 / 8.6 us, 4096 x 2048 10.8 / 8.7 / 8.0 / 6.5 us (1 row), 11264 x 2048 11.8 / 9.8 / 10.8 / 13.9 and 16.9 / 12.6 /
+    16.6 / 23.0 us, 28672 x 4096 31.7 / 22.5 / 26.7 / 43.4 and 31.0 / 37.5 / 45.6 / 90.7 us.
 
     With more rows a tile of 128 x 128 has an SM for itself, for 5 us and 0.36 us per 128 channels, and clusters of 4 and 8 find
     no room on some of the SMs.  Expanding takes 1.5 us and 0.48 us a million weights, and the GEMM then 0.4 us per 64 channels
@@ -488,14 +489,20 @@ def linear_slices(rows: int, n: int, k: int, sms: int = 148) -> int:
     stages = -(-k // 256)
     best, best_cost = 1, float("inf")
     if rows <= FEW_ROWS:
-        alone, shared, room = (0.65, 0.55, 4) if rows <= 16 else (1.4, 0.8, 2)
+        few = rows <= 16
+        base, alone, shared, room = (5.5, 0.65, 0.55, 4) if few else (4.4, 1.4, 0.8, 2)
+        own, own_base, own_stage, own_shared = (2, 4.1, 1.6, 0.6) if few else (1, 5.9, 2.7, 0.45)
         tiles = -(-n // 128) * -(-rows // 32)
         for s, exchange in ((1, 0.0), (2, 1.1), (4, 1.6), (8, 2.2)):
             if s > 1 and stages < s:
                 break
-            per_sm = math.ceil(tiles * s / sms - 0.1)
+            per, per_sm = -(-stages // s), math.ceil(tiles * s / sms - 0.1)
             waves = -(-per_sm // room)                  # of blocks, each with 2.5 us to begin and to end
-            cost = -(-stages // s) * max(alone, (per_sm if waves == 1 else waves * room) * shared) + exchange + (waves - 1) * 2.5
+            if per <= own:
+                cost = own_base + waves * per * own_stage * (1 + own_shared * (max(min(per_sm, room), 1) - 1))
+            else:
+                cost = base + per * max(alone, (per_sm if waves == 1 else waves * room) * shared) + exchange
+            cost += (max(waves, 1) - 1) * 2.5
             if cost < best_cost:
                 best, best_cost = s, cost
         return best
