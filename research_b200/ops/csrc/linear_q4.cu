@@ -1,9 +1,12 @@
-// y = x W^T with weights held in 4 bits (quant4.cuh): x [rows, K] bf16, W [N, K], y [rows, N] bf16 with fp32 sums.  For more
-// than 64 rows of x see linear_q4_many_kernel; what follows is up to 64.  The time is that of streaming the codes once (0.56 bytes a weight), as long as expanding them keeps up: at the
-// copy bandwidth an SM gets 46 codes a clock, which is what the arrangement below is for.
+// y = x W^T with weights held in 4 bits (quant4.cuh): x [rows, K] bf16, W [N, K], y [rows, N] bf16 with fp32 sums.  Up to 16
+// rows of x the codes themselves are multiplied, as follows; for more see linear_q4_many_kernel.  (With 16 rows of 28672 x 4096 /
+// 2048 x 2048 this one takes 23.7 / 6.3 us, with 17 that one 27.1 / 5.7; this one rounds no weight.)
 //
-// The weights are the 128-row operand of tcgen05.mma, from tensor memory, the rows of x its columns (16 or 32 at a time), both in
-// e4m3.  The bytes 0 .. 15 are, as e4m3, the numbers n 2^-9 (subnormals and the first binade are one straight line), so that a
+// The time is that of streaming the codes once (0.56 bytes a weight), as long as expanding them keeps up: at the copy
+// bandwidth an SM gets 46 codes a clock, which is what the arrangement below is for.  Measured, 1 row: 2048 x 2048 5.6 us, a
+// stage's latency; 28672 x 4096 22.4 us, 0.45 of the copy bandwidth, 0.55 us per stage of 256 channels and SM.
+//
+// The weights are the 128-row operand of tcgen05.mma, from tensor memory, the rows of x its 16 columns, both in e4m3.  The bytes 0 .. 15 are, as e4m3, the numbers n 2^-9 (subnormals and the first binade are one straight line), so that a
 // word of eight codes becomes eight operands by two masks and a shift, a third of what bf16 operands take, in half the tensor
 // memory.  A row of x is brought to [128, 256) by a power of two and split into two e4m3 numbers, high + low, which go into
 // one accumulator: the eight bits of a bf16 are two times four, so that is exact down to 2^-9 of the row's largest value, and
@@ -16,7 +19,7 @@
 // 4096 with 64 rows).  K is cut over the blocks of a cluster, which add up their partial sums in rank order: the same bits
 // every time.
 //
-// Blocks of short slices split x themselves (see own_stages); else a first kernel does once for all blocks, while the second
+// Blocks of short slices split x themselves (see kOwnStages); else a first kernel does once for all blocks, while the second
 // one, launched as its dependent, brings its first codes into L2.  The second one's warps:
 //   warp 0     TMA: 256 channels of codes (128 x 128 bytes) and of the split x through a ring of stages
 //   warp 1     MMA issuer: for each group the products with the high and the low parts
@@ -40,9 +43,10 @@ constexpr int kThreads = 192;
 constexpr int kStage = 256;                    // channels of a stage
 constexpr int kCodeBytes = 128 * kStage / 2;
 constexpr int kMaxStages = 8;
-// Stages of a slice of x up to which a block splits it itself: with 1 and 16 rows of 2048 x 2048 5.7 and 6.3 us instead of 6.4 and
-// 7.0 with the kernel before (one stage), and 4 us less on the host; two stages of 32 rows take 11.2 us instead of 8.8.
-constexpr int own_stages(int tokens) { return tokens == 16 ? 2 : 1; }
+constexpr int kFewRows = 16;                   // up to which the codes themselves are multiplied
+// Stages of a slice of x up to which a block splits it itself: with 1 and 16 rows of 2048 x 2048 (one stage) 5.7 and 6.3 us
+// instead of 6.4 and 7.0 with the kernel before, and 4 us less on the host.
+constexpr int kOwnStages = 2;
 constexpr int kFours = 32, kProducts = 48;     // tensor memory: half a stage's codes (128 bytes a row), 32 fours, products
 constexpr int ERR_Q4_A = 41, ERR_Q4_D = 42;    // status codes: operands or products that never came
 
@@ -125,8 +129,7 @@ __device__ __forceinline__ float4 ld_cluster4(uint32_t saddr, uint32_t rank) {
   return v;
 }
 
-template <int NT>
-constexpr int stage_bytes() { return kCodeBytes + (2 * 2 + 1) * NT * 128; }   // codes; [half][high, low] of x; its sums
+constexpr int kStageBytes = kCodeBytes + (2 * 2 + 1) * kFewRows * 128;   // codes; [half][high, low] of x; its sums
 
 // 16 channels of row r from channel c on, zeros where there are none
 __device__ __forceinline__ void load16(const __nv_bfloat16* x, long long ldx, int rows, int K, int aligned, int r, int c,
@@ -196,10 +199,10 @@ __device__ __forceinline__ void split_sum(float sum, uint4& first, uint4& second
   second = make_uint4(part[1] | part[2] << 8 | part[3] << 16 | part[4] << 24, 0, 0, 0);
 }
 
-// x [rows, K] -> per NT rows xq [high, low][NT][width] e4m3, behind all of them the groups' sums [rows][width / 64][32], and
-// xs [rows] fp32, rows rounded up to NT; a block per row.
+// x [rows, K] -> xq [high, low][kFewRows][width] e4m3, behind them the groups' sums [kFewRows][width / 64][32], and xs [kFewRows]
+// fp32; a block per row.
 __global__ void __launch_bounds__(512) linear_q4_split_kernel(const __nv_bfloat16* __restrict__ x, long long ldx, int rows,
-                                                              int K, int width, int NT, int aligned,
+                                                              int K, int width, int aligned,
                                                               uint8_t* __restrict__ xq,
                                                               float* __restrict__ xs) {
   __shared__ uint32_t s_most[16];
@@ -235,13 +238,13 @@ __global__ void __launch_bounds__(512) linear_q4_split_kernel(const __nv_bfloat1
     if (c >= width) continue;                  // no shuffles below
     uint4 high, low;
     split16(f, high, low);
-    uint8_t* to = xq + (static_cast<long long>(r / NT) * 2 * NT + r % NT) * width + c;
+    uint8_t* to = xq + static_cast<long long>(r) * width + c;
     *reinterpret_cast<uint4*>(to) = high;
-    *reinterpret_cast<uint4*>(to + static_cast<long long>(NT) * width) = low;
+    *reinterpret_cast<uint4*>(to + static_cast<long long>(kFewRows) * width) = low;
     if ((threadIdx.x & 3) == 0) {
       uint4 first, second;
       split_sum(sum, first, second);
-      uint8_t* at = xq + 2ll * gridDim.x * width + (static_cast<long long>(r) * width + c) / 2;
+      uint8_t* at = xq + 2ll * kFewRows * width + (static_cast<long long>(r) * width + c) / 2;
       *reinterpret_cast<uint4*>(at) = first;
       *reinterpret_cast<uint4*>(at + 16) = second;
     }
@@ -291,20 +294,18 @@ __device__ __forceinline__ void finish(float* red, const LinearParams& p, int ti
   }
 }
 
-// blocks an SM: by tensor memory (128 columns with 16 rows of x, else 256) and shared memory
-template <int NT>
-constexpr int blocks_per_sm() { return NT == 16 ? 4 : 2; }
+constexpr int kFewBlocks = 4;                  // an SM, by tensor memory (128 columns each) and shared memory
 
 // SPLIT: x comes split from the kernel before.  Else the block's slice has no more stages than there are slots, and its workers
 // split x themselves, with scales of the slice's own: a launch less.
-template <int NT, bool SPLIT>
-__global__ void __launch_bounds__(kThreads, blocks_per_sm<NT>())
+template <bool SPLIT>
+__global__ void __launch_bounds__(kThreads, kFewBlocks)
 linear_q4_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX,
                  const __grid_constant__ CUtensorMap tmS, const __grid_constant__ LinearParams p) {
-  constexpr int STAGE = stage_bytes<NT>();
-  constexpr int UNIT = NT == 16 ? 2 : 1;       // groups whose products are there at a time: NT columns, and NT of the ones'
-  constexpr int TMEM_COLUMNS = kProducts + UNIT * 2 * NT <= 128 ? 128 : 256;
-  static_assert(kProducts + UNIT * 2 * NT <= 256 && TMEM_COLUMNS * blocks_per_sm<NT>() <= 512, "tensor memory");
+  constexpr int NT = kFewRows, STAGE = kStageBytes;
+  constexpr int UNIT = 2;                      // groups whose products are there at a time: NT columns, and NT of the fours'
+  constexpr int TMEM_COLUMNS = 128;
+  static_assert(kProducts + UNIT * 2 * NT <= TMEM_COLUMNS && TMEM_COLUMNS * kFewBlocks <= 512, "tensor memory");
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   __shared__ uint64_t full[kMaxStages], empty[kMaxStages], go[1], done[1];
@@ -441,7 +442,7 @@ linear_q4_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant_
     pdl_wait();
     if constexpr (!SPLIT) {
       // PER threads for a token, of which thread q has every PER-th chunk of 16 channels: four neighbours have a group
-      constexpr int PER = 128 / NT, MOST = own_stages(NT) * 16 / PER;
+      constexpr int PER = 128 / NT, MOST = kOwnStages * 16 / PER;
       const int t = threadIdx.x - 64, token = t / PER, q = t % PER;
       float x[MOST][16];
       uint32_t most = 0;
@@ -571,19 +572,30 @@ linear_q4_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant_
   finish<NT>(red, p, tile, tokens0, rank, kThreads);
 }
 
-// More than 64 rows of x: y = x W^T in bf16, tiles of 128 weight rows and 128 tokens, one block an SM, the weights expanded into
-// tensor memory on their way.  The products of 128 x 128 x 128 take the tensor cores 512 clocks, expanding the codes for them
+// More than 16 rows of x: y = x W^T in bf16, tiles of 128 weight rows and 64 or 128 tokens, the weights expanded into tensor
+// memory on their way.  The products of 128 x 128 x 128 take the tensor cores 512 clocks, expanding the codes for them
 // takes each scheduler about 300 issue slots (a mask and a shift, 128 + n - 128, n s + z for two channels, rounded once), so that
 // a matrix of bf16 weights need be neither written nor read.  (Taking the groups' products by themselves, as above, would
 // need an FMA and a read of tensor memory for each of them and each group: 46 us for 777 rows of 5632 x 2048 channels.)
+// Measured: 777 rows of 5632 x 2048 channels (112 tiles) 22.9 us, 0.46 of the measured bf16 rate, 32 rows of 11264 x 2048 9.7 us,
+// 64 rows of 28672 x 4096 28.6 us.
 //   warp 0      TMA: codes of 256 channels, x of 128 channels, in the order of use
 //   warp 1      MMA issuer: one wait and one commit a step (each takes the thread a good 100 clocks in which it issues nothing:
 //               with barriers of their own for weights and x, 777 rows of 5632 x 2048 channels took 28.0 us instead of 23.1)
-//   warps 4-19  four for a quadrant's 32 weight rows: each expands half of every second step's channels
-constexpr int kManyTokens = 128, kManyThreads = 640;
-constexpr int kManyX = 2 * kManyTokens * 128, kManyCodeStages = 5;
-constexpr int kManySteps = 4;         // steps whose operands are there at a time, with one barrier for both operands
-constexpr int kManySums = kManySteps * 64;   // tensor memory: 4 x 64 columns of weights, 128 of sums
+//   warps 4-    for a quadrant's 32 weight rows: half of them has every second step's channels (each expanded by two warps where
+//               the block has the SM for itself)
+template <int NT, int BLOCKS>
+struct Many {                                                    // BLOCKS an SM
+  static constexpr int SIDES = BLOCKS == 1 ? 2 : 1;              // warps for a quadrant's step
+  static constexpr int THREADS = 128 + 256 * SIDES;
+  static constexpr int X = 2 * NT * 128;                         // bytes of a step's x
+  static constexpr int STEPS = BLOCKS == 1 ? 4 : 3;              // whose operands are there at a time, one barrier for both
+  static constexpr int CODE_STAGES = BLOCKS == 1 ? 5 : 3;
+  static constexpr int SUMS = STEPS * 64, COLUMNS = SUMS + NT <= 256 ? 256 : 512;   // tensor memory: weights, sums
+  static constexpr int BYTES = STEPS * X + CODE_STAGES * kCodeBytes + 1024;
+  static_assert(BYTES - 1024 >= NT * 128 * 4 && BLOCKS * (BYTES + 1280) <= 228 * 1024 && BLOCKS * COLUMNS <= 512 &&
+                NT <= 64 * SIDES, "an SM's room");
+};
 
 // Place in a ring of N, and the parity of its round.
 template <int N>
@@ -611,14 +623,15 @@ __device__ __forceinline__ void values(uint32_t word, uint32_t s2, uint32_t z2, 
   }
 }
 
-__global__ void __launch_bounds__(kManyThreads, 1)
+template <int NT, int BLOCKS>
+__global__ void __launch_bounds__(Many<NT, BLOCKS>::THREADS, BLOCKS)
 linear_q4_many_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX,
                       const __grid_constant__ LinearParams p) {
-  constexpr int NT = kManyTokens;
+  using M = Many<NT, BLOCKS>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* codes = smem + kManySteps * kManyX;
-  __shared__ uint64_t full[kManySteps], empty[kManySteps], c_full[kManyCodeStages], c_empty[kManyCodeStages], done[1];
+  uint8_t* codes = smem + M::STEPS * M::X;
+  __shared__ uint64_t full[M::STEPS], empty[M::STEPS], c_full[M::CODE_STAGES], c_empty[M::CODE_STAGES], done[1];
   __shared__ uint32_t tmem_slot[1];
   __shared__ int abort_word;
   pdl_launch_dependents();
@@ -632,14 +645,14 @@ linear_q4_many_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_cons
   const int steps = max(min(2 * per, p.width / 128 - step0), 0);
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < kManySteps; ++s) mbar_init(&full[s], 8 + 1), mbar_init(&empty[s], 1);   // expanders' warps, x
-    for (int s = 0; s < kManyCodeStages; ++s) mbar_init(&c_full[s], 1), mbar_init(&c_empty[s], 16);
+    for (int s = 0; s < M::STEPS; ++s) mbar_init(&full[s], 4 * M::SIDES + 1), mbar_init(&empty[s], 1);   // expanders' warps, x
+    for (int s = 0; s < M::CODE_STAGES; ++s) mbar_init(&c_full[s], 1), mbar_init(&c_empty[s], 8 * M::SIDES);
     mbar_init(done, 1);
     *abort_flag = 0;
     mbar_fence_init();
   }
   if (warp == 1) {
-    tmem_alloc(tmem_slot, 512);
+    tmem_alloc(tmem_slot, M::COLUMNS);
     tmem_relinquish();
   }
   tc_fence_before();
@@ -655,8 +668,8 @@ linear_q4_many_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_cons
       for (int i = 0; i < min((steps + 1) / 2, 4); ++i) tma_prefetch_l2_2d(&tmW, (step0 + 2 * i) * 64, tile * 128);
       pdl_wait();
       bool ok = true;
-      Place<kManySteps> x;
-      Place<kManyCodeStages> c;
+      Place<M::STEPS> x;
+      Place<M::CODE_STAGES> c;
       for (int j = 0; j < steps; ++j) {
         if ((j & 1) == 0) {
           ok = wait(&c_empty[c.at], c.round ^ 1, ab, ERR_WAIT_EMPTY);
@@ -667,10 +680,10 @@ linear_q4_many_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_cons
         }
         ok = wait(&empty[x.at], x.round ^ 1, ab, ERR_WAIT_EMPTY);
         if (!ok) break;
-        uint8_t* to = smem + x.at * kManyX;
-        mbar_expect_tx(&full[x.at], kManyX);
+        uint8_t* to = smem + x.at * M::X;
+        mbar_expect_tx(&full[x.at], M::X);
         tma_load_2d(to, &tmX, &full[x.at], (step0 + j) * 128, tokens0 * NT);
-        tma_load_2d(to + kManyX / 2, &tmX, &full[x.at], (step0 + j) * 128 + 64, tokens0 * NT);
+        tma_load_2d(to + M::X / 2, &tmX, &full[x.at], (step0 + j) * 128 + 64, tokens0 * NT);
         x.on();
       }
       if (!ok) {
@@ -683,16 +696,16 @@ linear_q4_many_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_cons
     if (elect_one()) {
       constexpr uint32_t idesc = make_idesc_bf16(128, NT, false, false);
       bool ok = true;
-      Place<kManySteps> x;
+      Place<M::STEPS> x;
       for (int j = 0; j < steps; ++j) {
         ok = wait(&full[x.at], x.round, ab, ERR_WAIT_FULL);
         if (!ok) break;
         tc_fence_after();
-        const uint64_t xdesc = make_smem_desc_sw128(smem_u32(smem + x.at * kManyX), 16, 1024);
+        const uint64_t xdesc = make_smem_desc_sw128(smem_u32(smem + x.at * M::X), 16, 1024);
         const uint32_t weights = tmem + x.at * 64;
 #pragma unroll
         for (int k = 0; k < 8; ++k)              // 16 channels each, 64 to a box of x
-          tc_mma_ts(tmem + kManySums, weights + k * 8, xdesc + (uint64_t)(((k >> 2) * (kManyX / 2) + (k & 3) * 32) >> 4), idesc,
+          tc_mma_ts(tmem + M::SUMS, weights + k * 8, xdesc + (uint64_t)(((k >> 2) * (M::X / 2) + (k & 3) * 32) >> 4), idesc,
                     (j | k) != 0 ? 1u : 0u);
         tc_commit(&empty[x.at]);
         x.on();
@@ -700,7 +713,7 @@ linear_q4_many_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_cons
       if (ok && steps > 0) tc_commit(done);
     }
   } else if (warp >= 4) {
-    const int quad = warp & 3, row = quad * 32 + lane, side = (warp - 4) >> 2 & 1, half = (warp - 4) >> 3;
+    const int quad = warp & 3, row = quad * 32 + lane, side = ((warp - 4) >> 2) % M::SIDES, half = (warp - 4) >> 2 >= M::SIDES;
     const uint32_t lane_sel = static_cast<uint32_t>(quad * 32) << 16;
     const uint2* pairs = reinterpret_cast<const uint2*>(
         p.affine + static_cast<long long>(min(tile * 128 + row, p.N - 1)) * (p.width / 16)) + step0;
@@ -709,31 +722,37 @@ linear_q4_many_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_cons
     pdl_wait();
     bool ok = true;
     // a step takes a warp longer than it takes the tensor cores, mostly by waits: half of the warps have the odd steps
-    Place<kManyCodeStages> c;
-    Place<kManySteps> w;
+    Place<M::CODE_STAGES> c;
+    Place<M::STEPS> w;
     if (half) w.on();
     uint2 pair = half < steps ? __ldg(pairs + half) : make_uint2(0, 0);
     for (int j = half; j < steps; j += 2) {
       ok = wait_warp(&c_full[c.at], c.round, ab, ERR_WAIT_FULL);
       if (!ok) break;
-      uint32_t r[2][16];
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {              // word 4 c + k: channels 64 (k & 1) + 8 (2 c + k / 2) ..
-        const uint4 v = *reinterpret_cast<const uint4*>(codes + c.at * kCodeBytes + sw128_offset(row, half * 4 + 2 * side + k));
-        const uint32_t s0 = __byte_perm(pair.x, pair.x, 0x1010), z0 = __byte_perm(pair.x, pair.x, 0x3232);
-        const uint32_t s1 = __byte_perm(pair.y, pair.y, 0x1010), z1 = __byte_perm(pair.y, pair.y, 0x3232);
-        values(v.x, s0, z0, mask, magic, &r[0][8 * k]);
-        values(v.y, s1, z1, mask, magic, &r[1][8 * k]);
-        values(v.z, s0, z0, mask, magic, &r[0][8 * k + 4]);
-        values(v.w, s1, z1, mask, magic, &r[1][8 * k + 4]);
-      }
+      const uint32_t s0 = __byte_perm(pair.x, pair.x, 0x1010), z0 = __byte_perm(pair.x, pair.x, 0x3232);
+      const uint32_t s1 = __byte_perm(pair.y, pair.y, 0x1010), z1 = __byte_perm(pair.y, pair.y, 0x3232);
       pair = j + 2 < steps ? __ldg(pairs + j + 2) : make_uint2(0, 0);
-      ok = wait_warp(&empty[w.at], w.round ^ 1, ab, ERR_Q4_D);
+#pragma unroll
+      for (int part = side; part < 2; part += M::SIDES) {    // half of the channels each
+        uint32_t r[2][16];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {            // word 4 c + k: channels 64 (k & 1) + 8 (2 c + k / 2) ..
+          const uint4 v = *reinterpret_cast<const uint4*>(codes + c.at * kCodeBytes + sw128_offset(row, half * 4 + 2 * part + k));
+          values(v.x, s0, z0, mask, magic, &r[0][8 * k]);
+          values(v.y, s1, z1, mask, magic, &r[1][8 * k]);
+          values(v.z, s0, z0, mask, magic, &r[0][8 * k + 4]);
+          values(v.w, s1, z1, mask, magic, &r[1][8 * k + 4]);
+        }
+        if (part == side) {
+          ok = wait_warp(&empty[w.at], w.round ^ 1, ab, ERR_Q4_D);
+          if (!ok) break;
+          tc_fence_after();
+        }
+        const uint32_t to = tmem + w.at * 64 + part * 16 + lane_sel;
+        tmem_st16(to, r[0]);
+        tmem_st16(to + 32, r[1]);
+      }
       if (!ok) break;
-      tc_fence_after();
-      const uint32_t to = tmem + w.at * 64 + side * 16 + lane_sel;
-      tmem_st16(to, r[0]);
-      tmem_st16(to + 32, r[1]);
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
@@ -747,17 +766,19 @@ linear_q4_many_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_cons
     if (steps > 0) ok = wait_warp(done, 0, ab, ERR_Q4_D) && ok;
     tc_fence_after();
     // every product has been made, so every copy has landed and every operand has been used: the ring is free
-    const int token = (half * 2 + side) * 32;
-    uint32_t v[32];
-    if (steps > 0 && ok) {
-      tmem_ld_32x32b_x32(tmem + kManySums + token + lane_sel, v);
-      tmem_ld_wait();
-    } else {
+    const int token = (half * M::SIDES + side) * 32;
+    if (token < NT) {
+      uint32_t v[32];
+      if (steps > 0 && ok) {
+        tmem_ld_32x32b_x32(tmem + M::SUMS + token + lane_sel, v);
+        tmem_ld_wait();
+      } else {
 #pragma unroll
-      for (int i = 0; i < 32; ++i) v[i] = 0;
+        for (int i = 0; i < 32; ++i) v[i] = 0;
+      }
+#pragma unroll
+      for (int i = 0; i < 32; ++i) red[(token + i) * 128 + row] = __uint_as_float(v[i]);
     }
-#pragma unroll
-    for (int i = 0; i < 32; ++i) red[(token + i) * 128 + row] = __uint_as_float(v[i]);
   }
   __syncwarp();
   tc_fence_before();
@@ -767,9 +788,9 @@ linear_q4_many_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_cons
     __syncthreads();
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc(tmem, 512);
+    tmem_dealloc(tmem, M::COLUMNS);
   }
-  finish<NT>(red, p, tile, tokens0, rank, kManyThreads);
+  finish<NT>(red, p, tile, tokens0, rank, M::THREADS);
 }
 
 // Rows of up to 64 channels (one group, words in channel order): one warp per weight row and eight rows of x, a lane per word.
@@ -820,35 +841,32 @@ int launch_cluster(void (*kern)(Args...), const LinearParams& p, int threads, in
   return static_cast<int>(cudaLaunchKernelEx(&cfg, kern, args...));
 }
 
-template <int NT, bool SPLIT>
+template <bool SPLIT>
 int launch(const CUtensorMap& tmW, const CUtensorMap& tmX, const CUtensorMap& tmS, LinearParams p, cudaStream_t stream) {
   const int blocks = (p.width + kStage - 1) / kStage, slice = (blocks + p.cluster - 1) / p.cluster;
-  p.stages = (222 * 1024 / blocks_per_sm<NT>() - 2048) / stage_bytes<NT>();
-  if (p.stages > kMaxStages) p.stages = kMaxStages;
-  if (p.stages > slice) p.stages = slice;
-  if (p.stages < 2) p.stages = 2;
-  const int ring = p.stages * stage_bytes<NT>(), sums = NT * 128 * 4;   // the partial sums reuse the ring
-  const int smem_bytes = (ring > sums ? ring : sums) + 1024;
+  constexpr int most = (222 * 1024 / kFewBlocks - 2048) / kStageBytes;
+  static_assert(most >= kOwnStages && most <= kMaxStages && most * kStageBytes >= kFewRows * 128 * 4, "slots; the sums reuse them");
+  p.stages = slice < most ? (slice < 2 ? 2 : slice) : most;
+  const int smem_bytes = p.stages * kStageBytes + 1024;
   static bool configured[b200host::kMaxDevices] = {};
-  static_assert((222 * 1024 / blocks_per_sm<NT>() - 2048) / stage_bytes<NT>() >= own_stages(NT), "slots");
-  if (int rc = b200host::ensure_dynamic_smem(linear_q4_kernel<NT, SPLIT>, 200 * 1024, configured)) return rc;
-  return launch_cluster(linear_q4_kernel<NT, SPLIT>, p, kThreads, smem_bytes, stream, tmW, tmX, tmS, p);
+  if (int rc = b200host::ensure_dynamic_smem(linear_q4_kernel<SPLIT>, most * kStageBytes + 1024, configured)) return rc;
+  return launch_cluster(linear_q4_kernel<SPLIT>, p, kThreads, smem_bytes, stream, tmW, tmX, tmS, p);
 }
 
+template <int NT, int BLOCKS>
 int launch_many(const CUtensorMap& tmW, const CUtensorMap& tmX, const LinearParams& p, cudaStream_t stream) {
-  constexpr int bytes = kManySteps * kManyX + kManyCodeStages * kCodeBytes + 1024;
-  static_assert(kManySteps * kManyX >= kManyTokens * 128 * 4 && bytes <= 226 * 1024, "shared memory");
+  using M = Many<NT, BLOCKS>;
   static bool configured[b200host::kMaxDevices] = {};
-  if (int rc = b200host::ensure_dynamic_smem(linear_q4_many_kernel, bytes, configured)) return rc;
-  return launch_cluster(linear_q4_many_kernel, p, kManyThreads, bytes, stream, tmW, tmX, p);
+  if (int rc = b200host::ensure_dynamic_smem(linear_q4_many_kernel<NT, BLOCKS>, M::BYTES, configured)) return rc;
+  return launch_cluster(linear_q4_many_kernel<NT, BLOCKS>, p, M::THREADS, M::BYTES, stream, tmW, tmX, p);
 }
 
 }  // namespace
 
 // out [rows, N] (row stride ldo) = x [rows, K] (ldx) * W^T, W as codes [N, width / 8] words and affine [N, width / 64] pairs;
-// `cluster` (1, 2, 4 or 8) slices of K.  `work` is the call's own: with R = rows rounded up to 16 (up to 16 rows) or
-// 32 and width = K rounded up to 256, 5 * R * width / 2 bytes and then R floats; none with more than 64 rows, and none where a
-// slice has up to 512 (256) channels.  With more than 64 rows there are more than 64 channels, and rows of x start on 16 bytes.
+// `cluster` (1, 2, 4 or 8) slices of K.  `work` is the call's own: up to 16 rows, where a slice has more than
+// 512 channels, 40 * width bytes and then 16 floats, width = K rounded up to 256.  With more than 16 rows of more than 64 channels
+// rows of x start on 16 bytes.
 extern "C" int b200_q4_linear(const void* x, long long ldx, const void* codes, const void* affine, void* out,
                               long long ldo, int rows, int N, int K, int cluster, void* work, void* status,
                               void* stream) {
@@ -867,28 +885,30 @@ extern "C" int b200_q4_linear(const void* x, long long ldx, const void* codes, c
   CUtensorMap tmW, tmX, tmS;
   int rc;
   if ((rc = make_map_2d(&tmW, CU_TENSOR_MAP_DATA_TYPE_UINT8, codes, width / 2, N, width / 2, 128, 128))) return rc;
-  if (rows > 64) {
-    if (((long long)(rows + 127) / 128) * ((N + 127) / 128) * cluster > 0x7fffffffll) return RC_BAD_SHAPE;
-    if ((rc = make_map_2d(&tmX, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, x, K, rows, ldx * 2, 64, kManyTokens))) return rc;
-    return launch_many(tmW, tmX, LinearParams{(const uint8_t*)affine, nullptr, (__nv_bfloat16*)out, ldo, rows, N, width, cluster,
-                                              0, (rows + kManyTokens - 1) / kManyTokens, (int*)status}, s);
+  if (rows > kFewRows) {
+    const int NT = rows <= 64 ? 64 : 128, tiles = (rows + NT - 1) / NT;
+    if ((long long)tiles * ((N + 127) / 128) * cluster > 0x7fffffffll) return RC_BAD_SHAPE;
+    if ((rc = make_map_2d(&tmX, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, x, K, rows, ldx * 2, 64, NT))) return rc;
+    const LinearParams p{(const uint8_t*)affine, nullptr, (__nv_bfloat16*)out, ldo, rows, N, width, cluster, 0, tiles, (int*)status};
+    if (NT == 128) return launch_many<128, 1>(tmW, tmX, p, s);
+    // two smaller blocks an SM where there are more than SMs: 64 rows, 224 blocks of 28672 x 4096 28.6 us instead of 35.5, 64 of
+    // 4096 x 14336 in two slices 34 us instead of 27.7
+    return (N + 127) / 128 * tiles * cluster > sm_count() ? launch_many<64, 2>(tmW, tmX, p, s) : launch_many<64, 1>(tmW, tmX, p, s);
   }
-  const int NT = rows <= 16 ? 16 : 32, tiles = (rows + NT - 1) / NT, tokens = NT * tiles;
   const int aligned = ldx % 8 == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0;
   const int xwidth = (K + kStage - 1) / kStage * kStage;
-  LinearParams p{(const uint8_t*)affine, nullptr, (__nv_bfloat16*)out, ldo, rows, N, width, cluster, 0, tiles,
+  LinearParams p{(const uint8_t*)affine, nullptr, (__nv_bfloat16*)out, ldo, rows, N, width, cluster, 0, 1,
                  (int*)status, (const __nv_bfloat16*)x, ldx, K, aligned};
-  if ((xwidth / kStage + cluster - 1) / cluster <= own_stages(NT))
-    return NT == 16 ? launch<16, false>(tmW, tmW, tmW, p, s) : launch<32, false>(tmW, tmW, tmW, p, s);
+  if ((xwidth / kStage + cluster - 1) / cluster <= kOwnStages) return launch<false>(tmW, tmW, tmW, p, s);
   if (!work || (reinterpret_cast<uintptr_t>(work) & 15)) return RC_BAD_ALIGNMENT;
   uint8_t* xq = static_cast<uint8_t*>(work);
-  uint8_t* sums = xq + 2ll * tokens * xwidth;
-  float* xs = reinterpret_cast<float*>(sums + tokens * (xwidth / 2ll));
-  if ((rc = make_map_2d(&tmX, CU_TENSOR_MAP_DATA_TYPE_UINT8, xq, xwidth, 2 * tokens, xwidth, 128, 2 * NT))) return rc;
-  if ((rc = make_map_2d(&tmS, CU_TENSOR_MAP_DATA_TYPE_UINT8, sums, xwidth / 2, tokens, xwidth / 2, 128, NT))) return rc;
-  if (cudaError_t e = launch_kernel(linear_q4_split_kernel, dim3(tokens), dim3(512), 0, s, pdl, (const __nv_bfloat16*)x, ldx,
-                                    rows, K, xwidth, NT, aligned, xq, xs))
+  uint8_t* sums = xq + 2ll * kFewRows * xwidth;
+  float* xs = reinterpret_cast<float*>(sums + kFewRows * (xwidth / 2ll));
+  if ((rc = make_map_2d(&tmX, CU_TENSOR_MAP_DATA_TYPE_UINT8, xq, xwidth, 2 * kFewRows, xwidth, 128, 2 * kFewRows))) return rc;
+  if ((rc = make_map_2d(&tmS, CU_TENSOR_MAP_DATA_TYPE_UINT8, sums, xwidth / 2, kFewRows, xwidth / 2, 128, kFewRows))) return rc;
+  if (cudaError_t e = launch_kernel(linear_q4_split_kernel, dim3(kFewRows), dim3(512), 0, s, pdl, (const __nv_bfloat16*)x, ldx,
+                                    rows, K, xwidth, aligned, xq, xs))
     return static_cast<int>(e);
   p.xs = xs;
-  return NT == 16 ? launch<16, true>(tmW, tmX, tmS, p, s) : launch<32, true>(tmW, tmX, tmS, p, s);
+  return launch<true>(tmW, tmX, tmS, p, s);
 }

@@ -30,7 +30,7 @@ from research_b200.ops import native
 
 GROUP = 64
 #: Rows of x up to which a linear multiplies the codes themselves; above, bf16 weights, expanded on their way or before.
-FEW_ROWS = 64
+FEW_ROWS = 16
 
 
 class Q4Rows(NamedTuple):
@@ -414,7 +414,7 @@ def _attention_runs(B: int, Hkv: int, rows: int, device: int) -> int:
 # --------------------------------------------------------------------------------------------------
 def linear_q4(x: torch.Tensor, w: Q4Rows) -> torch.Tensor:
     """``y = x W^T`` for ``x [..., K]`` and weights ``w`` of ``N`` 4-bit rows of K channels; ``y [..., N]`` in x's type.  Up to
-    64 rows of x the weights count as they are, and x to 2^-17 of its row's largest value (a row with an infinity or a NaN
+    16 rows of x the weights count as they are, and x to 2^-17 of its row's largest value (a row with an infinity or a NaN
     gives NaN); for more rows x counts as it is, and each weight as a bf16."""
 
     what = "linear_q4"
@@ -444,10 +444,10 @@ def linear_q4(x: torch.Tensor, w: Q4Rows) -> torch.Tensor:
 def _coded_linear(x: torch.Tensor, w: Q4Rows, rows: int, N: int, K: int, slices: int) -> torch.Tensor:
     work = None
     if rows > FEW_ROWS:
-        x = _rows_on_16_bytes(x)
-    elif K > (512 if rows <= 16 else 256) * slices:     # x as the kernel multiplies it, for slices that blocks do not split
-        tokens, width = 16 if rows <= 16 else -(-rows // 32) * 32, -(-K // 256) * 256
-        work = w.codes.new_empty(tokens * (2 * width + width // 2 + 4))
+        if K > GROUP:
+            x = _rows_on_16_bytes(x)
+    elif K > 512 * slices:                              # x as the kernel multiplies it, for slices that blocks do not split
+        work = w.codes.new_empty(-(-K // 256) * 256 * 40 + 64)
     ld, one = x.stride()
     if one != 1:
         x, ld = x.contiguous(), K
@@ -474,46 +474,46 @@ def linear_slices(rows: int, n: int, k: int, sms: int = 148) -> int:
     """Slices of K (1, 2, 4 or 8 blocks of a cluster) for a product with 4-bit weights: the count of least estimated time, or 0
     where that is to expand the weights first.
 
-    Up to 64 rows a stage of 256 channels takes a block 0.65 us (1.4 with more than 16 rows of x) by itself and an SM 0.55 (0.8)
-    where several of its up to four (two) blocks share it; slices add the exchange of partial sums.  Where a block splits its
-    slice of x itself, that is most of its time.  Measured with 1 / 32 rows, 1 / 2 / 4 / 8 slices: 2048 x 2048 10.7 / 8.3 / 7.4 / 5.7
-    and 15.6 / 10.9 / 8.8 / 8.6 us, 4096 x 2048 10.8 / 8.7 / 8.0 / 6.5 us (1 row), 11264 x 2048 11.8 / 9.8 / 10.8 / 13.9 and 16.9 / 12.6 /
-    16.6 / 23.0 us, 28672 x 4096 31.7 / 22.5 / 26.7 / 43.4 and 31.0 / 37.5 / 45.6 / 90.7 us.
+    Up to 16 rows a stage of 256 channels takes a block 0.65 us by itself and an SM 0.55 where several of its up to four blocks
+    share it; slices add the exchange of partial sums.  Where a block splits its slice of x itself, that is most of its time.
+    Measured with 1 row, 1 / 2 / 4 / 8 slices: 2048 x 2048 10.7 / 8.3 / 7.4 / 5.7 us, 4096 x 2048 10.8 / 8.7 / 8.0 / 6.5 us, 11264 x 2048
+    11.8 / 9.8 / 10.8 / 13.9 us, 28672 x 4096 31.7 / 22.5 / 26.7 / 43.4 us.
 
-    With more rows a tile of 128 x 128 has an SM for itself, for 5 us and 0.36 us per 128 channels, and clusters of 4 and 8 find
-    no room on some of the SMs.  Expanding takes 1.5 us and 0.48 us a million weights, and the GEMM then 0.4 us per 64 channels
-    of its tiles of 128 x 256.  Measured 1 / 2 / 4 / 8 slices, expanded: 128 rows, 2048 x 2048 11.1 / 8.7 / 7.5 / 16.5, 17.6 us; 65 rows,
-    4096 x 4096 16.4 / 11.0 / 9.5 / 22.6, 31.7 us; 777 rows, 2048 x 5632 22.8 / 29.8 / 44.7 / 80.6, 38.2 us; 1024 rows, 4096 x 4096
+    With more rows a step of 128 channels takes a tile 0.34 us (0.36 with more than 64 rows) by itself, twice that in pairs on an
+    SM (up to 64 rows), and clusters of 4 and 8 find no room on some of the SMs.  Expanding first takes 1.5 us and 0.48 us a
+    million weights, and the GEMM then 0.4 us per 64 channels of its tiles of 128 x 256.  Measured 1 / 2 / 4 / 8 slices, expanded:
+    32 rows, 2048 x 2048 9.4 / 7.2 / 5.9 / 11.0 us, 11264 x 2048 9.8 / 10.8 / 13.1 / 21.1 us, 28672 x 4096 27.7 / 32.4 / 38.7 / 59.7 us; 128
+    rows, 2048 x 2048 11.1 / 8.7 / 7.5 / 16.5, 17.6 us; 777 rows, 2048 x 5632 22.8 / 29.8 / 44.7 / 80.6, 38.2 us; 1024 rows, 4096 x 4096
     36.9 / 52.3 / 81.1 / 172.9, 36.2 us; 2048 rows, 2048 x 2048 23.9 / 38.7 / 66.3 / 156.5, 19.0 us."""
 
+    if k <= GROUP:
+        return 1 if rows <= 64 else 0
     stages = -(-k // 256)
     best, best_cost = 1, float("inf")
-    if rows <= FEW_ROWS:
-        few = rows <= 16
-        base, alone, shared, room = (5.5, 0.65, 0.55, 4) if few else (4.4, 1.4, 0.8, 2)
-        own, own_base, own_stage, own_shared = (2, 4.1, 1.6, 0.6) if few else (1, 5.9, 2.7, 0.45)
-        tiles = -(-n // 128) * -(-rows // 32)
-        for s, exchange in ((1, 0.0), (2, 1.1), (4, 1.6), (8, 2.2)):
-            if s > 1 and stages < s:
-                break
-            per, per_sm = -(-stages // s), math.ceil(tiles * s / sms - 0.1)
-            waves = -(-per_sm // room)                  # of blocks, each with 2.5 us to begin and to end
-            if per <= own:
-                cost = own_base + waves * per * own_stage * (1 + own_shared * (max(min(per_sm, room), 1) - 1))
+    for s, exchange, full in ((1, 0.0, 1.0), (2, 0.3, 1.0), (4, 0.5, 0.9), (8, 1.2, 0.75)):
+        if s > 1 and stages < s:
+            break
+        per = -(-stages // s)
+        if rows <= FEW_ROWS:
+            per_sm = max(math.ceil(-(-n // 128) * s / sms - 0.1), 1)
+            waves = -(-per_sm // 4)                     # of blocks, each with 2.5 us to begin and to end
+            if per <= 2:
+                cost = 4.1 + waves * per * 1.6 * (1 + 0.6 * (min(per_sm, 4) - 1))
             else:
-                cost = base + per * max(alone, (per_sm if waves == 1 else waves * room) * shared) + exchange
-            cost += (max(waves, 1) - 1) * 2.5
-            if cost < best_cost:
-                best, best_cost = s, cost
+                cost = 5.5 + per * max(0.65, (per_sm if waves == 1 else waves * 4) * 0.55) + 1.8 * exchange
+            cost += (waves - 1) * 2.5
+        else:
+            blocks = -(-n // 128) * -(-rows // (64 if rows <= 64 else 128)) * s
+            if rows <= 64 and blocks > sms:
+                waves = math.ceil(blocks / (2 * sms))
+                cost = 4.4 + 1.36 * per * waves + (waves - 1) * 6.0 + exchange
+            else:
+                waves = math.ceil(blocks / (sms * full))
+                cost = (4.6 + 0.68 * per if rows <= 64 else 5.0 + 0.72 * per) * waves + exchange + (1.7 if rows > 64 else 0.0)
+        if cost < best_cost:
+            best, best_cost = s, cost
+    if rows <= 64:
         return best
-    if k > GROUP:
-        tiles = -(-n // 128) * -(-rows // 128)
-        for s, exchange, blocks in ((1, 0.0, sms), (2, 0.5, sms), (4, 0.7, sms * 0.9), (8, 1.5, sms * 0.75)):
-            if s > 1 and stages < s:
-                break
-            cost = math.ceil(tiles * s / blocks) * (5.0 + 0.72 * -(-stages // s)) + 1.7 + exchange
-            if cost < best_cost:
-                best, best_cost = s, cost
     waves = math.ceil(-(-n // 256) * -(-rows // 128) / sms)
     return best if best_cost < 3.5 + 0.48e-6 * n * k + waves * (2.0 + 0.4 * -(-k // 64)) else 0
 

@@ -309,9 +309,10 @@ def test_linear_against_64_bits(rows, N, K):
     x = torch.randn(rows, K, generator=g, device="cuda").to(BF16)
     w = q4.quantize_rows_q4(torch.randn(N, K, generator=g, device="cuda") * 0.05)
     want, sums, plain = _linear64(x, w, K)
-    # from 65 rows the weights are rounded to bf16 and the sums run over K in one accumulator
+    # from 17 rows (65 of up to 64 channels) the weights are rounded to bf16 and the sums run over K in one accumulator: to the
+    # result's rounding come 2^-8 of each |x w|, and 2^-23 of the running sum for each of K additions
     tol = 2.0 ** -8 * want.abs() + sums
-    if rows > 64:
+    if rows > (16 if K > 64 else 64):
         tol = 2.0 ** -8 * want.abs() + plain * (1.01 * 2.0 ** -8 + 2.0 ** -23 * K)
     got = q4.linear_q4(x, w)
     assert got.shape == (rows, N) and got.dtype == BF16
@@ -346,7 +347,7 @@ def test_linear_of_many_rows(rows, N, K, slices):
     assert (off <= tol).all(), (off - tol).max()
 
 
-@pytest.mark.parametrize("rows", [3, 20, 50])
+@pytest.mark.parametrize("rows", [3, 9, 16])
 def test_linear_rows_of_uneven_size(rows):
     """A channel of 2^12 times the others' size, a row of tiny values, a row of zeros, one of huge values."""
 
