@@ -314,16 +314,23 @@ KVCache = PagedKVCache
 
 class QuantizedWeights:
     """4-bit copies of a model's linear weights, in use from :func:`quantize_weights` until :meth:`remove` (or the end of a
-    ``with`` block).  They are copies: parameters that change meanwhile are not seen."""
+    ``with`` block).  They are copies: parameters that change meanwhile are not seen.  What a parameter had before (copies
+    of an outer block) it has again afterwards."""
 
-    def __init__(self, params: list[torch.nn.Parameter]):
-        self._params = params
+    def __init__(self):
+        self._before: list[tuple[torch.nn.Parameter, quantized.Q4Rows | None]] = []
+
+    def _add(self, p: torch.nn.Parameter, rows: quantized.Q4Rows) -> None:
+        self._before.append((p, getattr(p, "q4", None)))
+        p.q4 = rows
 
     def remove(self) -> None:
-        for p in self._params:
-            if hasattr(p, "q4"):
+        while self._before:
+            p, rows = self._before.pop()
+            if rows is not None:
+                p.q4 = rows
+            elif hasattr(p, "q4"):
                 del p.q4
-        self._params = []
 
     def __enter__(self) -> "QuantizedWeights":
         return self
@@ -343,19 +350,23 @@ def quantize_weights(model) -> QuantizedWeights:
 
     if getattr(getattr(model, "ex", None), "tp_size", 1) > 1:
         raise ContractError("generation.weight_bits=4 needs whole weights: the model is split over tensor-parallel ranks")
-    params = []
+    weights = QuantizedWeights()
     dtype = getattr(model, "compute_dtype", torch.float32)
-    for index, layer in enumerate(model.layers):
-        if model.layer_prepare is not None:
-            model.layer_prepare(index)
-        for module in layer.modules():
-            for name in _BLOCK_LINEARS:
-                p = module._parameters.get(name)
-                if p is None or p.dim() != 2:                   # routed experts are stacks of matrices
-                    continue
-                p.q4 = quantized.quantize_rows_q4(Fn.compute_weight(p, torch.empty(0, dtype=dtype, device=p.device)))
-                params.append(p)
-    return QuantizedWeights(params)
+    try:
+        for index, layer in enumerate(model.layers):
+            if model.layer_prepare is not None:
+                model.layer_prepare(index)
+            for module in layer.modules():
+                for name in _BLOCK_LINEARS:
+                    p = module._parameters.get(name)
+                    if p is None or p.dim() != 2:               # routed experts are stacks of matrices
+                        continue
+                    weights._add(p, quantized.quantize_rows_q4(
+                        Fn.compute_weight(p, torch.empty(0, dtype=dtype, device=p.device))))
+    except BaseException:
+        weights.remove()
+        raise
+    return weights
 
 
 @torch.no_grad()

@@ -676,8 +676,8 @@ int launch(const AttnParams& p, cudaStream_t s) {
   // 256 threads 23.1 us, 512 21.8, 1024 26.0; 7 pieces of 512 heads, 256 threads 46.6 us, and 512 find less room beside the
   // first kernel
   const bool many = p.warps > 32 * p.B * p.Hkv;
-  return static_cast<int>(b200host::launch_kernel(many ? decode_q4_merge_kernel<D, kRows, 512> : decode_q4_merge_kernel<D, kRows, 256>,
-                                                  dim3(p.B * p.Hq), dim3(many ? 512 : 256), 0, s, pdl, p));
+  auto* merge = many ? decode_q4_merge_kernel<D, kRows, 512> : decode_q4_merge_kernel<D, kRows, 256>;
+  return static_cast<int>(b200host::launch_kernel(merge, dim3(p.B * p.Hq), dim3(many ? 512 : 256), 0, s, pdl, p));
 }
 
 }  // namespace

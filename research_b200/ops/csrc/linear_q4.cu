@@ -6,10 +6,11 @@
 // bandwidth an SM gets 46 codes a clock, which is what the arrangement below is for.  Measured, 1 row: 2048 x 2048 5.6 us, a
 // stage's latency; 28672 x 4096 22.4 us, 0.45 of the copy bandwidth, 0.55 us per stage of 256 channels and SM.
 //
-// The weights are the 128-row operand of tcgen05.mma, from tensor memory, the rows of x its 16 columns, both in e4m3.  The bytes 0 .. 15 are, as e4m3, the numbers n 2^-9 (subnormals and the first binade are one straight line), so that a
-// word of eight codes becomes eight operands by two masks and a shift, a third of what bf16 operands take, in half the tensor
-// memory.  A row of x is brought to [128, 256) by a power of two and split into two e4m3 numbers, high + low, which go into
-// one accumulator: the eight bits of a bf16 are two times four, so that is exact down to 2^-9 of the row's largest value, and
+// The weights are the 128-row operand of tcgen05.mma, from tensor memory, the rows of x its 16 columns, both in e4m3.  The
+// bytes 0 .. 15 are, as e4m3, the numbers n 2^-9 (subnormals and the first binade are one straight line), so that a word of
+// eight codes becomes eight operands by two masks and a shift, a third of what bf16 operands take, in half the tensor memory.
+// A row of x is brought to [128, 256) by a power of two and split into two e4m3 numbers, high + low, which go into one
+// accumulator: the eight bits of a bf16 are two times four, so that is exact down to 2^-9 of the row's largest value, and
 // below that off by 2^-17 of it at most.  The product of each group is taken by itself.  The sum X_g of x over a group gets
 // into every lane as a product too, of fours with 32 e4m3 numbers that add up to a quarter of it (16 times its sixteenth, then
 // what is left: to 2^-15 of the row's largest value); scales and least values are applied to both in fp32:
@@ -889,7 +890,8 @@ extern "C" int b200_q4_linear(const void* x, long long ldx, const void* codes, c
     const int NT = rows <= 64 ? 64 : 128, tiles = (rows + NT - 1) / NT;
     if ((long long)tiles * ((N + 127) / 128) * cluster > 0x7fffffffll) return RC_BAD_SHAPE;
     if ((rc = make_map_2d(&tmX, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, x, K, rows, ldx * 2, 64, NT))) return rc;
-    const LinearParams p{(const uint8_t*)affine, nullptr, (__nv_bfloat16*)out, ldo, rows, N, width, cluster, 0, tiles, (int*)status};
+    const LinearParams p{(const uint8_t*)affine, nullptr, (__nv_bfloat16*)out, ldo, rows, N, width, cluster, 0, tiles,
+                         (int*)status};
     if (NT == 128) return launch_many<128, 1>(tmW, tmX, p, s);
     // two smaller blocks an SM where there are more than SMs: 64 rows, 224 blocks of 28672 x 4096 28.6 us instead of 35.5, 64 of
     // 4096 x 14336 in two slices 34 us instead of 27.7

@@ -169,6 +169,17 @@ def test_quantized_weights_are_used_without_gradients_only(kind):
     held.remove()                                                       # twice is once
 
 
+def test_generation_within_quantized_weights_leaves_them_in_use():
+    model = _model()
+    ids = torch.randint(0, 256, (1, 5))
+    with quantize_weights(model):
+        p = model.layers[0].attn.wqkv
+        rows = p.q4
+        generate_tokens(model, ids, max_new_tokens=2, weight_bits=4)
+        assert p.q4 is rows
+    assert not hasattr(p, "q4")
+
+
 def test_a_model_that_is_split_is_refused_and_gradients_too():
     model = _model()
     whole, model.ex = model.ex, SimpleNamespace(tp_size=2)
