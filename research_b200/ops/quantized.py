@@ -29,8 +29,6 @@ from research_b200.errors import KernelError
 from research_b200.ops import native
 
 GROUP = 64
-#: Rows of x up to which a linear multiplies the codes themselves; above, bf16 weights, expanded on their way or before.
-FEW_ROWS = 16
 
 
 class Q4Rows(NamedTuple):
@@ -414,8 +412,8 @@ def _attention_runs(B: int, Hkv: int, rows: int, device: int) -> int:
 # --------------------------------------------------------------------------------------------------
 def linear_q4(x: torch.Tensor, w: Q4Rows) -> torch.Tensor:
     """``y = x W^T`` for ``x [..., K]`` and weights ``w`` of ``N`` 4-bit rows of K channels; ``y [..., N]`` in x's type.  Up to
-    16 rows of x the weights count as they are, and x to 2^-17 of its row's largest value (a row with an infinity or a NaN
-    gives NaN); for more rows x counts as it is, and each weight as a bf16."""
+    8 or 16 rows of x (:func:`few_rows`) the weights count as they are; for more rows each counts as a
+    bf16.  An infinity or a NaN in a row of x leaves no number in its results."""
 
     what = "linear_q4"
     if x.dim() < 1 or not x.is_floating_point() or x.shape[-1] < 1:
@@ -442,23 +440,27 @@ def linear_q4(x: torch.Tensor, w: Q4Rows) -> torch.Tensor:
 
 
 def _coded_linear(x: torch.Tensor, w: Q4Rows, rows: int, N: int, K: int, slices: int) -> torch.Tensor:
-    work = None
-    if rows > FEW_ROWS:
-        if K > GROUP:
-            x = _rows_on_16_bytes(x)
-    elif K > 512 * slices:                              # x as the kernel multiplies it, for slices that blocks do not split
-        work = w.codes.new_empty(-(-K // 256) * 256 * 40 + 64)
+    if rows > few_rows(N, K):
+        x = _rows_on_16_bytes(x)
     ld, one = x.stride()
     if one != 1:
         x, ld = x.contiguous(), K
-    device = x.device
     out = x.new_empty(rows, N)
     native._check((native._lib or native.load()).b200_q4_linear(
-        x.data_ptr(), ld, w.codes.data_ptr(), w.affine.data_ptr(), out.data_ptr(), N, rows, N, K,
-        slices, native._ptr(work), native.status_word(device).data_ptr(), native._stream()),
-        "b200_q4_linear")
-    native.LAUNCHES += work is not None                 # _check counts one launch; the split of x is another
+        x.data_ptr(), ld, w.codes.data_ptr(), w.affine.data_ptr(), out.data_ptr(), N, rows, N, K, slices,
+        native.status_word(x.device).data_ptr(), native._stream()), "b200_q4_linear")
     return out
+
+
+def few_rows(n: int, k: int) -> int:
+    """Rows of x up to which a linear of ``n`` x ``k`` weights multiplies the codes themselves; more rows have bf16 weights,
+    expanded on their way or before."""
+
+    if k <= GROUP:
+        return 64
+    if k <= 2048 or (k <= 16384 and n * k <= 2 ** 24):
+        return 16
+    return 8 if k <= 32768 else 0
 
 
 def _rows_on_16_bytes(x: torch.Tensor) -> torch.Tensor:
@@ -471,45 +473,32 @@ def _rows_on_16_bytes(x: torch.Tensor) -> torch.Tensor:
 
 @functools.lru_cache(maxsize=4096)
 def linear_slices(rows: int, n: int, k: int, sms: int = 148) -> int:
-    """Slices of K (1, 2, 4 or 8 blocks of a cluster) for a product with 4-bit weights: the count of least estimated time, or 0
-    where that is to expand the weights first.
+    """Slices of K (1, 2, 4 or 8 blocks of a cluster) for a product of more than :func:`few_rows` rows with 4-bit weights: the
+    count of least estimated time, or 0 where that is to expand the weights first.
 
-    Up to 16 rows a stage of 256 channels takes a block 0.65 us by itself and an SM 0.55 where several of its up to four blocks
-    share it; slices add the exchange of partial sums.  Where a block splits its slice of x itself, that is most of its time.
-    Measured with 1 row, 1 / 2 / 4 / 8 slices: 2048 x 2048 10.7 / 8.3 / 7.4 / 5.7 us, 4096 x 2048 10.8 / 8.7 / 8.0 / 6.5 us, 11264 x 2048
-    11.8 / 9.8 / 10.8 / 13.9 us, 28672 x 4096 31.7 / 22.5 / 26.7 / 43.4 us.
+    A step of 128 channels takes a tile of 128 weights and 64 rows 0.34 us (0.36 with 128 rows) by itself, twice that in
+    pairs on an SM (up to 64 rows), and clusters of 4 and 8 find no room on some of the SMs.  Expanding first takes 1.5 us and
+    0.48 us a million weights, and the GEMM then 0.4 us per 64 channels of its tiles of 128 x 256.  Measured 1 / 2 / 4 / 8 slices,
+    expanded: 32 rows, 2048 x 2048 9.4 / 7.2 / 5.9 / 11.0 us, 11264 x 2048 9.8 / 10.8 / 13.1 / 21.1 us, 28672 x 4096 27.7 / 32.4 /
+    38.7 / 59.7 us; 128 rows, 2048 x 2048 11.1 / 8.7 / 7.5 / 16.5, 17.6 us; 777 rows, 2048 x 5632 22.8 / 29.8 / 44.7 / 80.6, 38.2 us; 1024
+    rows, 4096 x 4096 36.9 / 52.3 / 81.1 / 172.9, 36.2 us; 2048 rows, 2048 x 2048 23.9 / 38.7 / 66.3 / 156.5, 19.0 us."""
 
-    With more rows a step of 128 channels takes a tile 0.34 us (0.36 with more than 64 rows) by itself, twice that in pairs on an
-    SM (up to 64 rows), and clusters of 4 and 8 find no room on some of the SMs.  Expanding first takes 1.5 us and 0.48 us a
-    million weights, and the GEMM then 0.4 us per 64 channels of its tiles of 128 x 256.  Measured 1 / 2 / 4 / 8 slices, expanded:
-    32 rows, 2048 x 2048 9.4 / 7.2 / 5.9 / 11.0 us, 11264 x 2048 9.8 / 10.8 / 13.1 / 21.1 us, 28672 x 4096 27.7 / 32.4 / 38.7 / 59.7 us; 128
-    rows, 2048 x 2048 11.1 / 8.7 / 7.5 / 16.5, 17.6 us; 777 rows, 2048 x 5632 22.8 / 29.8 / 44.7 / 80.6, 38.2 us; 1024 rows, 4096 x 4096
-    36.9 / 52.3 / 81.1 / 172.9, 36.2 us; 2048 rows, 2048 x 2048 23.9 / 38.7 / 66.3 / 156.5, 19.0 us."""
-
+    if rows <= few_rows(n, k):
+        return 1
     if k <= GROUP:
-        return 1 if rows <= 64 else 0
+        return 0
     stages = -(-k // 256)
     best, best_cost = 1, float("inf")
     for s, exchange, full in ((1, 0.0, 1.0), (2, 0.3, 1.0), (4, 0.5, 0.9), (8, 1.2, 0.75)):
         if s > 1 and stages < s:
             break
-        per = -(-stages // s)
-        if rows <= FEW_ROWS:
-            per_sm = max(math.ceil(-(-n // 128) * s / sms - 0.1), 1)
-            waves = -(-per_sm // 4)                     # of blocks, each with 2.5 us to begin and to end
-            if per <= 2:
-                cost = 4.1 + waves * per * 1.6 * (1 + 0.6 * (min(per_sm, 4) - 1))
-            else:
-                cost = 5.5 + per * max(0.65, (per_sm if waves == 1 else waves * 4) * 0.55) + 1.8 * exchange
-            cost += (waves - 1) * 2.5
+        per, blocks = -(-stages // s), -(-n // 128) * -(-rows // (64 if rows <= 64 else 128)) * s
+        if rows <= 64 and blocks > sms:
+            waves = math.ceil(blocks / (2 * sms))
+            cost = 4.4 + 1.36 * per * waves + (waves - 1) * 6.0 + exchange
         else:
-            blocks = -(-n // 128) * -(-rows // (64 if rows <= 64 else 128)) * s
-            if rows <= 64 and blocks > sms:
-                waves = math.ceil(blocks / (2 * sms))
-                cost = 4.4 + 1.36 * per * waves + (waves - 1) * 6.0 + exchange
-            else:
-                waves = math.ceil(blocks / (sms * full))
-                cost = (4.6 + 0.68 * per if rows <= 64 else 5.0 + 0.72 * per) * waves + exchange + (1.7 if rows > 64 else 0.0)
+            waves = math.ceil(blocks / (sms * full))
+            cost = (4.6 + 0.68 * per if rows <= 64 else 5.0 + 0.72 * per) * waves + exchange + (1.7 if rows > 64 else 0.0)
         if cost < best_cost:
             best, best_cost = s, cost
     if rows <= 64:

@@ -3,11 +3,6 @@
 Tolerances count roundings.  A bf16 result is off by 2^-8 of itself at most (half a step).  In front of that, sums of
 products ``x n`` are formed in fp32, in the tensor cores' order: a chain of at most 8 additions per group of 64, each off by
 2^-23 of a running sum that is at most ``sum |x| (16 s + |z|)`` in the result's units, hence 2^-20 of that.
-
-A linear's row of x is split into two e4m3 numbers after a power of two has brought its largest value X to 128 .. 256.  A bf16
-of 2^-2 and more is their sum exactly (its 8 bits are 4 in the first and, of what is left, 4 in the second, whose last place
-is 2^-9 or more); a smaller one, below X / 512, is off by half of 2^-9, which is 2^-17 X, times a code of up to 15.  The sum over
-a group is held as 16 a + b + c + d + e, a quarter of it: what is left over is half of 2^-9 again, four times that 2^-15 X.
 """
 
 import math
@@ -288,18 +283,15 @@ def test_offsets_past_32_bits():
 
 # ------------------------------------------------------------------------------------------------- linear
 def _linear64(x, w, K):
-    """Result in 64 bits, what the tolerance of up to 64 rows adds to its rounding, and ``|x| |W|^T``."""
+    """Result in 64 bits, what the tolerance of codes as they are adds to its rounding, and ``|x| |W|^T``."""
 
     a, width = w.affine.double(), w.codes.shape[1] * 2
     s, z = a[..., 0].abs(), a[..., 1].abs()
     xd = torch.nn.functional.pad(x.double().abs(), (0, width - K)).unflatten(-1, (-1, 64))          # rows, groups, 64
     full = q4.dequantize_rows_reference(w, K, torch.float64)
     want = x.double() @ full.t()
-    most = xd.amax((1, 2), keepdim=True)
-    small = (xd < most / 512).double().sum(-1)
     sums = xd.sum(-1) @ (16 * s + z).t()                    # 2^-20 per group, and 2^-23 for each of K / 64 additions of groups
-    split = most[:, 0] * (2.0 ** -17 * small @ (15 * s).t() + 2.0 ** -15 * z.sum(-1))
-    return want, sums * (2.0 ** -20 + 2.0 ** -23 * (K / 64)) + split, x.double().abs() @ full.abs().t()
+    return want, sums * (2.0 ** -20 + 2.0 ** -23 * (K / 64)), x.double().abs() @ full.abs().t()
 
 
 @pytest.mark.parametrize("rows", [1, 2, 7, 8, 9, 16, 17, 31, 33, 48, 64, 65, 200])
@@ -309,10 +301,10 @@ def test_linear_against_64_bits(rows, N, K):
     x = torch.randn(rows, K, generator=g, device="cuda").to(BF16)
     w = q4.quantize_rows_q4(torch.randn(N, K, generator=g, device="cuda") * 0.05)
     want, sums, plain = _linear64(x, w, K)
-    # from 17 rows (65 of up to 64 channels) the weights are rounded to bf16 and the sums run over K in one accumulator: to the
-    # result's rounding come 2^-8 of each |x w|, and 2^-23 of the running sum for each of K additions
+    # above few_rows the weights are rounded to bf16 and the sums run over K in one accumulator: to the result's rounding come
+    # 2^-8 of each |x w|, and 2^-23 of the running sum for each of K additions
     tol = 2.0 ** -8 * want.abs() + sums
-    if rows > (16 if K > 64 else 64):
+    if rows > q4.few_rows(N, K):
         tol = 2.0 ** -8 * want.abs() + plain * (1.01 * 2.0 ** -8 + 2.0 ** -23 * K)
     got = q4.linear_q4(x, w)
     assert got.shape == (rows, N) and got.dtype == BF16
@@ -345,6 +337,23 @@ def test_linear_of_many_rows(rows, N, K, slices):
     off[:, N - 2] = 0.0
     tol = 2.0 ** -8 * want.abs() + plain * (1.01 * 2.0 ** -8 + 2.0 ** -23 * K)
     assert (off <= tol).all(), (off - tol).max()
+
+
+@pytest.mark.parametrize("rows,N,K", [(1, 20003, 5632), (16, 7200, 2300), (7, 300, 16000), (8, 40, 32768), (11, 100, 16384),
+                                      (9, 100, 17000), (1, 100, 33000), (5, 70000, 130), (13, 3001, 999), (2, 17, 4096)])
+def test_linear_of_long_rows_and_many_weights(rows, N, K):
+    """One block to a row, clusters of two to eight, more tiles than a cluster's blocks hold sums of, and rows too long."""
+
+    g = _gen(rows + K)
+    x = torch.randn(rows, K, generator=g, device="cuda").to(BF16)
+    w = q4.quantize_rows_q4(torch.randn(N, K, generator=g, device="cuda") * 0.05)
+    want, tol, plain = _linear64(x, w, K)
+    if rows > q4.few_rows(N, K):
+        tol = plain * (1.01 * 2.0 ** -8 + 2.0 ** -23 * K)
+    got = q4.linear_q4(x, w)
+    off = (got.double() - want).abs()
+    assert (off <= 2.0 ** -8 * want.abs() + tol).all(), (off - 2.0 ** -8 * want.abs() - tol).max()
+    assert torch.equal(got, q4.linear_q4(x, w))
 
 
 @pytest.mark.parametrize("rows", [3, 9, 16])
