@@ -26,7 +26,7 @@ using namespace b200;
 
 constexpr int kStage = 256;                    // channels of a stage of codes
 constexpr int kCodeBytes = 128 * kStage / 2;
-constexpr int ERR_Q4_A = 41, ERR_Q4_D = 42;    // status codes: operands or products that never came
+constexpr int ERR_Q4_D = 42;                   // status code: operands that were never used, or products that never came
 
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
