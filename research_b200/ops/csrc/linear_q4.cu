@@ -87,6 +87,17 @@ __global__ void __launch_bounds__(WARPS * 32) linear_q4_few_kernel(const __grid_
   uint4 code[2][KB];
   uint2 pair[2][KB];
   auto at_row = [&](int tile, int m) { return static_cast<long long>(min(tile * 16 + 8 * m + g, p.N - 1)); };
+#pragma unroll
+  for (int m = 0; m < 2; ++m)
+#pragma unroll
+    for (int b = 0; b < KB; ++b) code[m][b] = make_uint4(0, 0, 0, 0), pair[m][b] = make_uint2(0, 0);
+  b200::pdl_launch_dependents();
+  // what runs before may be what writes the weights: they are read after the wait, and only brought into L2 ahead of it
+#pragma unroll
+  for (int m = 0; m < 2; ++m)
+    if (kb0 < blocks)
+      asm volatile("prefetch.global.L2 [%0];" ::"l"(p.codes + at_row(first, m) * row_bytes + (4ll * kb0 + t) * 16));
+  b200::pdl_wait();
   auto load_w = [&](int tile) {
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
@@ -101,17 +112,6 @@ __global__ void __launch_bounds__(WARPS * 32) linear_q4_few_kernel(const __grid_
         }
     }
   };
-#pragma unroll
-  for (int m = 0; m < 2; ++m)
-#pragma unroll
-    for (int b = 0; b < KB; ++b) code[m][b] = make_uint4(0, 0, 0, 0), pair[m][b] = make_uint2(0, 0);
-  b200::pdl_launch_dependents();
-  // what runs before may be what writes the weights: they are read after the wait, and only brought into L2 ahead of it
-#pragma unroll
-  for (int m = 0; m < 2; ++m)
-    if (kb0 < blocks)
-      asm volatile("prefetch.global.L2 [%0];" ::"l"(p.codes + at_row(first, m) * row_bytes + (4ll * kb0 + t) * 16));
-  b200::pdl_wait();
   if (first < tiles) load_w(first);
 
   // x as the column operand: column g is row 8 c + g of x; channels of this lane's words
