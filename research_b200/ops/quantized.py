@@ -216,8 +216,9 @@ def _check_pools(what: str, k_pool: Q4Rows, v_pool: Q4Rows, B: int, Hkv: int | N
 
 
 def _per_sequence(what: str, name: str, t: torch.Tensor | None, B: int, like: torch.Tensor) -> torch.Tensor | None:
-    if t is None:
-        return None
+    if t is None or (t.dtype is torch.int32 and t.dim() == 1 and t.shape[0] == B and t.is_contiguous()
+                     and t.get_device() == like.get_device()):
+        return t
     if t.dim() != 1 or t.shape[0] != B or t.dtype not in (torch.int32, torch.int64):
         raise KernelError(f"{what}: {name} is an int32 or int64 tensor [{B}], got {tuple(t.shape)} {t.dtype}")
     if t.get_device() != like.get_device():
@@ -341,16 +342,16 @@ def kv_read_paged_q4(k_pool: Q4Rows, v_pool: Q4Rows, rows: int, start: torch.Ten
     _head_dim(what, D)
     if dtype != torch.bfloat16:
         raise KernelError(f"{what} writes bf16 on a CUDA device, got {dtype}")
-    out = k_pool.affine.new_empty(2, B, rows, Hkv, D)
-    if out.numel() and pages * page_rows:
-        with _on(out):
+    k, v = k_pool.affine.new_empty(B, rows, Hkv, D), v_pool.affine.new_empty(B, rows, Hkv, D)
+    if k.numel() and pages * page_rows:
+        with _on(k):
             native._check((native._lib or native.load()).b200_q4_kv_read(
-                out.data_ptr(), out.data_ptr() + out.numel(), k_pool.codes.data_ptr(), k_pool.affine.data_ptr(),
+                k.data_ptr(), v.data_ptr(), k_pool.codes.data_ptr(), k_pool.affine.data_ptr(),
                 v_pool.codes.data_ptr(), v_pool.affine.data_ptr(), native._ptr(start), B, rows, Hkv, D, pages,
                 page_rows, native._stream()), "b200_q4_kv_read")
     else:
-        out.zero_()
-    return out.unbind(0)
+        k.zero_(), v.zero_()
+    return k, v
 
 
 def decode_attention_paged_q4(q: torch.Tensor, k_pool: Q4Rows, v_pool: Q4Rows, lengths: torch.Tensor,
@@ -392,7 +393,7 @@ def decode_attention_paged_q4(q: torch.Tensor, k_pool: Q4Rows, v_pool: Q4Rows, l
     with _on(q):
         runs = _attention_runs(B, Hkv, pages * page_rows, q.get_device())
         slots = (runs + B * Hkv) * (Hq // Hkv)
-        parts = torch.empty(slots * (D + 2), dtype=torch.float32, device=q.device)
+        parts = q.new_empty(slots * (D + 2), dtype=torch.float32)
         native._check(lib.b200_q4_decode_attn(
             q.data_ptr(), per_row, k_pool.codes.data_ptr(), k_pool.affine.data_ptr(), v_pool.codes.data_ptr(),
             v_pool.affine.data_ptr(), lengths.data_ptr(), native._ptr(lo), out.data_ptr(), parts.data_ptr(),
