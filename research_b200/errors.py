@@ -15,3 +15,7 @@ class ContractError(JaxtitanError):
 
 class KernelError(ContractError):
     """A native kernel launcher refused its arguments or a device-side bounded wait ran out."""
+
+
+class CacheCapacityError(ContractError, IndexError):
+    """A position is outside the rows that a K/V cache has."""

@@ -15,7 +15,7 @@ from dataclasses import dataclass
 
 import torch
 
-from research_b200.errors import ContractError
+from research_b200.errors import CacheCapacityError, ContractError
 from research_b200.ops import functional as Fn
 from research_b200.ops import quantized
 
@@ -50,6 +50,13 @@ class PagedKVCache:
             yield self
         finally:
             self._from_zero = before
+
+    def require_rows(self, first: int, end: int) -> None:
+        """Refuse a write of rows ``first .. end - 1`` that leaves the cache.  For a step (one token per sequence) the caller
+        asks, who has the position on the host; on a CUDA device the layers could only wait for it."""
+
+        if first < 0 or end > self.max_len:
+            raise CacheCapacityError(f"rows {first} .. {end - 1} are not all in a cache of {self.max_len} rows")
 
     def _pages(self, pool: torch.Tensor, layer: int) -> torch.Tensor:
         # with the identity page table, sequence b owns pages [b * pages_per_seq, (b + 1) * pages_per_seq)
@@ -163,6 +170,8 @@ class QuantizedKVCache(PagedKVCache):
             step = getattr(self, "_step_positions", None)       # made by the first layer, reused by the others
             if layer == 0 or step is None or step[0] is not positions:
                 pos = positions[:, 0].to(torch.int32).contiguous()
+                if not positions.is_cuda and positions.numel():
+                    self.require_rows(int(positions.min()), int(positions.max()) + 1)
                 step = self._step_positions = (positions, pos, pos + 1, {None: None})
             _, pos, lengths, bounds = step
             if window not in bounds:
@@ -172,16 +181,16 @@ class QuantizedKVCache(PagedKVCache):
         first = positions[:, :1]
         in_a_row = self._from_zero or bool(
             (positions == first + torch.arange(T, device=q.device, dtype=positions.dtype)).all())
-        if not in_a_row:
-            for t in range(T):                                  # a position given twice keeps its last row
-                write(k[:, t:t + 1], v[:, t:t + 1], kp, vp, positions[:, t])
-        elif self._from_zero or not bool(first.any()):
+        if in_a_row and (self._from_zero or not bool(first.any())):
             write(k, v, kp, vp)
             return self._attend_rows(q, k, v, 0, window, positions, native_ok)
-        else:
+        start, end = int(positions.min()), int(positions.max()) + 1
+        self.require_rows(start, end)
+        if in_a_row:
             write(k, v, kp, vp, positions[:, 0])
-        start = int(first.min())
-        end = int(positions.max()) + 1
+        else:
+            for t in range(T):                                  # a position given twice keeps its last row
+                write(k[:, t:t + 1], v[:, t:t + 1], kp, vp, positions[:, t])
         keys, vals = quantized.kv_read_paged_q4(kp, vp, end) if native_ok else quantized.kv_read_paged_q4_reference(
             kp, vp, end, channels=D, dtype=q.dtype)
         if in_a_row and start + T == end:                       # every sequence at the same place
@@ -273,6 +282,12 @@ def sample_next_token(logits: torch.Tensor, *, temperature: float, top_k: int | 
     return token, logp.gather(1, token[:, None])[:, 0]
 
 
+def _require_rows(cache, position: int) -> None:
+    # any object that stores rows and attends over them will do
+    if isinstance(cache, PagedKVCache):
+        cache.require_rows(position, position + 1)
+
+
 class GraphedDecodeStep:
     """One decode step (embedding -> layers -> logits of the new token) captured in a CUDA graph.
 
@@ -284,6 +299,8 @@ class GraphedDecodeStep:
     def __init__(self, model, cache: PagedKVCache, first_token: torch.Tensor, first_position: int):
         B = first_token.shape[0]
         dev = first_token.device
+        self.cache = cache
+        _require_rows(cache, int(first_position))
         self.token = first_token.reshape(B, 1).to(torch.int32).clone()
         self.position = torch.full((B, 1), int(first_position), device=dev, dtype=torch.int32)
         side = torch.cuda.Stream(device=dev)
@@ -297,6 +314,7 @@ class GraphedDecodeStep:
             self.logits = model.run_with_cache(self.token, self.position, cache, last_only=True)[:, -1]
 
     def __call__(self, token: torch.Tensor, position: int) -> torch.Tensor:
+        _require_rows(self.cache, int(position))
         self.token.copy_(token.reshape(-1, 1))
         self.position.fill_(int(position))
         self.graph.replay()
@@ -386,9 +404,11 @@ def prefill(model, prompt_ids: torch.Tensor, cache: PagedKVCache) -> torch.Tenso
 
 @torch.no_grad()
 def decode_one(model, token: torch.Tensor, position: int, cache: PagedKVCache) -> torch.Tensor:
-    """One decode step: ``token`` ``[B]`` at ``position`` -> next-token logits ``[B, V]``; the cache grows by one."""
+    """One decode step: ``token`` ``[B]`` at ``position`` -> next-token logits ``[B, V]``; the cache grows by one.  A position
+    that the cache has no row for is refused (:class:`research_b200.errors.CacheCapacityError`)."""
 
     B = token.shape[0]
+    _require_rows(cache, int(position))
     device = next(model.parameters()).device
     pos = torch.full((B, 1), int(position), device=device, dtype=torch.int32)
     logits = model.run_with_cache(token.to(device=device, dtype=torch.int32)[:, None], pos, cache, last_only=True)
