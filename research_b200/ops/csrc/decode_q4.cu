@@ -701,9 +701,8 @@ extern "C" int b200_q4_decode_attn(const void* q, long long q_batch, const void*
       runs < 1 || (long long)pages * page_rows > 0x7fffff00ll || (long long)B * Hq > 0x7fffffffll || !part_o || !part_ml)
     return b200host::RC_BAD_SHAPE;
   if (runs > kBlocks * b200host::sm_count() * kWarps) return b200host::RC_BAD_SHAPE;
-  if ((q_batch & 7) || ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k_codes) |
-                         reinterpret_cast<uintptr_t>(k_affine) | reinterpret_cast<uintptr_t>(v_codes) |
-                         reinterpret_cast<uintptr_t>(v_affine) | reinterpret_cast<uintptr_t>(out)) & 15))
+  if ((q_batch & 7) || ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & 15) ||
+      !rows_aligned(k_codes, k_affine, D) || !rows_aligned(v_codes, v_affine, D))
     return b200host::RC_BAD_ALIGNMENT;
   AttnParams p{(const __nv_bfloat16*)q, q_batch, (const uint8_t*)k_codes, (const uint8_t*)k_affine,
                (const uint8_t*)v_codes, (const uint8_t*)v_affine, (const int*)lengths, (const int*)lo,

@@ -627,9 +627,9 @@ extern "C" int b200_q4_linear(const void* x, long long ldx, const void* codes, c
   using namespace b200host;
   if (rows <= 0 || rows > (1 << 24) || N <= 0 || K <= 0 || K > (1 << 30) || !status) return RC_BAD_SHAPE;
   if (cluster != 1 && cluster != 2 && cluster != 4 && cluster != 8) return RC_BAD_SHAPE;
-  if ((reinterpret_cast<uintptr_t>(codes) | reinterpret_cast<uintptr_t>(affine)) & 15) return RC_BAD_ALIGNMENT;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   const int width = row_width(K);
+  if (!rows_aligned(codes, affine, width)) return RC_BAD_ALIGNMENT;
   if (width == 64)
     return static_cast<int>(launch_kernel(linear_q4_narrow_kernel, dim3((N + 3) / 4, (rows + 7) / 8), dim3(128), 0, s,
                                           pdl_enabled() != 0, (const __nv_bfloat16*)x, ldx, (const uint32_t*)codes,

@@ -249,9 +249,7 @@ extern "C" int b200_q4_kv_write(const void* k, const void* v, long long k_row, l
   if ((k_row | k_batch | v_row | v_batch) & 7) return b200host::RC_BAD_ALIGNMENT;
   if (k_row < 0 || v_row < 0 || k_row > 0x7fffffff || v_row > 0x7fffffff) return b200host::RC_TOO_LARGE;
   if ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15) return b200host::RC_BAD_ALIGNMENT;
-  if ((reinterpret_cast<uintptr_t>(k_codes) | reinterpret_cast<uintptr_t>(v_codes) |
-       reinterpret_cast<uintptr_t>(k_affine) | reinterpret_cast<uintptr_t>(v_affine)) & 15)
-    return b200host::RC_BAD_ALIGNMENT;
+  if (!rows_aligned(k_codes, k_affine, D) || !rows_aligned(v_codes, v_affine, D)) return b200host::RC_BAD_ALIGNMENT;
   KvParams p{{(const __nv_bfloat16*)k, (const __nv_bfloat16*)v}, {nullptr, nullptr},
              {(uint32_t*)k_codes, (uint32_t*)v_codes}, {(uint32_t*)k_affine, (uint32_t*)v_affine}, (const int*)start,
              {k_batch, v_batch}, {(int)k_row, (int)v_row}, T, Hkv, pages, page_rows, 0, {}, {}, {}};
@@ -263,10 +261,8 @@ extern "C" int b200_q4_kv_read(void* k, void* v, const void* k_codes, const void
                                const void* v_affine, const void* start, int B, int T, int Hkv, int D, int pages,
                                int page_rows, void* stream) {
   if (!kv_shape_ok(B, T, Hkv, D, pages, page_rows)) return b200host::RC_BAD_SHAPE;
-  if ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) | reinterpret_cast<uintptr_t>(k_codes) |
-       reinterpret_cast<uintptr_t>(v_codes) | reinterpret_cast<uintptr_t>(k_affine) |
-       reinterpret_cast<uintptr_t>(v_affine)) & 15)
-    return b200host::RC_BAD_ALIGNMENT;
+  if ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15) return b200host::RC_BAD_ALIGNMENT;
+  if (!rows_aligned(k_codes, k_affine, D) || !rows_aligned(v_codes, v_affine, D)) return b200host::RC_BAD_ALIGNMENT;
   KvParams p{{nullptr, nullptr}, {(__nv_bfloat16*)k, (__nv_bfloat16*)v}, {(uint32_t*)k_codes, (uint32_t*)v_codes},
              {(uint32_t*)k_affine, (uint32_t*)v_affine}, (const int*)start, {0, 0}, {0, 0}, T, Hkv, pages,
              page_rows, 0, {}, {}, {}};
@@ -277,8 +273,8 @@ extern "C" int b200_q4_kv_read(void* k, void* v, const void* k_codes, const void
 extern "C" int b200_q4_quantize_rows(const void* x, long long ldx, void* codes, void* affine, long long rows,
                                      int channels, void* stream) {
   if (rows <= 0 || channels <= 0 || channels > (1 << 30)) return b200host::RC_BAD_SHAPE;
-  if ((reinterpret_cast<uintptr_t>(codes) | reinterpret_cast<uintptr_t>(affine)) & 15) return b200host::RC_BAD_ALIGNMENT;
   const int width = row_width(channels);
+  if (!rows_aligned(codes, affine, width)) return b200host::RC_BAD_ALIGNMENT;
   quantize_rows_q4_kernel<<<blocks_for(rows * (width / 8)), 256, 0, reinterpret_cast<cudaStream_t>(stream)>>>(
       (const __nv_bfloat16*)x, ldx, (uint32_t*)codes, (uint32_t*)affine, rows, channels, width);
   return static_cast<int>(cudaGetLastError());
@@ -288,8 +284,7 @@ extern "C" int b200_q4_quantize_rows(const void* x, long long ldx, void* codes, 
 extern "C" int b200_q4_dequantize_rows(const void* codes, const void* affine, void* out, long long rows, int width,
                                        void* stream) {
   if (rows <= 0 || width <= 0 || (width != 64 && width % 128)) return b200host::RC_BAD_SHAPE;
-  if ((reinterpret_cast<uintptr_t>(codes) | reinterpret_cast<uintptr_t>(affine) | reinterpret_cast<uintptr_t>(out)) & 15)
-    return b200host::RC_BAD_ALIGNMENT;
+  if (!rows_aligned(codes, affine, width) || (reinterpret_cast<uintptr_t>(out) & 15)) return b200host::RC_BAD_ALIGNMENT;
   return static_cast<int>(b200host::launch_kernel(
       dequantize_rows_q4_kernel, dim3(blocks_for(rows * (width / 8))), dim3(256), 0,
       reinterpret_cast<cudaStream_t>(stream), b200host::pdl_enabled() != 0, (const uint32_t*)codes,

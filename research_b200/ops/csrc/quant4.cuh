@@ -17,6 +17,12 @@ constexpr int kGroup = 64;
 
 __host__ __device__ inline int row_width(int channels) { return channels <= 64 ? 64 : (channels + 127) / 128 * 128; }
 
+// Whether codes and pairs lie where the kernels may read them: codes in 16 bytes at a time, pairs in the 4 (rows of 64) or 8
+// that a block has, so that a slice of a larger tensor between any two of its rows will do.
+inline bool rows_aligned(const void* codes, const void* affine, int width) {
+  return (reinterpret_cast<uintptr_t>(codes) & 15) == 0 && (reinterpret_cast<uintptr_t>(affine) & (width == 64 ? 3 : 7)) == 0;
+}
+
 // word of a row of `width` channels -> its first channel
 __device__ __forceinline__ int word_channel(int word, int width) {
   if (width == 64) return word * 8;

@@ -47,3 +47,77 @@ def test_a_piece_past_the_cache_is_refused_before_it_is_written():
         with pytest.raises(CacheCapacityError):
             cache.update_and_attend(0, q, k, v, at, None)
     assert all(torch.equal(a, b) for a, b in zip(held, [t for pool in (cache.k, cache.v) for t in pool]))
+
+
+# ------------------------------------------------------------------------------------------------- addresses
+def _same(a, b):
+    return a.shape == b.shape and bool(((a == b) | (a.isnan() & b.isnan())).all())
+
+
+def _off_16(rows, bytes_off):
+    """The same 4-bit rows with their pairs ``bytes_off`` bytes behind an address of 16 bytes."""
+
+    from research_b200.ops import quantized as q4
+
+    n = bytes_off // 2
+    flat = torch.empty(rows.affine.numel() + 8, dtype=BF16, device="cuda")
+    pairs = flat[n:n + rows.affine.numel()].view(rows.affine.shape)
+    pairs.copy_(rows.affine)
+    assert pairs.data_ptr() % 16 == bytes_off
+    return q4.Q4Rows(rows.codes.clone(), pairs)
+
+
+@pytest.mark.parametrize("D,off", [(64, 4), (64, 8), (64, 12), (128, 8)])
+def test_pairs_of_a_cache_start_anywhere_that_a_row_may(D, off):
+    """The cache calls read a row's pairs, 4 bytes (heads of 64) or 8 (of 128), at a time."""
+
+    from research_b200.ops import quantized as q4
+
+    g = torch.Generator(device="cuda").manual_seed(D + off)
+    B, pages, H, ps, T = 2, 3, 3, 25, 40
+    k, v = (torch.randn(B, T, H, D, generator=g, device="cuda").to(BF16) for _ in range(2))
+    q = torch.randn(B, 2 * H, D, generator=g, device="cuda").to(BF16)
+    plain = [q4.empty_rows(B, pages, H, ps, channels=D, device="cuda") for _ in range(2)]
+    odd = [_off_16(pool, off) for pool in plain]
+    start = torch.tensor([0, 31], device="cuda", dtype=torch.int32)
+    for pools in (plain, odd):
+        q4.kv_write_paged_q4(k, v, *pools, start)
+    for a, b in zip(plain, odd):
+        assert torch.equal(a.codes, b.codes) and torch.equal(a.affine, b.affine)
+    for a, b in zip(q4.kv_read_paged_q4(*plain, T, start), q4.kv_read_paged_q4(*odd, T, start)):
+        assert torch.equal(a, b)
+    assert torch.equal(q4.decode_attention_paged_q4(q, *plain, start + T, start), q4.decode_attention_paged_q4(q, *odd, start + T, start))
+    assert torch.equal(q4.dequantize_rows_q4(plain[0], D), q4.dequantize_rows_q4(odd[0], D))
+
+
+@pytest.mark.parametrize("K,off", [(50, 4), (64, 12), (100, 8), (300, 8), (2048, 8)])
+@pytest.mark.parametrize("rows", [1, 12, 40, 90, 2000])
+def test_pairs_of_weights_start_anywhere_that_a_row_may(K, off, rows):
+    from research_b200.ops import quantized as q4
+
+    g = torch.Generator(device="cuda").manual_seed(K + rows)
+    w = q4.quantize_rows_q4(torch.randn(203, K, generator=g, device="cuda"))
+    x = torch.randn(rows, K, generator=g, device="cuda").to(BF16)
+    want = q4.linear_q4(x, w)
+    assert torch.equal(q4.linear_q4(x, _off_16(w, off)), want)
+    # weight rows of a larger matrix
+    part = q4.Q4Rows(w.codes[1:], w.affine[1:])
+    assert torch.equal(q4.linear_q4(x, part), q4.linear_q4(x, q4.Q4Rows(*(t.clone() for t in part))))
+    assert _same(q4.dequantize_rows_q4(part, K), q4.dequantize_rows_q4(w, K)[1:])
+
+
+@pytest.mark.parametrize("D,H,page,pages", [(64, 2, 25, 1), (64, 1, 7, 3), (64, 3, 1, 5), (128, 1, 5, 1)])
+def test_layers_of_a_cache_of_odd_pages(D, H, page, pages):
+    """Each layer of a cache is a slice; the second one's pairs start where the first one's end."""
+
+    from research_b200.infer import QuantizedKVCache
+
+    caches = [QuantizedKVCache(layers=layers, batch=1, max_len=page * pages, kv_heads=H, head_dim=D, page_size=page,
+                               dtype=BF16, device=torch.device("cuda")) for layers in (3, 1)]
+    end = min(page * pages, 5)
+    for first, T in ((0, end - 1), (end - 1, 1)):
+        at = (torch.arange(T, dtype=torch.int32, device="cuda") + first)[None]
+        q, k, v = (torch.randn(1, T, h, D, device="cuda", dtype=BF16) for h in (2 * H, H, H))
+        want = caches[1].update_and_attend(0, q, k, v, at, None)
+        for layer in range(3):
+            assert torch.equal(caches[0].update_and_attend(layer, q, k, v, at, None), want)
