@@ -281,13 +281,20 @@ def _expand(rows: Q4Rows) -> torch.Tensor:
 # --------------------------------------------------------------------------------------------------
 # cache
 # --------------------------------------------------------------------------------------------------
+def _copied(t: torch.Tensor) -> torch.Tensor:
+    """A dense copy on an address of its own, also of what is dense already."""
+
+    return t.clone(memory_format=torch.contiguous_format)
+
+
 def _heads_apart(t: torch.Tensor, Hkv: int, D: int) -> tuple[torch.Tensor, int, int]:
-    """``t [B, T, Hkv, D]`` as the kernel reads it (a copy where heads are not D apart), with the strides of rows and sequences."""
+    """``t [B, T, Hkv, D]`` as the kernel reads it (a copy where heads are not D apart or rows off 16 bytes), with the strides
+    of rows and sequences."""
 
     batch, row, head, one = t.stride()
     if one == 1 and head == D and row % 8 == 0 and batch % 8 == 0 and t.data_ptr() % 16 == 0:
         return t, row, batch
-    return t.contiguous(), Hkv * D, t.shape[1] * Hkv * D
+    return _copied(t), Hkv * D, t.shape[1] * Hkv * D
 
 
 def kv_write_paged_q4(k: torch.Tensor, v: torch.Tensor, k_pool: Q4Rows, v_pool: Q4Rows,
@@ -383,7 +390,7 @@ def decode_attention_paged_q4(q: torch.Tensor, k_pool: Q4Rows, v_pool: Q4Rows, l
                           f"{q.dtype}, Hq={Hq}, Hkv={Hkv}")
     per_row, per_head, one = q.stride()
     if one != 1 or per_head != D or per_row % 8 or q.data_ptr() % 16:
-        q, per_row = q.contiguous(), Hq * D
+        q, per_row = _copied(q), Hq * D
     out = q.new_empty(B, Hq * D)
     if out.numel() == 0:
         return out
@@ -469,7 +476,7 @@ def _rows_on_16_bytes(x: torch.Tensor) -> torch.Tensor:
 
     if x.stride(1) == 1 and x.stride(0) % 8 == 0 and x.stride(0) >= x.shape[1] and x.data_ptr() % 16 == 0:
         return x
-    return F.pad(x, (0, -x.shape[1] % 8))[:, :x.shape[1]] if x.shape[1] % 8 else x.clone(memory_format=torch.contiguous_format)
+    return F.pad(x, (0, -x.shape[1] % 8))[:, :x.shape[1]] if x.shape[1] % 8 else _copied(x)
 
 
 @functools.lru_cache(maxsize=4096)

@@ -121,3 +121,20 @@ def test_layers_of_a_cache_of_odd_pages(D, H, page, pages):
         want = caches[1].update_and_attend(0, q, k, v, at, None)
         for layer in range(3):
             assert torch.equal(caches[0].update_and_attend(layer, q, k, v, at, None), want)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_dense_keys_values_and_queries_start_on_any_address(D):
+    from research_b200.ops import quantized as q4
+
+    B, T, H = 2, 7, 2
+    dense = lambda n, *shape: torch.randn(n + 1, device="cuda").to(BF16)[1:].view(shape)  # noqa: E731
+    k, v = (dense(B * T * H * D, B, T, H, D) for _ in range(2))
+    q = dense(B * 4 * D, B, 4, D)
+    assert all(t.is_contiguous() and t.data_ptr() % 16 == 2 for t in (k, v, q))
+    pools, same = ([q4.empty_rows(B, 2, H, 5, channels=D, device="cuda") for _ in range(2)] for _ in range(2))
+    q4.kv_write_paged_q4(k, v, *pools)
+    q4.kv_write_paged_q4(k.clone(), v.clone(), *same)
+    assert all(torch.equal(a, b) for x, y in zip(pools, same) for a, b in zip(x, y))
+    n = torch.tensor([7, 3], device="cuda")
+    assert torch.equal(q4.decode_attention_paged_q4(q, *pools, n), q4.decode_attention_paged_q4(q.clone(), *pools, n))
