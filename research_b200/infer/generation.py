@@ -15,7 +15,7 @@ from dataclasses import dataclass
 
 import torch
 
-from research_b200.errors import CacheCapacityError, ContractError
+from research_b200.errors import CacheCapacityError, ContractError, KernelError
 from research_b200.ops import functional as Fn
 from research_b200.ops import quantized
 
@@ -157,9 +157,12 @@ class QuantizedKVCache(PagedKVCache):
 
     def update_and_attend(self, layer: int, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
                           positions: torch.Tensor, window: int | None) -> torch.Tensor:
-        """Write k, v at ``positions`` ([B,T]) and attend q over everything written so far (causal)."""
+        """Write k, v at ``positions`` ([B,T]) and attend q over everything written so far (causal).  A single prompt (B = 1,
+        from row 0 on) goes to every sequence of the cache."""
 
         B, T, Hq, D = q.shape
+        if B != self.batch and (B != 1 or T == 1):
+            raise KernelError(f"a cache of {self.batch} sequences does not take rows of {B}")
         kp, vp = self._pages(self.k, layer), self._pages(self.v, layer)
         native_ok = q.is_cuda and q.dtype == torch.bfloat16 and D in (64, 128) and Hq <= 8 * k.shape[2]
         # on a CUDA device the restatements take what the kernels do not: other types, head sizes and head counts
@@ -182,8 +185,10 @@ class QuantizedKVCache(PagedKVCache):
         in_a_row = self._from_zero or bool(
             (positions == first + torch.arange(T, device=q.device, dtype=positions.dtype)).all())
         if in_a_row and (self._from_zero or not bool(first.any())):
-            write(k, v, kp, vp)
+            write(k.expand(self.batch, -1, -1, -1), v.expand(self.batch, -1, -1, -1), kp, vp)
             return self._attend_rows(q, k, v, 0, window, positions, native_ok)
+        if B != self.batch:
+            raise KernelError(f"a cache of {self.batch} sequences takes a single prompt from row 0 on only")
         start, end = int(positions.min()), int(positions.max()) + 1
         self.require_rows(start, end)
         if in_a_row:

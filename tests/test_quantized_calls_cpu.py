@@ -3,8 +3,10 @@
 import pytest
 import torch
 
-from research_b200.infer.generation import decode_one, init_kv_cache, prefill
-from tests.test_quantized_generation_cpu import _model
+from research_b200.errors import KernelError
+from research_b200.infer.generation import QuantizedKVCache, decode_one, init_kv_cache, prefill
+from research_b200.ops import quantized as q4
+from tests.test_quantized_generation_cpu import _cache, _model, _rows
 
 
 # ------------------------------------------------------------------------------------------------- capacity
@@ -39,3 +41,25 @@ def test_positions_that_the_cache_does_not_have_are_refused_before_anything_is_w
     for positions in ([[6, 7]] * 2, [[7], [7]]):
         at = torch.tensor(positions, dtype=torch.int32)
         assert torch.isfinite(cache.update_and_attend(0, *tokens(at.shape[1]), at, None)).all()
+
+
+# ------------------------------------------------------------------------------------------------- one prompt for all
+@pytest.mark.parametrize("T", [2, 5, 11])
+def test_one_prompt_for_every_sequence_of_a_cache(T):
+    """As in a 16-bit cache on the GPU: a single prompt goes to all sequences; any other number that is not the cache's is refused."""
+
+    torch.manual_seed(T)
+    q, k, v = (torch.randn(1, T, h, 16) for h in (4, 2, 2))
+    pos = torch.arange(T, dtype=torch.int32)[None]
+    cache, alone = _cache(QuantizedKVCache, batch=3, layers=2), _cache(QuantizedKVCache, batch=1)
+    assert torch.equal(cache.update_and_attend(1, q, k, v, pos, None), alone.update_and_attend(0, q, k, v, pos, None))
+    for pool, x in ((cache.k, k), (cache.v, v)):
+        held = q4.dequantize_rows_q4(q4.quantize_rows_q4(x), 16, torch.float32)
+        assert torch.equal(_rows(pool, 1, 3, T, 16), held.expand(3, T, 2, 16))
+        assert not pool.codes[0].any() and not pool.affine[0].any()
+    before = [t.clone() for pool in (cache.k, cache.v) for t in pool]
+    for n, at in ((2, pos), (4, pos), (1, pos + 1), (2, pos[:, :1]), (1, pos[:, :1])):
+        t = at.shape[1]
+        with pytest.raises(KernelError, match="3 sequences"):
+            cache.update_and_attend(1, *(x[:, :t].expand(n, t, *x.shape[2:]) for x in (q, k, v)), at.expand(n, t).contiguous(), None)
+    assert all(torch.equal(a, b) for a, b in zip(before, [t for pool in (cache.k, cache.v) for t in pool]))

@@ -138,3 +138,32 @@ def test_dense_keys_values_and_queries_start_on_any_address(D):
     assert all(torch.equal(a, b) for x, y in zip(pools, same) for a, b in zip(x, y))
     n = torch.tensor([7, 3], device="cuda")
     assert torch.equal(q4.decode_attention_paged_q4(q, *pools, n), q4.decode_attention_paged_q4(q.clone(), *pools, n))
+
+
+# ------------------------------------------------------------------------------------------------- one prompt for all
+@pytest.mark.parametrize("dtype,D", [(BF16, 64), (BF16, 128), (torch.float32, 64)])
+def test_one_prompt_for_every_sequence_of_a_cache(dtype, D):
+    from research_b200.errors import KernelError
+    from research_b200.infer import QuantizedKVCache
+    from research_b200.ops import quantized as q4
+
+    T = 133
+    cache = QuantizedKVCache(layers=2, batch=3, max_len=T + 5, kv_heads=2, head_dim=D, page_size=24, dtype=dtype,
+                             device=torch.device("cuda"))
+    q, k, v = (torch.randn(1, T, h, D, device="cuda", dtype=dtype) for h in (4, 2, 2))
+    pos = torch.arange(T, device="cuda", dtype=torch.int32)[None]
+    with cache.prompt():
+        got = cache.update_and_attend(1, q, k, v, pos, None)
+    alone = QuantizedKVCache(layers=1, batch=1, max_len=T + 5, kv_heads=2, head_dim=D, page_size=24, dtype=dtype,
+                             device=torch.device("cuda"))
+    assert torch.equal(got, alone.update_and_attend(0, q, k, v, pos, None))
+    for pool, x in ((cache.k, k), (cache.v, v)):
+        held = q4.quantize_rows_q4(x)
+        at = torch.arange(T, device="cuda")
+        pages = cache._pages(pool, 1)
+        assert torch.equal(pages.codes[:, at // 24, :, at % 24].transpose(0, 1), held.codes.expand(3, -1, -1, -1))
+        assert torch.equal(pages.affine[:, at // 24, :, at % 24].transpose(0, 1), held.affine.expand(3, -1, -1, -1, -1))
+    for n, at in ((2, pos), (4, pos), (1, pos[:, :9] + 1), (2, pos[:, :1])):
+        t = at.shape[1]
+        with pytest.raises(KernelError, match="3 sequences"):
+            cache.update_and_attend(1, *(x[:, :t].expand(n, t, *x.shape[2:]) for x in (q, k, v)), at.expand(n, t).contiguous(), None)
