@@ -153,7 +153,7 @@ class QuantizedKVCache(PagedKVCache):
         return quantized.empty_rows(*shape[:-1], channels=shape[-1], device=device)
 
     def _pages(self, pool, layer: int):
-        return quantized.Q4Rows(*(t[layer].view(self.batch, self.pages_per_seq, *t.shape[2:]) for t in pool))
+        return quantized.Q4Rows(*(t[layer].view(self.batch, self.pages_per_seq, *t.shape[2:]) for t in pool), pool.channels)
 
     def update_and_attend(self, layer: int, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
                           positions: torch.Tensor, window: int | None) -> torch.Tensor:

@@ -31,11 +31,25 @@ from research_b200.ops import native
 GROUP = 64
 
 
-class Q4Rows(NamedTuple):
-    """Rows in 4 bits: ``codes`` uint8 ``[..., W / 2]``, ``affine`` bf16 ``[..., W / 64, 2]`` (scale, least value)."""
-
+class _CodesAndPairs(NamedTuple):
     codes: torch.Tensor
     affine: torch.Tensor
+
+
+class Q4Rows(_CodesAndPairs):
+    """Rows in 4 bits: ``codes`` uint8 ``[..., W / 2]``, ``affine`` bf16 ``[..., W / 64, 2]`` (scale, least value).
+
+    ``channels`` is how many of the W a row has, where that is known: :func:`quantize_rows_q4` and :func:`empty_rows` say so,
+    and a call with rows of another number is refused.  Rows that are put together from tensors without it (None) are only
+    held against their width."""
+
+    channels: int | None = None
+
+    def __new__(cls, codes: torch.Tensor, affine: torch.Tensor, channels: int | None = None):
+        self = tuple.__new__(cls, (codes, affine))
+        if channels is not None:
+            self.channels = channels
+        return self
 
 
 def row_width(channels: int) -> int:
@@ -49,7 +63,7 @@ def empty_rows(*shape: int, channels: int, device=None) -> Q4Rows:
 
     width = row_width(channels)
     return Q4Rows(torch.zeros(*shape, width // 2, dtype=torch.uint8, device=device),
-                  torch.zeros(*shape, width // GROUP, 2, dtype=torch.bfloat16, device=device))
+                  torch.zeros(*shape, width // GROUP, 2, dtype=torch.bfloat16, device=device), channels)
 
 
 # --------------------------------------------------------------------------------------------------
@@ -81,7 +95,7 @@ def quantize_rows_reference(x: torch.Tensor) -> Q4Rows:
     words = n.unflatten(-2, (-1, pair)).unflatten(-1, (8, 8)).transpose(-3, -2)
     nibbles = words[..., [_NIBBLE.index(k) for k in range(8)]]
     return Q4Rows((nibbles[..., 0::2] | (nibbles[..., 1::2] << 4)).flatten(-4),
-                  torch.cat([s, z], dim=-1).to(torch.bfloat16))
+                  torch.cat([s, z], dim=-1).to(torch.bfloat16), channels)
 
 
 def dequantize_rows_reference(rows: Q4Rows, channels: int, dtype: torch.dtype = torch.float32) -> torch.Tensor:
@@ -145,6 +159,7 @@ def decode_attention_paged_q4_reference(q: torch.Tensor, k_pool: Q4Rows, v_pool:
 
 
 def linear_q4_reference(x: torch.Tensor, w: Q4Rows) -> torch.Tensor:
+    _check_channels("linear_q4", w, x.shape[-1])
     return F.linear(x.float(), dequantize_rows_reference(w, x.shape[-1])).to(x.dtype)
 
 
@@ -173,7 +188,17 @@ def _on(t: torch.Tensor):
     return _SAME if t.get_device() == torch._C._cuda_getDevice() else torch.cuda.device(t.device)
 
 
+def _check_channels(what: str, rows: Q4Rows, channels: int) -> None:
+    if rows.channels is not None and rows.channels != channels:
+        raise KernelError(f"{what}: rows of {channels} channels do not go with 4-bit rows of {rows.channels} channels")
+
+
 def _check_rows(what: str, rows: Q4Rows, channels: int) -> None:
+    _check_channels(what, rows, channels)
+    _check_width(what, rows, channels)
+
+
+def _check_width(what: str, rows: Q4Rows, channels: int) -> None:
     width = row_width(channels)
     codes, affine = rows
     *shape, half = codes.shape
@@ -202,7 +227,7 @@ def _check_pools(what: str, k_pool: Q4Rows, v_pool: Q4Rows, B: int, Hkv: int | N
             if pool.codes.dim() != 5:
                 raise KernelError(f"{what}: a cache has codes [B, pages, Hkv, page_rows, D / 2], got "
                                   f"{tuple(pool.codes.shape)}")
-            _check_rows(what, pool, D)
+            _check_width(what, pool, D)
         if shape != vc.shape:
             raise KernelError(f"{what}: the K and the V cache must have one shape, got {tuple(shape)} and {tuple(vc.shape)}")
         _same_device(what, kc, vc)
@@ -253,7 +278,7 @@ def quantize_rows_q4(x: torch.Tensor) -> Q4Rows:
             native._check((native._lib or native.load()).b200_q4_quantize_rows(
                 x2.data_ptr(), x2.stride(0), codes.data_ptr(), affine.data_ptr(), x2.shape[0], x2.shape[1],
                 native._stream()), "b200_q4_quantize_rows")
-    return Q4Rows(codes, affine)
+    return Q4Rows(codes, affine, x.shape[-1])
 
 
 def dequantize_rows_q4(rows: Q4Rows, channels: int, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
@@ -309,6 +334,8 @@ def kv_write_paged_q4(k: torch.Tensor, v: torch.Tensor, k_pool: Q4Rows, v_pool: 
         raise KernelError(f"{what}: k and v are [B, T, Hkv, D] of one shape and type, got {tuple(k.shape)} {k.dtype} and "
                           f"{tuple(v.shape)} {v.dtype}")
     B, T, Hkv, D = k.shape
+    _check_channels(what, k_pool, D)
+    _check_channels(what, v_pool, D)
     pages, _, page_rows = _check_pools(what, k_pool, v_pool, B, Hkv, D)
     _same_device(what, k, v, k_pool.codes)
     start = _per_sequence(what, "start", start, B, k)
@@ -339,6 +366,9 @@ def kv_read_paged_q4(k_pool: Q4Rows, v_pool: Q4Rows, rows: int, start: torch.Ten
 
     what = "kv_read_paged_q4"
     D = k_pool.codes.shape[-1] * 2 if head_dim is None else head_dim
+    if head_dim is not None:                            # else all that is stored, padding too
+        _check_channels(what, k_pool, D)
+        _check_channels(what, v_pool, D)
     B = k_pool.codes.shape[0]
     pages, Hkv, page_rows = _check_pools(what, k_pool, v_pool, B, None, D)
     start = _per_sequence(what, "start", start, B, k_pool.codes)
@@ -371,6 +401,8 @@ def decode_attention_paged_q4(q: torch.Tensor, k_pool: Q4Rows, v_pool: Q4Rows, l
     if q.dim() != 3 or not q.is_floating_point():
         raise KernelError(f"{what}: q is [B, Hq, D], got {tuple(q.shape)} {q.dtype}")
     B, Hq, D = q.shape
+    _check_channels(what, k_pool, D)
+    _check_channels(what, v_pool, D)
     pages, Hkv, page_rows = _check_pools(what, k_pool, v_pool, B, None, D)
     if Hkv == 0 or Hq % Hkv:
         raise KernelError(f"{what}: {Hq} query heads do not share {Hkv} K/V heads evenly")

@@ -63,3 +63,53 @@ def test_one_prompt_for_every_sequence_of_a_cache(T):
         with pytest.raises(KernelError, match="3 sequences"):
             cache.update_and_attend(1, *(x[:, :t].expand(n, t, *x.shape[2:]) for x in (q, k, v)), at.expand(n, t).contiguous(), None)
     assert all(torch.equal(a, b) for a, b in zip(before, [t for pool in (cache.k, cache.v) for t in pool]))
+
+
+# ------------------------------------------------------------------------------------------------- channels
+def test_rows_of_other_channels_of_the_same_width_are_refused():
+    """100 and 120 channels are both stored as 128; rows know which they are."""
+
+    w = q4.quantize_rows_q4(torch.randn(4, 120))
+    x = torch.randn(2, 100)
+    refused = lambda: pytest.raises(KernelError, match="rows of 100 channels")  # noqa: E731
+    with refused():
+        q4.linear_q4(x, w)
+    with refused():
+        q4.linear_q4_reference(x, w)
+    with refused():
+        q4.dequantize_rows_q4(w, 100)
+    assert q4.linear_q4(torch.randn(2, 120), w).shape == (2, 4)
+    pools = [q4.empty_rows(2, 3, 2, 4, channels=120) for _ in range(2)]
+    right = [q4.empty_rows(2, 3, 2, 4, channels=100) for _ in range(2)]
+    rows, n = torch.randn(2, 5, 2, 100), torch.ones(2, dtype=torch.int32)
+    for k_pool, v_pool in ((pools[0], pools[1]), (right[0], pools[1]), (pools[0], right[1])):
+        with refused():
+            q4.kv_write_paged_q4(rows, rows, k_pool, v_pool)
+        with refused():
+            q4.kv_read_paged_q4(k_pool, v_pool, 1, head_dim=100)
+        with refused():
+            q4.decode_attention_paged_q4(rows[:, 0], k_pool, v_pool, n)
+    assert not any(t.any() for pool in (*pools, *right) for t in pool)
+    q4.kv_write_paged_q4(rows, rows, *right)
+    back = q4.kv_read_paged_q4(*right, 5, head_dim=100, dtype=torch.float32)[0]
+    assert torch.equal(back, q4.dequantize_rows_q4(q4.quantize_rows_q4(rows), 100, torch.float32))
+    assert q4.kv_read_paged_q4(*right, 5)[0].shape == (2, 5, 2, 128)                # the stored width, padding and all
+
+
+def test_rows_keep_their_channels():
+    import copy
+    import pickle
+
+    w = q4.quantize_rows_q4(torch.randn(4, 120))
+    for same in (w, copy.copy(w), copy.deepcopy(w), pickle.loads(pickle.dumps(w))):
+        assert type(same) is q4.Q4Rows and same.channels == 120
+        assert len(same) == 2 and torch.equal(same.codes, w.codes) and torch.equal(same.affine, w.affine)
+    codes, affine = w
+    raw = q4.Q4Rows(codes, affine)                                                  # not said: the width alone is looked at
+    assert raw.channels is None and q4.Q4Rows(codes, affine, 120).channels == 120
+    x = torch.randn(3, 120)
+    assert torch.equal(q4.linear_q4(x, raw), q4.linear_q4(x, w))
+    cache = _cache(QuantizedKVCache, dim=16)
+    assert cache.k.channels == cache._pages(cache.k, 0).channels == 16
+    with pytest.raises(KernelError, match="rows of 20 channels"):
+        cache.update_and_attend(0, *(torch.randn(2, 1, h, 20) for h in (4, 2, 2)), torch.zeros(2, 1, dtype=torch.int32), None)
