@@ -337,23 +337,34 @@ KVCache = PagedKVCache
 
 class QuantizedWeights:
     """4-bit copies of a model's linear weights, in use from :func:`quantize_weights` until :meth:`remove` (or the end of a
-    ``with`` block).  They are copies: parameters that change meanwhile are not seen.  What a parameter had before (copies
-    of an outer block) it has again afterwards."""
+    ``with`` block).  They are copies: parameters that change meanwhile are not seen.  Of several copies of a parameter the
+    latest that has not been removed is in use, whatever the order in which the others go; after the last one the parameter
+    has what it had before."""
 
     def __init__(self):
-        self._before: list[tuple[torch.nn.Parameter, quantized.Q4Rows | None]] = []
+        self._parameters: list[torch.nn.Parameter] = []
+        self._mark = object()                                   # this one's entries among a parameter's copies
 
     def _add(self, p: torch.nn.Parameter, rows: quantized.Q4Rows) -> None:
-        self._before.append((p, getattr(p, "q4", None)))
+        if not hasattr(p, "q4_copies"):
+            p.q4_copies = [(None, p.q4)] if hasattr(p, "q4") else []
+        p.q4_copies.append((self._mark, rows))
         p.q4 = rows
+        self._parameters.append(p)
 
     def remove(self) -> None:
-        while self._before:
-            p, rows = self._before.pop()
-            if rows is not None:
-                p.q4 = rows
+        while self._parameters:
+            p = self._parameters.pop()
+            copies = getattr(p, "q4_copies", None)
+            if copies is None:                                  # a parameter of two modules: seen already
+                continue
+            copies[:] = [c for c in copies if c[0] is not self._mark]
+            if copies:
+                p.q4 = copies[-1][1]
             elif hasattr(p, "q4"):
                 del p.q4
+            if not copies or copies[-1][0] is None:             # none is left
+                del p.q4_copies
 
     def __enter__(self) -> "QuantizedWeights":
         return self

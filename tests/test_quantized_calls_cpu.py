@@ -4,6 +4,7 @@ import pytest
 import torch
 
 from research_b200.errors import KernelError
+from research_b200.infer import quantize_weights
 from research_b200.infer.generation import QuantizedKVCache, decode_one, init_kv_cache, prefill
 from research_b200.ops import quantized as q4
 from tests.test_quantized_generation_cpu import _cache, _model, _rows
@@ -113,3 +114,45 @@ def test_rows_keep_their_channels():
     assert cache.k.channels == cache._pages(cache.k, 0).channels == 16
     with pytest.raises(KernelError, match="rows of 20 channels"):
         cache.update_and_attend(0, *(torch.randn(2, 1, h, 20) for h in (4, 2, 2)), torch.zeros(2, 1, dtype=torch.int32), None)
+
+
+# ------------------------------------------------------------------------------------------------- copies of weights
+def test_copies_of_weights_may_be_taken_back_in_any_order():
+    model = _model()
+    p = model.layers[0].attn.wqkv
+    owners, rows = [], []
+    for _ in range(3):
+        owners.append(quantize_weights(model))
+        rows.append(p.q4)
+    for index, in_use in ((1, 2), (2, 0), (1, 0), (0, None)):           # the latest that is still there; twice is once
+        owners[index].remove()
+        assert getattr(p, "q4", None) is (None if in_use is None else rows[in_use])
+    assert not any(hasattr(p, "q4") for p in model.parameters())
+    named = [(p, set(vars(p))) for p in model.parameters()]
+    a, b = quantize_weights(model), quantize_weights(model)
+    a.remove()
+    b.remove()
+    assert all(set(vars(p)) == before for p, before in named)           # nothing of it stays
+
+
+def test_rows_that_a_parameter_had_before_come_back():
+    model = _model()
+    p = model.layers[0].attn.wo
+    p.q4 = mine = q4.quantize_rows_q4(p.detach())
+    a = quantize_weights(model)
+    with quantize_weights(model):
+        a.remove()
+        assert p.q4 is not mine
+    assert p.q4 is mine
+    del p.q4
+
+
+def test_a_parameter_of_two_modules():
+    model = _model()
+    model.layers[1].attn.wo = model.layers[0].attn.wo
+    p = model.layers[0].attn.wo
+    a, b = quantize_weights(model), quantize_weights(model)
+    a.remove()
+    assert hasattr(p, "q4")
+    b.remove()
+    assert not hasattr(p, "q4") and not hasattr(p, "q4_copies")
