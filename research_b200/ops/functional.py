@@ -129,13 +129,13 @@ class _LinearFn(torch.autograd.Function):
 
 def linear(x: torch.Tensor, p: torch.Tensor) -> torch.Tensor:
     """``y = x @ W^T`` with ``W`` stored ``[out, in]``; where ``W`` has 4-bit rows (its ``q4``) and nothing records
-    gradients, with those."""
+    or carries derivatives, with those."""
 
     rows = getattr(p, "q4", None)
-    if rows is not None and not torch.is_grad_enabled():
+    if rows is not None and _no_derivatives():
         return (quantized.linear_q4 if use_native(x) or not x.is_cuda else quantized.linear_q4_reference)(x, rows)
     if use_native(x):
-        if not torch.is_grad_enabled() and x.numel() // x.shape[-1] <= 64:
+        if _no_derivatives() and x.numel() // x.shape[-1] <= 64:
             # decode-sized input: stream the weight with the whole device (split-K), no autograd bookkeeping
             w = compute_weight(p, x)
             y = native.gemm_skinny(x.reshape(-1, x.shape[-1]), w)

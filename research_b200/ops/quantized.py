@@ -11,7 +11,8 @@ bf16: wider ones are rounded to it first.
 bytes for 64 channels.  Eight channels make a 32-bit word, channel ``i`` of the eight at nibble ``i // 2 + 4 * (i % 2)``;
 words of a block of 128 alternate between its two groups (word ``2 g + h``: channels ``64 h + 8 g ..``).
 
-Nothing here has a gradient: a call that would record one is refused.  On a CUDA device bf16 tensors go to the kernels of
+Nothing here has a gradient: a call that would record one, of rows, queries or the pairs of 4-bit rows, or that would carry a
+forward-mode tangent, is refused.  :func:`quantize_rows_q4` makes plain data, also of what requires a gradient.  On a CUDA device bf16 tensors go to the kernels of
 ``csrc/quant4.cu``, ``csrc/decode_q4.cu`` and ``csrc/linear_q4.cu``; on the CPU the restatements below run, in any dtype.
 """
 
@@ -24,6 +25,7 @@ from typing import NamedTuple
 
 import torch
 import torch.nn.functional as F
+from torch.autograd import forward_ad
 
 from research_b200.errors import KernelError
 from research_b200.ops import native
@@ -167,9 +169,14 @@ def linear_q4_reference(x: torch.Tensor, w: Q4Rows) -> torch.Tensor:
 # argument checks
 # --------------------------------------------------------------------------------------------------
 def _no_gradient(what: str, *tensors: torch.Tensor) -> None:
-    for t in tensors:
-        if t.requires_grad and torch.is_grad_enabled():
-            raise KernelError(f"{what} has no gradient: call it under torch.no_grad() or on detached tensors")
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t.requires_grad:
+                raise KernelError(f"{what} has no gradient: call it under torch.no_grad() or on detached tensors")
+    if forward_ad._current_level >= 0:                  # which torch.no_grad() does not end
+        for t in tensors:
+            if forward_ad.unpack_dual(t).tangent is not None:
+                raise KernelError(f"{what} has no forward-mode derivative: call it on primal tensors")
 
 
 def _same_device(what: str, first: torch.Tensor, *others: torch.Tensor | None) -> None:
@@ -265,6 +272,7 @@ def quantize_rows_q4(x: torch.Tensor) -> Q4Rows:
 
     if x.dim() < 1 or x.shape[-1] < 1 or not x.is_floating_point():
         raise KernelError(f"quantize_rows_q4 needs rows of floating point numbers, got {tuple(x.shape)} {x.dtype}")
+    _no_gradient("quantize_rows_q4", x)
     if not x.is_cuda:
         return quantize_rows_reference(x)
     x2 = x.to(torch.bfloat16).reshape(-1, x.shape[-1])
@@ -285,6 +293,7 @@ def dequantize_rows_q4(rows: Q4Rows, channels: int, dtype: torch.dtype = torch.b
     """Values ``[..., channels]`` of 4-bit rows, rounded once to ``dtype`` (bf16 on a CUDA device)."""
 
     _check_rows("dequantize_rows_q4", rows, channels)
+    _no_gradient("dequantize_rows_q4", rows.affine)
     if not rows.codes.is_cuda:
         return dequantize_rows_reference(rows, channels, dtype)
     if dtype != torch.bfloat16:
@@ -341,7 +350,7 @@ def kv_write_paged_q4(k: torch.Tensor, v: torch.Tensor, k_pool: Q4Rows, v_pool: 
     start = _per_sequence(what, "start", start, B, k)
     if start is None and T > pages * page_rows:
         raise KernelError(f"{what}: {T} rows do not fit a cache of {pages} pages of {page_rows}")
-    _no_gradient(what, k, v)
+    _no_gradient(what, k, v, k_pool.affine, v_pool.affine)
     if k.numel() == 0:
         return
     if not k.is_cuda:
@@ -374,6 +383,7 @@ def kv_read_paged_q4(k_pool: Q4Rows, v_pool: Q4Rows, rows: int, start: torch.Ten
     start = _per_sequence(what, "start", start, B, k_pool.codes)
     if rows < 0:
         raise KernelError(f"{what}: rows must not be negative, got {rows}")
+    _no_gradient(what, k_pool.affine, v_pool.affine)
     if not k_pool.codes.is_cuda:
         return kv_read_paged_q4_reference(k_pool, v_pool, rows, start, channels=D, dtype=dtype)
     _head_dim(what, D)
@@ -413,7 +423,7 @@ def decode_attention_paged_q4(q: torch.Tensor, k_pool: Q4Rows, v_pool: Q4Rows, l
     scale = float(D ** -0.5 if scale is None else scale)
     if not math.isfinite(scale):
         raise KernelError(f"{what}: the scale is a finite number, got {scale}")
-    _no_gradient(what, q)
+    _no_gradient(what, q, k_pool.affine, v_pool.affine)
     if not q.is_cuda:
         return decode_attention_paged_q4_reference(q, k_pool, v_pool, lengths, lo, scale)
     _head_dim(what, D)
@@ -463,7 +473,7 @@ def linear_q4(x: torch.Tensor, w: Q4Rows) -> torch.Tensor:
         raise KernelError(f"{what}: weights are [N, K] as 4-bit rows, got codes {tuple(w.codes.shape)}")
     _check_rows(what, w, K)
     _same_device(what, x, w.codes)
-    _no_gradient(what, x)
+    _no_gradient(what, x, w.affine)
     if not x.is_cuda:
         return linear_q4_reference(x, w)
     if x.dtype != torch.bfloat16:

@@ -2,6 +2,8 @@
 
 import pytest
 import torch
+import torch.nn.functional as F
+from torch.autograd import forward_ad
 
 from research_b200.errors import KernelError
 from research_b200.infer import quantize_weights
@@ -156,3 +158,60 @@ def test_a_parameter_of_two_modules():
     assert hasattr(p, "q4")
     b.remove()
     assert not hasattr(p, "q4") and not hasattr(p, "q4_copies")
+
+
+# ------------------------------------------------------------------------------------------------- derivatives
+def _calls():
+    """Each call with its floating point arguments, by name."""
+
+    w = q4.quantize_rows_q4(torch.randn(5, 70))
+    pools = [q4.quantize_rows_q4(torch.randn(2, 2, 2, 4, 64)) for _ in range(2)]
+    n = torch.tensor([3, 8])
+    held = lambda rows, affine: q4.Q4Rows(rows.codes, affine)  # noqa: E731
+    pairs = dict(ka=pools[0].affine, va=pools[1].affine)
+    rows = lambda: torch.randn(2, 3, 2, 64)  # noqa: E731
+    return [
+        (lambda x, a: q4.linear_q4(x, held(w, a)), dict(x=torch.randn(2, 70), a=w.affine)),
+        (lambda a: q4.dequantize_rows_q4(held(w, a), 70), dict(a=w.affine)),
+        (lambda k, v, ka, va: q4.kv_write_paged_q4(k, v, held(pools[0], ka), held(pools[1], va)), dict(k=rows(), v=rows(), **pairs)),
+        (lambda ka, va: q4.kv_read_paged_q4(held(pools[0], ka), held(pools[1], va), 3), pairs),
+        (lambda q, ka, va: q4.decode_attention_paged_q4(q, held(pools[0], ka), held(pools[1], va), n),
+         dict(q=torch.randn(2, 4, 64), **pairs)),
+    ]
+
+
+@pytest.mark.parametrize("index", range(5))
+def test_a_call_that_would_record_a_derivative_is_refused(index):
+    call, arguments = _calls()[index]
+    call(**arguments)
+    for name, value in arguments.items():
+        with pytest.raises(KernelError, match="has no gradient"):
+            call(**{**arguments, name: value.clone().requires_grad_()})
+        with torch.no_grad():
+            call(**{**arguments, name: value.clone().requires_grad_()})
+            with forward_ad.dual_level():
+                with pytest.raises(KernelError, match="no forward-mode derivative"):
+                    call(**{**arguments, name: forward_ad.make_dual(value.clone(), torch.ones_like(value))})
+                call(**arguments)
+
+
+def test_quantised_rows_are_plain_data():
+    x = torch.randn(3, 70, requires_grad=True)
+    rows = q4.quantize_rows_q4(x)
+    assert not rows.affine.requires_grad and torch.equal(rows.affine, q4.quantize_rows_q4(x.detach()).affine)
+    with forward_ad.dual_level(), pytest.raises(KernelError, match="no forward-mode derivative"):
+        q4.quantize_rows_q4(forward_ad.make_dual(x.detach(), torch.ones(3, 70)))
+
+
+def test_a_linear_with_4_bit_rows_takes_the_parameter_under_a_forward_mode_level():
+    from research_b200.ops import functional as Fn
+
+    p = torch.nn.Parameter(torch.randn(5, 70))
+    p.q4 = q4.quantize_rows_q4(p)
+    x, dx = torch.randn(2, 70), torch.randn(2, 70)
+    with torch.no_grad(), forward_ad.dual_level():
+        y, dy = forward_ad.unpack_dual(Fn.linear(forward_ad.make_dual(x, dx), p))
+        torch.testing.assert_close(y, F.linear(x, p))
+        torch.testing.assert_close(dy, F.linear(dx, p))
+    with torch.no_grad():
+        assert torch.equal(Fn.linear(x, p), q4.linear_q4(x, p.q4))

@@ -167,3 +167,31 @@ def test_one_prompt_for_every_sequence_of_a_cache(dtype, D):
         t = at.shape[1]
         with pytest.raises(KernelError, match="3 sequences"):
             cache.update_and_attend(1, *(x[:, :t].expand(n, t, *x.shape[2:]) for x in (q, k, v)), at.expand(n, t).contiguous(), None)
+
+
+# ------------------------------------------------------------------------------------------------- derivatives
+def test_forward_mode_tangents_are_not_dropped():
+    from torch.autograd import forward_ad
+
+    from research_b200.errors import KernelError
+    from research_b200.ops import functional as Fn
+    from research_b200.ops import quantized as q4
+
+    w = q4.quantize_rows_q4(torch.randn(40, 128, device="cuda"))
+    p = torch.nn.Parameter(torch.randn(40, 128, device="cuda"))
+    p.q4 = w
+    pools = [q4.quantize_rows_q4(torch.randn(2, 2, 2, 8, 64, device="cuda")) for _ in range(2)]
+    n = torch.tensor([3, 8], device="cuda")
+    with torch.no_grad(), forward_ad.dual_level():
+        dual = lambda *shape: forward_ad.make_dual(*(torch.randn(*shape, device="cuda").to(BF16) for _ in range(2)))  # noqa: E731
+        row = dual(2, 1, 2, 64)
+        for call in (lambda: q4.linear_q4(dual(3, 128), w), lambda: q4.kv_write_paged_q4(row, row, *pools),
+                     lambda: q4.decode_attention_paged_q4(dual(2, 4, 64), *pools, n), lambda: q4.quantize_rows_q4(dual(3, 128))):
+            with pytest.raises(KernelError, match="no forward-mode derivative"):
+                call()
+        for rows in (1, 100):                              # the parameter's own kernels have none either, and say so
+            with pytest.raises(RuntimeError):
+                Fn.linear(dual(rows, 128), p)
+    with torch.no_grad():
+        x = torch.randn(3, 128, device="cuda").to(BF16)
+        assert torch.equal(Fn.linear(x, p), q4.linear_q4(x, w))
