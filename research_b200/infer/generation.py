@@ -299,13 +299,16 @@ class GraphedDecodeStep:
     A decode step of a small batch is a few hundred short kernels, so its cost is launch latency, not work; the
     captured graph replays them with one launch.  Token and position live in static device buffers that are
     overwritten before each replay; sampling stays outside the graph.  Shapes are fixed at capture (batch size,
-    cache capacity)."""
+    cache capacity), and so are the weights: 4-bit copies that were in use then are used, and kept, for as long as the
+    step lives, also after their removal from the model."""
 
     def __init__(self, model, cache: PagedKVCache, first_token: torch.Tensor, first_position: int):
         B = first_token.shape[0]
         dev = first_token.device
-        self.cache = cache
         _require_rows(cache, int(first_position))
+        # the graph holds addresses only
+        self.cache, self.model = cache, model
+        self._rows = [p.q4 for p in model.parameters() if hasattr(p, "q4")]
         self.token = first_token.reshape(B, 1).to(torch.int32).clone()
         self.position = torch.full((B, 1), int(first_position), device=dev, dtype=torch.int32)
         side = torch.cuda.Stream(device=dev)

@@ -195,3 +195,23 @@ def test_forward_mode_tangents_are_not_dropped():
     with torch.no_grad():
         x = torch.randn(3, 128, device="cuda").to(BF16)
         assert torch.equal(Fn.linear(x, p), q4.linear_q4(x, w))
+
+
+# ------------------------------------------------------------------------------------------------- graphs
+def test_a_captured_step_keeps_the_copies_of_weights_that_it_reads():
+    from research_b200.infer import init_kv_cache, prefill, quantize_weights
+    from research_b200.infer.generation import GraphedDecodeStep
+
+    model = _trainer().result.model.eval()
+    cache = init_kv_cache(model, 2, 64, cache_bits=4)
+    token = torch.tensor([5, 7], device="cuda")
+    with quantize_weights(model):
+        prefill(model, torch.randint(0, 512, (2, 40), device="cuda"), cache)
+        places = {p.q4.codes.data_ptr() for p in model.parameters() if hasattr(p, "q4")}
+        sizes = [t.numel() * t.element_size() for p in model.parameters() if hasattr(p, "q4") for t in p.q4]
+        step = GraphedDecodeStep(model, cache, token, 40)
+        want = step(token, 40).clone()
+    assert not any(hasattr(p, "q4") for p in model.parameters())
+    other = [torch.full((n,), 255, dtype=torch.uint8, device="cuda") for n in sizes for _ in range(2)]
+    assert not places & {t.data_ptr() for t in other}           # the rows are still the step's
+    assert torch.equal(step(token, 40), want)
