@@ -92,7 +92,8 @@ __global__ void __launch_bounds__(WARPS * 32) linear_q4_few_kernel(const __grid_
 #pragma unroll
     for (int b = 0; b < KB; ++b) code[m][b] = make_uint4(0, 0, 0, 0), pair[m][b] = make_uint2(0, 0);
   b200::pdl_launch_dependents();
-  // what runs before may be what writes the weights: they are read after the wait, and only brought into L2 ahead of it
+  // what runs before may be what writes the weights: they are read after the wait, by loads that do not take them for
+  // unchanging, and only brought into L2 ahead of it
 #pragma unroll
   for (int m = 0; m < 2; ++m)
     if (kb0 < blocks)
@@ -108,7 +109,7 @@ __global__ void __launch_bounds__(WARPS * 32) linear_q4_few_kernel(const __grid_
       for (int b = 0; b < KB; ++b)
         if (kb0 + b < blocks) {
           code[m][b] = ld_stream(c + 4 * b);
-          pair[m][b] = __ldg(f + b);
+          pair[m][b] = f[b];
         }
     }
   };
@@ -473,13 +474,13 @@ linear_q4_many_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_cons
     Place<M::CODE_STAGES> c;
     Place<M::STEPS> w;
     if (half) w.on();
-    uint2 pair = half < steps ? __ldg(pairs + half) : make_uint2(0, 0);
+    uint2 pair = half < steps ? pairs[half] : make_uint2(0, 0);
     for (int j = half; j < steps; j += 2) {
       ok = wait_warp(&c_full[c.at], c.round, ab, ERR_WAIT_FULL);
       if (!ok) break;
       const uint32_t s0 = __byte_perm(pair.x, pair.x, 0x1010), z0 = __byte_perm(pair.x, pair.x, 0x3232);
       const uint32_t s1 = __byte_perm(pair.y, pair.y, 0x1010), z1 = __byte_perm(pair.y, pair.y, 0x3232);
-      pair = j + 2 < steps ? __ldg(pairs + j + 2) : make_uint2(0, 0);
+      pair = j + 2 < steps ? pairs[j + 2] : make_uint2(0, 0);
 #pragma unroll
       for (int part = side; part < 2; part += M::SIDES) {    // half of the channels each
         uint32_t r[2][16];

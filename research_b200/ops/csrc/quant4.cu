@@ -196,8 +196,8 @@ __global__ void __launch_bounds__(256) quantize_rows_q4_kernel(const __nv_bfloat
   }
 }
 
-__global__ void __launch_bounds__(256) dequantize_rows_q4_kernel(const uint32_t* __restrict__ codes,
-                                                                 const uint32_t* __restrict__ affine,
+// Codes and pairs may be the predecessor's work: only the output is said to be alone.
+__global__ void __launch_bounds__(256) dequantize_rows_q4_kernel(const uint32_t* codes, const uint32_t* affine,
                                                                  __nv_bfloat16* __restrict__ out, long long rows,
                                                                  int width) {
   const int words = width / 8;

@@ -215,3 +215,30 @@ def test_a_linear_with_4_bit_rows_takes_the_parameter_under_a_forward_mode_level
         torch.testing.assert_close(dy, F.linear(dx, p))
     with torch.no_grad():
         assert torch.equal(Fn.linear(x, p), q4.linear_q4(x, p.q4))
+
+
+# ------------------------------------------------------------------------------------------------- kernels that start early
+def test_kernels_that_start_early_do_not_take_their_inputs_for_unchanging():
+    """What the predecessor may still be writing when a kernel starts is read by plain loads: ``__ldg``, and loads through
+    ``const * __restrict__``, are for memory that nothing writes as long as the kernel runs."""
+
+    import re
+    from pathlib import Path
+
+    csrc = Path(q4.__file__).parent / "csrc"
+    seen = []
+    for name in ("quant4.cuh", "quant4.cu", "decode_q4.cu", "linear_q4.cu"):
+        text = re.sub(r"//[^\n]*", "", (csrc / name).read_text())
+        for head in re.finditer(r"__global__([^{]*?(\w+_kernel)\s*\([^{]*)\{", text):
+            depth, at = 1, head.end()
+            while depth:
+                depth += {"{": 1, "}": -1}.get(text[at], 0)
+                at += 1
+            body = text[head.end():at]
+            if "pdl_wait()" not in body:
+                continue
+            seen.append(head.group(2))
+            assert not re.findall(r"__ldg|ld\.global\.nc|ldcs", body), head.group(2)
+            assert not re.findall(r"const\s+[\w:]+\s*\*\s*__restrict__", head.group(1)), head.group(2)
+    assert {"kv_write_q4_kernel", "kv_read_q4_kernel", "dequantize_rows_q4_kernel", "decode_q4_kernel", "decode_q4_merge_kernel",
+            "linear_q4_few_kernel", "linear_q4_many_kernel", "linear_q4_narrow_kernel"} == set(seen)

@@ -215,3 +215,30 @@ def test_a_captured_step_keeps_the_copies_of_weights_that_it_reads():
     other = [torch.full((n,), 255, dtype=torch.uint8, device="cuda") for n in sizes for _ in range(2)]
     assert not places & {t.data_ptr() for t in other}           # the rows are still the step's
     assert torch.equal(step(token, 40), want)
+
+
+# ------------------------------------------------------------------------------------------------- kernels that start early
+@pytest.mark.parametrize("rows", [1, 16, 40, 200])
+def test_weights_that_the_predecessor_has_just_written(rows):
+    """A cache's rows as weights: each product starts before the write of its weights has ended, and waits for it."""
+
+    from research_b200.ops import quantized as q4
+
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    N, D = 4096, 128
+    pools = [q4.empty_rows(1, 1, 1, N, channels=D, device="cuda") for _ in range(2)]
+    weights = [q4.Q4Rows(*(t.view(N, -1) if i == 0 else t.view(N, 2, 2) for i, t in enumerate(pool)), D) for pool in pools]
+    x = torch.randn(rows, D, generator=g, device="cuda").to(BF16)
+    full = [torch.randn(2, 1, N, 1, D, generator=g, device="cuda").to(BF16) for _ in range(2)]
+    want = [[q4.linear_q4(x, q4.quantize_rows_q4(t.view(N, D))) for t in pair] for pair in full]
+    back = [[q4.dequantize_rows_q4(q4.quantize_rows_q4(t.view(N, D)), D) for t in pair] for pair in full]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        got = []
+        for pair in full:
+            q4.kv_write_paged_q4(*pair, *pools)
+            got.append([q4.linear_q4(x, w) for w in weights])
+            q4.kv_write_paged_q4(*pair, *pools)
+            got[-1].append(q4.dequantize_rows_q4(weights[0], D))
+        for a, b, c in zip(got, want, back):
+            assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1]) and torch.equal(a[2], c[0])
