@@ -242,3 +242,34 @@ def test_weights_that_the_predecessor_has_just_written(rows):
             got[-1].append(q4.dequantize_rows_q4(weights[0], D))
         for a, b, c in zip(got, want, back):
             assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1]) and torch.equal(a[2], c[0])
+
+
+# ------------------------------------------------------------------------------------------------- precision
+@pytest.mark.parametrize("D,G", [(128, 2), (128, 4), (64, 4), (64, 8), (128, 7)])
+def test_weights_are_rounded_to_neither_side(D, G):
+    """Rows in pairs of one key and opposite values: every weight's share cancels, and what is left is what the weights'
+    two bf16 parts lost.
+
+    With s = 1, values of +- 7.5 are the codes 15 and 0 of z = -7.5: a channel is 15 sum p over one row of each pair, less
+    7.5 sum p over all.  The low part of a weight is below 2^-7 of it and is rounded by 2^-8 of itself at most, to either
+    side: N such errors add up to 15 * 6 * 2^-15 sqrt(sum p^2) but once in 10^7.  A tile's sums are made in fp32 (4 products
+    of 2^-22, 14 additions of 2^-24, of 7.5), and its own two sums cancel before tiles are joined.  Cut off instead of
+    rounded, the weights would lose 2^-16 each on average, to one side."""
+
+    from research_b200.ops import quantized as q4
+
+    g = torch.Generator(device="cuda").manual_seed(D + G)
+    rows, ps = 8192, 128
+    k = torch.randn(1, rows // 2, 1, D, generator=g, device="cuda").repeat_interleave(2, 1)
+    sign = 1.0 - 2.0 * ((torch.arange(rows, device="cuda")[:, None] + torch.arange(D, device="cuda")) % 2)
+    v = (7.5 * sign)[None, :, None]
+    pools = [q4.quantize_rows_q4(t.reshape(1, rows // ps, ps, 1, D).transpose(2, 3).contiguous().to(BF16)) for t in (k, v)]
+    assert (pools[1].affine[..., 0] == 1.0).all() and (pools[1].affine[..., 1] == -7.5).all()
+    q = (0.8 * torch.randn(1, G, D, generator=g, device="cuda")).to(BF16)
+    n = torch.tensor([rows], device="cuda", dtype=torch.int32)
+    got = q4.decode_attention_paged_q4(q, *pools, n).double().view(G, D)
+    keys = q4.dequantize_rows_reference(pools[0], D, torch.float64).transpose(2, 3).reshape(rows, D)
+    p = torch.softmax(q[0].double() @ keys.t() * D ** -0.5, -1)
+    assert torch.equal(p[:, 0::2], p[:, 1::2])
+    tol = 15 * 6 * 2.0 ** -15 * p[:, 0::2].square().sum(-1).sqrt() + 7.5 * (4 * 2.0 ** -22 + 14 * 2.0 ** -24)
+    assert (got.abs() <= tol[:, None]).all(), (got.abs().amax(-1) / tol, got.mean(-1))
