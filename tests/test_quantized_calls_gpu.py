@@ -273,3 +273,67 @@ def test_weights_are_rounded_to_neither_side(D, G):
     assert torch.equal(p[:, 0::2], p[:, 1::2])
     tol = 15 * 6 * 2.0 ** -15 * p[:, 0::2].square().sum(-1).sqrt() + 7.5 * (4 * 2.0 ** -22 + 14 * 2.0 ** -24)
     assert (got.abs() <= tol[:, None]).all(), (got.abs().amax(-1) / tol, got.mean(-1))
+
+
+def bf16_weights_tolerance(x, full):
+    """What a product of bf16 ``x`` and ``full`` (float64 copies) with fp32 sums may be off by: half a bf16 step of the result,
+    and of the sum's running value, a walk of K products that stays within 5 of its standard deviations, four units of
+    2^-24 for each of the K / 16 products that are added to it, and for the joining of up to 8 slices."""
+
+    want = x @ full.t()
+    walk = 5 * (x.square() @ full.t().square()).sqrt()
+    return want, 2.0 ** -8 * want.abs() + (x.shape[1] / 16 + 8) * 2.0 ** -22 * walk
+
+
+@pytest.mark.parametrize("rows,N,K", [(17, 2048, 2048), (32, 1000, 1856), (64, 77, 5632), (33, 130, 705), (16, 5000, 4000), (9, 100, 17000),
+                                      (1, 100, 33000), (100, 1000, 4000), (128, 9, 16000), (777, 512, 1100), (300, 2600, 520),
+                                      (129, 333, 705), (1000, 4096, 300), (65, 1000, 130), (70, 50, 64), (2000, 700, 2048)])
+def test_products_of_many_rows_are_those_of_the_weights_as_bf16(rows, N, K):
+    """Above few_rows every weight counts as a bf16, one number: against those in 64 bits the result has nothing but its own
+    rounding and that of the sums left, which a channel or a bit of a weight more or less is far above."""
+
+    from research_b200.ops import quantized as q4
+
+    assert rows > q4.few_rows(N, K)
+    g = torch.Generator(device="cuda").manual_seed(rows + K)
+    x = torch.randn(rows, K, generator=g, device="cuda").to(BF16)
+    w = q4.quantize_rows_q4(torch.randn(N, K, generator=g, device="cuda") * 0.05)
+    want, tol = bf16_weights_tolerance(x.double(), q4.dequantize_rows_reference(w, K, BF16).double())
+    off = (q4.linear_q4(x, w).double() - want).abs()
+    assert (off <= tol).all(), (off / tol).max()
+
+
+@pytest.mark.parametrize("kind", ["decoder", "trinity"])
+def test_logits_with_4_bit_weights_are_those_of_a_model_that_holds_their_values(kind):
+    """A prompt and a step through 4-bit weights, against the same model with the values put in place of its parameters.
+
+    Both multiply the same numbers, but for the step, whose weights are not rounded to bf16; the rest is the bf16 roundings of
+    two layers' activations, 2^-8 each, of which two dozen in a row add up to 2^-8 sqrt(24) < 2^-5 of the logits' norm.  What
+    4 bits cost themselves is more than that."""
+
+    from research_b200.infer import decode_one, init_kv_cache, prefill, quantize_weights
+    from research_b200.ops import quantized as q4
+
+    model = _trainer(kind).result.model.eval()
+    g = torch.Generator(device="cuda").manual_seed(1)
+    prompts = torch.randint(0, 512, (2, 40), generator=g, device="cuda")
+    token = torch.tensor([3, 400], device="cuda")
+
+    @torch.no_grad()
+    def logits():
+        cache = init_kv_cache(model, 2, 64)
+        return [prefill(model, prompts, cache).double(), decode_one(model, token, 40, cache).double()]
+
+    before = logits()
+    with quantize_weights(model), torch.no_grad():
+        got = logits()
+        held = [(p, p.q4) for p in model.parameters() if hasattr(p, "q4")]
+    assert len(held) >= 8
+    with torch.no_grad():
+        for p, rows in held:
+            p.copy_(q4.dequantize_rows_q4(rows, p.shape[1]))
+            if getattr(p, "shadow", None) is not None:
+                p.shadow.copy_(p)
+    for a, b, c in zip(got, logits(), before):
+        assert (a - b).norm() <= 2.0 ** -5 * b.norm(), (a - b).norm() / b.norm()
+        assert (a - c).norm() > 2.0 ** -5 * c.norm(), (a - c).norm() / c.norm()
