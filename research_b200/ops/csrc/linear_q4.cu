@@ -1,6 +1,6 @@
 // y = x W^T with weights held in 4 bits (quant4.cuh): x [rows, K] bf16, W [N, K], y [rows, N] bf16 with fp32 sums.
 //
-// Up to 8 or 16 rows of x (see few_rows) the time is that of streaming the codes once (0.56 bytes a weight), as long as
+// Up to 8 or 16 rows of x (the caller's choice) the time is that of streaming the codes once (0.56 bytes a weight), as long as
 // expanding them keeps up: at the copy bandwidth an SM gets 46 codes a clock.  linear_q4_few_kernel expands nothing: the codes
 // go from memory to registers to mma.sync m16n8k16 as the bf16 numbers that their bits are, n 2^-133 (subnormals and the first
 // binade are one straight line), by a mask each and one shift for four of eight; x is the column operand, brought to about
@@ -590,18 +590,11 @@ int launch_cluster(void (*kern)(Args...), int cluster, long long blocks, int thr
   return static_cast<int>(cudaLaunchKernelEx(&cfg, kern, args...));
 }
 
-// Rows of x up to which the codes are multiplied as they are.  A cluster of up to 8 blocks has registers for 8 rows of 32768
-// channels or 16 of 16384; more than 8 rows are better off there where they need no cluster or have few weights: 16 rows of 11264 x
-// 2048 take 8.2 us against 10 to 12, of 2048 x 5632 7.3 against 9.0, of 28672 x 4096 35 against 27, of 4096 x 14336 27 against 17.
-int few_rows(int N, int K) {
-  if (K <= 2048 || (K <= 8 * 16 * 128 && static_cast<long long>(N) * K <= 1 << 24)) return 16;
-  return K <= 8 * 16 * 256 ? 8 : 0;
-}
-
 template <int KB, int WARPS, int NC>
 int launch_few(FewParams p, int blocks_per_sm, cudaStream_t stream) {
   const int tiles = (p.N + 15) / 16;
   p.cluster = (p.width / 128 + WARPS * KB - 1) / (WARPS * KB);
+  if (p.cluster > 8) return b200host::RC_BAD_SHAPE;   // more channels than a cluster's registers hold of x
   // clusters of more than 2 and 4 find no room on some of the SMs
   int clusters = blocks_per_sm * b200host::sm_count() * (p.cluster > 4 ? 75 : p.cluster > 2 ? 90 : 100) / 100 / p.cluster;
   if (clusters > tiles) clusters = tiles;
@@ -621,13 +614,13 @@ int launch_many(const CUtensorMap& tmW, const CUtensorMap& tmX, const LinearPara
 }  // namespace
 
 // out [rows, N] (row stride ldo) = x [rows, K] (ldx) * W^T, W as codes [N, width / 8] words and affine [N, width / 64] pairs.  With
-// more than 64 channels and more than few_rows(N, K) rows K is cut into `cluster` (1, 2, 4 or 8) slices, and rows of x start on
-// 16 bytes.
+// more than 64 channels the caller says how: `cluster` 0 multiplies the codes as they are (up to 16 rows of 16384 channels or 8
+// of 32768), 1, 2, 4 or 8 cuts K into as many slices of expanded weights, for which rows of x start on 16 bytes.
 extern "C" int b200_q4_linear(const void* x, long long ldx, const void* codes, const void* affine, void* out,
                               long long ldo, int rows, int N, int K, int cluster, void* status, void* stream) {
   using namespace b200host;
   if (rows <= 0 || rows > (1 << 24) || N <= 0 || K <= 0 || K > (1 << 30) || !status) return RC_BAD_SHAPE;
-  if (cluster != 1 && cluster != 2 && cluster != 4 && cluster != 8) return RC_BAD_SHAPE;
+  if (cluster < 0 || cluster > 8 || (cluster & (cluster - 1))) return RC_BAD_SHAPE;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   const int width = row_width(K);
   if (!rows_aligned(codes, affine, width)) return RC_BAD_ALIGNMENT;
@@ -635,7 +628,8 @@ extern "C" int b200_q4_linear(const void* x, long long ldx, const void* codes, c
     return static_cast<int>(launch_kernel(linear_q4_narrow_kernel, dim3((N + 3) / 4, (rows + 7) / 8), dim3(128), 0, s,
                                           pdl_enabled() != 0, (const __nv_bfloat16*)x, ldx, (const uint32_t*)codes,
                                           (const uint32_t*)affine, (__nv_bfloat16*)out, ldo, rows, N, K));
-  if (rows <= few_rows(N, K)) {
+  if (cluster == 0) {
+    if (rows > 16) return RC_BAD_SHAPE;
     const int aligned = ldx % 8 == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0, blocks = width / 128;
     const FewParams p{(const __nv_bfloat16*)x, ldx, (const uint8_t*)codes, (const uint8_t*)affine, (__nv_bfloat16*)out, ldo, rows,
                       N, K, width, aligned, 1};

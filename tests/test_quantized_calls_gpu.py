@@ -337,3 +337,24 @@ def test_logits_with_4_bit_weights_are_those_of_a_model_that_holds_their_values(
     for a, b, c in zip(got, logits(), before):
         assert (a - b).norm() <= 2.0 ** -5 * b.norm(), (a - b).norm() / b.norm()
         assert (a - c).norm() > 2.0 ** -5 * c.norm(), (a - c).norm() / c.norm()
+
+
+def test_who_multiplies_is_said_once():
+    """The kernel for few rows runs where few_rows says so, and the launcher refuses what it has no room for."""
+
+    from research_b200.ops import native
+    from research_b200.ops import quantized as q4
+
+    def launch(rows, K, cluster):
+        x = torch.zeros(rows, K, device="cuda", dtype=BF16)
+        w = q4.empty_rows(8, channels=K, device="cuda")
+        out = torch.empty(rows, 8, device="cuda", dtype=BF16)
+        return native.load().b200_q4_linear(x.data_ptr(), K, w.codes.data_ptr(), w.affine.data_ptr(), out.data_ptr(), 8, rows, 8, K,
+                                            cluster, native.status_word(x.device).data_ptr(), native._stream())
+
+    for K in (128, 1000, 2048, 2056, 16384, 16392, 32768, 32776):
+        rows = q4.few_rows(8, K)
+        assert rows in (0, 8, 16) and (rows == 0 or launch(rows, K, 0) == 0)
+    for rows, K, cluster in ((17, 128, 0), (9, 16392, 0), (1, 32776, 0), (1, 256, 3), (1, 256, -1), (1, 256, 16)):
+        assert launch(rows, K, cluster) == -2
+    torch.cuda.synchronize()
