@@ -493,6 +493,10 @@ def generate_tokens(model, prompt_ids: torch.Tensor, *, max_new_tokens: int, tem
     model.train(was_training)
     out = torch.stack(tokens, dim=1).cpu()
     lps = torch.stack(logprobs, dim=1).cpu()
+    if device.type == "cuda":
+        from research_b200.ops import native
+
+        native.check_status(device)                             # a kernel whose wait ran out has left zeros
     prompts = prompt_ids.cpu().tolist()
     generated = out.tolist()
     return GenerationResult(prompts, generated, [p + g for p, g in zip(prompts, generated)], lps.tolist())

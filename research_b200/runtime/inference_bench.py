@@ -86,6 +86,10 @@ def run_inference_bench(spec, *, batch: int, prompt: int, new_tokens: int, tempe
     for _ in range(warmup):
         one_run()
     runs = [one_run() for _ in range(repeats)]
+    if cuda:
+        from research_b200.ops import native
+
+        native.check_status(dev)
     all_prefill = [1e3 * r[0] for r in runs]
     runs.sort(key=lambda r: r[2])
     _, t_first, t_decode = runs[len(runs) // 2]

@@ -358,3 +358,22 @@ def test_who_multiplies_is_said_once():
     for rows, K, cluster in ((17, 128, 0), (9, 16392, 0), (1, 32776, 0), (1, 256, 3), (1, 256, -1), (1, 256, 16)):
         assert launch(rows, K, cluster) == -2
     torch.cuda.synchronize()
+
+
+# ------------------------------------------------------------------------------------------------- waits that ran out
+@pytest.mark.parametrize("bits", [4, 16])
+def test_generation_says_when_a_wait_ran_out(bits):
+    """A kernel whose bounded wait runs out sets the status word and leaves zeros: no tokens are made of them."""
+
+    from research_b200.errors import KernelError
+    from research_b200.infer import generate_tokens
+    from research_b200.ops import native
+
+    model = _trainer().result.model.eval()
+    prompts = torch.randint(0, 512, (2, 20), device="cuda")
+    call = lambda: generate_tokens(model, prompts, max_new_tokens=3, top_k=1, cache_bits=bits, weight_bits=bits)  # noqa: E731
+    want = call().generated_ids
+    native.status_word(prompts.device)[0:1].fill_(42)
+    with pytest.raises(KernelError, match="ran out"):
+        call()
+    assert call().generated_ids == want and not any(hasattr(p, "q4") for p in model.parameters())
