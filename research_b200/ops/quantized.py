@@ -134,7 +134,10 @@ def kv_read_paged_q4_reference(k_pool: Q4Rows, v_pool: Q4Rows, rows: int, start=
                                dtype: torch.dtype = torch.bfloat16):
     at, inside = _pool_index(k_pool, rows, start)
     b = torch.arange(at.shape[0], device=at.device)[:, None].expand_as(at)
-    at, page_rows = at.clamp(0, k_pool.codes.shape[1] * k_pool.codes.shape[3] - 1), k_pool.codes.shape[3]
+    _, pages, heads, page_rows, _ = k_pool.codes.shape
+    if pages * page_rows == 0:
+        return tuple(torch.zeros(*at.shape, heads, channels, dtype=dtype, device=at.device) for _ in range(2))
+    at = at.clamp(0, pages * page_rows - 1)
     out = []
     for pool in (k_pool, v_pool):
         held = Q4Rows(*(t[b, at // page_rows, :, at % page_rows] for t in pool))

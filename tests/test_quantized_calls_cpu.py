@@ -242,3 +242,16 @@ def test_kernels_that_start_early_do_not_take_their_inputs_for_unchanging():
             assert not re.findall(r"const\s+[\w:]+\s*\*\s*__restrict__", head.group(1)), head.group(2)
     assert {"kv_write_q4_kernel", "kv_read_q4_kernel", "dequantize_rows_q4_kernel", "decode_q4_kernel", "decode_q4_merge_kernel",
             "linear_q4_few_kernel", "linear_q4_many_kernel", "linear_q4_narrow_kernel"} == set(seen)
+
+
+# ------------------------------------------------------------------------------------------------- a cache without rows
+@pytest.mark.parametrize("pages,page_rows", [(0, 4), (2, 0), (0, 0)])
+def test_a_cache_without_rows(pages, page_rows):
+    """Rows that the cache does not have are left out, read as zeros, and count for nothing."""
+
+    pools = [q4.empty_rows(2, pages, 2, page_rows, channels=64) for _ in range(2)]
+    k = torch.randn(2, 3, 2, 64)
+    q4.kv_write_paged_q4(k, k, *pools, torch.tensor([0, 1]))
+    for back in q4.kv_read_paged_q4(*pools, 3, torch.tensor([0, 1])):
+        assert back.shape == (2, 3, 2, 64) and back.dtype == torch.bfloat16 and not back.any()
+    assert not q4.decode_attention_paged_q4(torch.randn(2, 4, 64), *pools, torch.tensor([0, 5])).any()
