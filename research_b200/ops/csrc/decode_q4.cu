@@ -20,9 +20,11 @@
 // the rounding costs 1 to 2 % of the time.  A single bf16 would cost as much as the rounding of the result does.)
 //
 // Measured (inputs of several sets in turn, larger than L2), heads of 128: 64 sequences of 512 .. 4096 rows, 16 heads over 8,
-// 46.6 us, of 16384 rows 136.7 us, 77 % of the copy bandwidth; 2 sequences of 32768 rows, 32 heads over 8, 21.8 us; one of 777
-// rows 7.3 us, which are two launches and one tile's latency.  With codes as 128 + n (a second operation each, and the 128
-// taken off again) and a maximum followed tile by tile the first took 53 us.
+// 47.6 us, of 16384 rows 139.9 us, 75 % of the copy bandwidth; 2 sequences of 32768 rows, 32 heads over 8, 22.0 us; one of 777
+// rows 7.6 us, which are two launches and one tile's latency.  No unit is full (59 % of the issue slots, 58 % of the DRAM rate at
+// 16384 rows): twelve warps an SM with one tile under way each wait for latency.  With codes as 128 + n (a second operation
+// each, and the 128 taken off again) and a maximum followed tile by tile the first took 53 us.  That and the other comparisons
+// below were taken with both parts of p s cut off.
 #include <math.h>
 #include <math_constants.h>
 
@@ -676,7 +678,7 @@ int launch(const AttnParams& p, cudaStream_t s) {
   // fewer runs than the device has blocks: one warp of a block each, on as many SMs
   const int most = kBlocks * b200host::sm_count(), grid = p.warps < most ? p.warps : most;
   if (cudaError_t e = b200host::launch_kernel(kern, dim3(grid), dim3(kWarps * 32), bytes, s, pdl, p)) return static_cast<int>(e);
-  // where a head has many pieces, more threads read them at once: 64 heads in 111 pieces each, both kernels,
+  // where a head has many pieces, more threads read them at once: 64 heads in 103 or 104 pieces each, both kernels,
   // 256 threads 23.1 us, 512 21.8, 1024 26.0; 7 pieces of 512 heads, 256 threads 46.6 us, and 512 find less room beside the
   // first kernel
   const bool many = p.warps > 32 * p.B * p.Hkv;

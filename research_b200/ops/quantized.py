@@ -408,7 +408,9 @@ def decode_attention_paged_q4(q: torch.Tensor, k_pool: Q4Rows, v_pool: Q4Rows, l
                               lo: torch.Tensor | None = None, scale: float | None = None) -> torch.Tensor:
     """Attention of one query token per sequence, ``q [B, Hq, D]``, over rows ``lo[b] <= r < lengths[b]`` of caches of 4-bit
     rows ``[B, pages, Hkv, page_rows, D]`` (``lengths``, ``lo`` int32 or int64 ``[B]``; rows beyond the cache do not count, a
-    sequence without a row gets zeros).  Up to 8 query heads share a K/V head.  Returns ``[B, Hq * D]`` in q's type."""
+    sequence without a row gets zeros).  Up to 8 query heads share a K/V head.  Returns ``[B, Hq * D]`` in q's type.  On a CUDA
+    device weights of up to 2^8 times values are added up in fp32 before the division: V of up to 2^95 in size cannot overflow
+    it in a cache of 2^24 rows."""
 
     what = "decode_attention_paged_q4"
     if q.dim() != 3 or not q.is_floating_point():
