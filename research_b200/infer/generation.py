@@ -149,7 +149,8 @@ class QuantizedKVCache(PagedKVCache):
     cache attends over its own rows, which it still has in full; a later piece of several tokens reads the rows before it
     back, rounded to the queries' type.  Positions that the cache has no row for are refused, but for a step whose positions
     are on a CUDA device, which nothing waits for: there a row outside is left out, and :func:`decode_one` and
-    :class:`GraphedDecodeStep` look before.  ``k`` and ``v`` are :class:`research_b200.ops.quantized.Q4Rows` ``[layers, pages, kv_heads, page_size, ..]``."""
+    :class:`GraphedDecodeStep` look before.  ``k`` and ``v`` are :class:`research_b200.ops.quantized.Q4Rows`
+    ``[layers, pages, kv_heads, page_size, ..]``."""
 
     def _pool(self, shape, dtype, device):
         return quantized.empty_rows(*shape[:-1], channels=shape[-1], device=device)

@@ -12,8 +12,9 @@ bytes for 64 channels.  Eight channels make a 32-bit word, channel ``i`` of the 
 words of a block of 128 alternate between its two groups (word ``2 g + h``: channels ``64 h + 8 g ..``).
 
 Nothing here has a gradient: a call that would record one, of rows, queries or the pairs of 4-bit rows, or that would carry a
-forward-mode tangent, is refused.  :func:`quantize_rows_q4` makes plain data, also of what requires a gradient.  On a CUDA device bf16 tensors go to the kernels of
-``csrc/quant4.cu``, ``csrc/decode_q4.cu`` and ``csrc/linear_q4.cu``; on the CPU the restatements below run, in any dtype.
+forward-mode tangent, is refused.  :func:`quantize_rows_q4` makes plain data, also of what requires a gradient.  On a CUDA
+device bf16 tensors go to the kernels of ``csrc/quant4.cu``, ``csrc/decode_q4.cu`` and ``csrc/linear_q4.cu``; on the CPU the
+restatements below run, in any dtype.
 """
 
 from __future__ import annotations
@@ -356,6 +357,12 @@ def kv_write_paged_q4(k: torch.Tensor, v: torch.Tensor, k_pool: Q4Rows, v_pool: 
     _no_gradient(what, k, v, k_pool.affine, v_pool.affine)
     if k.numel() == 0:
         return
+    (k_codes, k_affine), (v_codes, v_affine) = k_pool, v_pool
+    k_codes_at, k_affine_at, v_codes_at, v_affine_at = (k_codes.data_ptr(), k_affine.data_ptr(), v_codes.data_ptr(),
+                                                        v_affine.data_ptr())
+    # both are written at once
+    if abs(k_codes_at - v_codes_at) < k_codes.numel() or abs(k_affine_at - v_affine_at) < 2 * k_affine.numel():
+        raise KernelError(f"{what}: the K and the V cache share memory")
     if not k.is_cuda:
         return kv_write_paged_q4_reference(k, v, k_pool, v_pool, start)
     _head_dim(what, D)
@@ -365,9 +372,8 @@ def kv_write_paged_q4(k: torch.Tensor, v: torch.Tensor, k_pool: Q4Rows, v_pool: 
     v, v_row, v_batch = _heads_apart(v, Hkv, D)
     with _on(k):
         native._check((native._lib or native.load()).b200_q4_kv_write(
-            k.data_ptr(), v.data_ptr(), k_row, k_batch, v_row, v_batch, k_pool.codes.data_ptr(),
-            k_pool.affine.data_ptr(), v_pool.codes.data_ptr(), v_pool.affine.data_ptr(), native._ptr(start), B, T, Hkv,
-            D, pages, page_rows, native._stream()), "b200_q4_kv_write")
+            k.data_ptr(), v.data_ptr(), k_row, k_batch, v_row, v_batch, k_codes_at, k_affine_at, v_codes_at, v_affine_at,
+            native._ptr(start), B, T, Hkv, D, pages, page_rows, native._stream()), "b200_q4_kv_write")
 
 
 def kv_read_paged_q4(k_pool: Q4Rows, v_pool: Q4Rows, rows: int, start: torch.Tensor | None = None, *,

@@ -255,3 +255,25 @@ def test_a_cache_without_rows(pages, page_rows):
     for back in q4.kv_read_paged_q4(*pools, 3, torch.tensor([0, 1])):
         assert back.shape == (2, 3, 2, 64) and back.dtype == torch.bfloat16 and not back.any()
     assert not q4.decode_attention_paged_q4(torch.randn(2, 4, 64), *pools, torch.tensor([0, 5])).any()
+
+
+# ------------------------------------------------------------------------------------------------- shared memory
+def test_caches_that_share_memory_are_not_written():
+    """K and V rows of one place would be written at once; reading one cache as both is fine."""
+
+    k, v = torch.randn(2, 3, 2, 64), torch.randn(2, 3, 2, 64)
+    pool, other = (q4.empty_rows(2, 2, 2, 4, channels=64) for _ in range(2))
+    codes, affine = torch.zeros(2 * pool.codes.numel(), dtype=torch.uint8), torch.zeros(2 * pool.affine.numel(), dtype=torch.bfloat16)
+    n, m = pool.codes.numel(), pool.affine.numel()
+    near = q4.Q4Rows(codes[:n].view(pool.codes.shape), affine[:m].view(pool.affine.shape))
+    for same in ((pool, pool), (pool, q4.Q4Rows(pool.codes, other.affine)), (pool, q4.Q4Rows(other.codes, pool.affine)),
+                 (near, q4.Q4Rows(codes[32:n + 32].view(pool.codes.shape), affine[m:].view(pool.affine.shape)))):
+        with pytest.raises(KernelError, match="share memory"):
+            q4.kv_write_paged_q4(k, v, *same)
+    assert not any(t.any() for t in (*pool, *other, codes, affine))
+    q4.kv_write_paged_q4(k, v, near, q4.Q4Rows(codes[n:].view(pool.codes.shape), affine[m:].view(pool.affine.shape)))
+    q4.kv_write_paged_q4(k, v, pool, other)
+    assert torch.equal(near.codes, pool.codes) and torch.equal(codes[n:].view(pool.codes.shape), other.codes)
+    back = q4.kv_read_paged_q4(pool, pool, 3)
+    assert torch.equal(*back)
+    q4.decode_attention_paged_q4(torch.randn(2, 4, 64), pool, pool, torch.tensor([1, 3]))
