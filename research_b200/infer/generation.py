@@ -58,6 +58,15 @@ class PagedKVCache:
         if first < 0 or end > self.max_len:
             raise CacheCapacityError(f"rows {first} .. {end - 1} are not all in a cache of {self.max_len} rows")
 
+    def _same_step(self, layer: int, positions: torch.Tensor):
+        """What another layer made of the same positions in this step, if any: the first layer makes it anew, and so does
+        one whose positions have been written to since."""
+
+        step = getattr(self, "_step_positions", None)
+        if layer == 0 or step is None or step[0] is not positions or step[1] != _version(positions):
+            return None
+        return step
+
     def _pages(self, pool: torch.Tensor, layer: int) -> torch.Tensor:
         # with the identity page table, sequence b owns pages [b * pages_per_seq, (b + 1) * pages_per_seq)
         return pool[layer].view(self.batch, self.pages_per_seq, pool.shape[2], self.page_size, pool.shape[4])
@@ -80,11 +89,11 @@ class PagedKVCache:
 
             # the positions of a step are the same for every layer: the contiguous copy and the lengths are made by
             # the first layer and reused by the others (two launches per step instead of two per layer)
-            step = getattr(self, "_step_positions", None)
-            if layer == 0 or step is None or step[0] is not positions:
+            step = self._same_step(layer, positions)
+            if step is None:
                 pos = positions[:, 0].to(torch.int32).contiguous()
-                step = self._step_positions = (positions, pos, pos + 1)
-            _, pos, lengths = step
+                step = self._step_positions = (positions, _version(positions), pos, pos + 1)
+            _, _, pos, lengths = step
             kv_append_paged(k[:, 0], v[:, 0], kp, vp, pos)
             lo = None if window is None else (pos - (window - 1)).clamp_min(0).to(torch.int32)
             return decode_attention_paged(q[:, 0], kp, vp, lengths, lo)[:, None]
@@ -173,13 +182,13 @@ class QuantizedKVCache(PagedKVCache):
         attend = (quantized.decode_attention_paged_q4 if native_ok or not q.is_cuda
                   else quantized.decode_attention_paged_q4_reference)
         if T == 1:
-            step = getattr(self, "_step_positions", None)       # made by the first layer, reused by the others
-            if layer == 0 or step is None or step[0] is not positions:
+            step = self._same_step(layer, positions)            # made by the first layer, reused by the others
+            if step is None:
                 pos = positions[:, 0].to(torch.int32).contiguous()
                 if not positions.is_cuda and positions.numel():
                     self.require_rows(int(positions.min()), int(positions.max()) + 1)
-                step = self._step_positions = (positions, pos, pos + 1, {None: None})
-            _, pos, lengths, bounds = step
+                step = self._step_positions = (positions, _version(positions), pos, pos + 1, {None: None})
+            _, _, pos, lengths, bounds = step
             if window not in bounds:
                 bounds[window] = (pos - (window - 1)).clamp_min(0)
             write(k, v, kp, vp, pos)
@@ -227,6 +236,12 @@ class QuantizedKVCache(PagedKVCache):
             lo = (at - (window - 1)).clamp_min(0).expand(B, front + T).contiguous()
         o, _ = native.attn_fwd(q, keys, vals, causal=True, lo=lo, q_offset=start - front)
         return o[:, front:].reshape(B, T, Hq * D)
+
+
+def _version(t: torch.Tensor) -> int:
+    """Count of the writes to a tensor (0 for one made in inference mode, which does not count them)."""
+
+    return 0 if t.is_inference() else t._version
 
 
 def _packed_view(t: torch.Tensor) -> bool:

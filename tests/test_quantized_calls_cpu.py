@@ -277,3 +277,22 @@ def test_caches_that_share_memory_are_not_written():
     back = q4.kv_read_paged_q4(pool, pool, 3)
     assert torch.equal(*back)
     q4.decode_attention_paged_q4(torch.randn(2, 4, 64), pool, pool, torch.tensor([1, 3]))
+
+
+# ------------------------------------------------------------------------------------------------- positions in place
+@pytest.mark.parametrize("layer", [0, 1])
+def test_positions_that_change_in_place_are_seen_by_every_layer(layer):
+    """A program's own position buffer, moved on by fill_ between two steps through a part of the layers."""
+
+    torch.manual_seed(0)
+    cache, fresh = (_cache(QuantizedKVCache, layers=2) for _ in range(2))
+    at = torch.zeros(2, 1, dtype=torch.int32)
+    for position in range(5):
+        at.fill_(position)
+        q, k, v = (torch.randn(2, 1, h, 16) for h in (4, 2, 2))
+        got = cache.update_and_attend(layer, q, k, v, at, 3)
+        assert torch.equal(got, fresh.update_and_attend(layer, q, k, v, at.clone(), 3))
+    assert all(torch.equal(a, b) for x, y in ((cache.k, fresh.k), (cache.v, fresh.v)) for a, b in zip(x, y))
+    with torch.inference_mode():
+        got = cache.update_and_attend(0, q, k, v, torch.full((2, 1), 5, dtype=torch.int32), None)
+        assert torch.isfinite(got).all()

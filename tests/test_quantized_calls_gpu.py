@@ -377,3 +377,22 @@ def test_generation_says_when_a_wait_ran_out(bits):
     with pytest.raises(KernelError, match="ran out"):
         call()
     assert call().generated_ids == want and not any(hasattr(p, "q4") for p in model.parameters())
+
+
+# ------------------------------------------------------------------------------------------------- positions in place
+@pytest.mark.parametrize("bits", [4, 16])
+def test_positions_that_change_in_place_are_seen_by_every_layer(bits):
+    from research_b200.infer import QuantizedKVCache
+    from research_b200.infer.generation import PagedKVCache
+
+    kind = QuantizedKVCache if bits == 4 else PagedKVCache
+    cache, fresh = (kind(layers=2, batch=2, max_len=128, kv_heads=2, head_dim=64, page_size=64, dtype=BF16,
+                         device=torch.device("cuda")) for _ in range(2))
+    at = torch.zeros(2, 1, dtype=torch.int32, device="cuda")
+    for position in range(4):
+        at.fill_(position)
+        q, k, v = (torch.randn(2, 1, h, 64, device="cuda", dtype=BF16) for h in (4, 2, 2))
+        got = cache.update_and_attend(1, q, k, v, at, None)
+        assert torch.equal(got, fresh.update_and_attend(1, q, k, v, at.clone(), None))
+    pools = [[t for pool in (c.k, c.v) for t in (pool if bits == 4 else [pool])] for c in (cache, fresh)]
+    assert all(torch.equal(a, b) for a, b in zip(*pools))
